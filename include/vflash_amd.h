@@ -432,6 +432,38 @@ int vflash_nvfp4_w4a4_linear(const void* a, int64_t lda, const void* a_scales, c
                              const void* w_scales, const float* alpha, int64_t m, int64_t n,
                              int64_t k, const void* bias, void* out, int64_t ldo, void* stream);
 
+/*
+ * Packed attention: softmax(scale q k^T) v for sequences that lie one after another, with grouped
+ * heads (query head h reads key head h / (heads / key_heads)).  No reference counterpart: the
+ * reference's attention is a torch call.
+ *   q    bf16 (f16 when f16) [tokens, heads, dim], element (t, h, d) at t * q_ts + h * q_hs + d
+ *   k, v the same type, [keys, key_heads, dim] with their own strides (0 allowed)
+ *   q_offsets int64 [batch + 1]: sequence b has the queries q_offsets[b] .. q_offsets[b + 1] - 1
+ *   k_offsets int64: its keys begin at row k_offsets[b] and end before k_offsets[b + 1]
+ *             (then batch + 1 values), or, with k_lengths int64 [batch], are k_lengths[b] rows
+ *             (then batch values): a cache with room past each sequence, which is not read
+ *   causal    query i of a sequence of nq queries and nk keys sees the keys j <= i + nk - nq
+ *   out  [tokens, heads, dim] of the same type, elements at t * o_ts + h * o_hs + d.  Rows that see no key, and
+ *        rows outside every sequence, are zeros.  Scores, softmax and sums are binary32;
+ *        probabilities are rounded to the operands' type for their product with v.
+ * Offsets and lengths are read on the device and clamped to the operands: values that decrease or
+ * overlap give unspecified results, but nothing outside the operands is read or written.  A
+ * masked key has no effect through k; its v enters with weight 0 if it lies in its sequence (0
+ * times an infinity is NaN).
+ *   workspace  vflash_packed_attention_workspace(...) bytes (0: may be NULL), 16-byte aligned,
+ *              without contents to keep; one call at a time
+ *   Requires dim % 8 == 0, 8 <= dim <= 128, every stride a multiple of 8 and the pointers 16-byte
+ *   aligned, k_ts and v_ts < 2^23, tokens and keys < 2^31, scale positive and finite.
+ */
+int64_t vflash_packed_attention_workspace(int64_t tokens, int64_t keys, int64_t batch, int64_t heads,
+                                          int64_t key_heads, int64_t dim);
+int vflash_packed_attention(const void* q, int64_t q_ts, int64_t q_hs, const void* k, int64_t k_ts, int64_t k_hs,
+                            const void* v, int64_t v_ts, int64_t v_hs, int f16, int64_t tokens, int64_t keys,
+                            int64_t heads, int64_t key_heads, int64_t dim, const int64_t* q_offsets,
+                            const int64_t* k_offsets, const int64_t* k_lengths, int64_t batch, int causal,
+                            float scale, void* out, int64_t o_ts, int64_t o_hs, void* workspace,
+                            int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,221 @@
+"""Packed attention on the GPU against its definition in 64 bits."""
+
+import pytest
+import torch
+
+from tests.attention_reference import check
+from vflash_amd.attention import packed_attention
+
+pytestmark = pytest.mark.gpu
+BF16, F16 = torch.bfloat16, torch.float16
+
+
+def offsets(lengths, dev):
+    return torch.tensor([sum(lengths[:i]) for i in range(len(lengths) + 1)], dtype=torch.int64, device=dev)
+
+
+def make(dev, nq, nk, heads, kv, dim, dtype, seed=0, std=2.0):
+    g = torch.Generator(device=dev).manual_seed(seed)
+    q = (torch.randn(sum(nq), heads, dim, generator=g, device=dev) * std).to(dtype)
+    k, v = (torch.randn(sum(nk), kv, dim, generator=g, device=dev).to(dtype) for _ in range(2))
+    return q, k, v
+
+
+LENGTHS = [
+    ([1], [1]), ([1], [77]), ([1, 1, 1], [31, 32, 33]), ([1] * 5, [0, 1, 127, 129, 2000]), ([1], [5000]),
+    ([2, 3], [300, 1]), ([5], [5]), ([64], [64]), ([63, 65], [63, 65]), ([0, 200, 0, 1, 129], [0, 200, 7, 1, 129]),
+    ([100], [300]), ([40], [17]), ([130, 33], [0, 500]), ([300], [1100]), ([1, 700], [900, 700]),
+]
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("heads,kv,dim,dtype", [(8, 2, 128, BF16), (3, 3, 64, F16), (7, 1, 96, BF16), (10, 2, 80, F16)])
+@pytest.mark.parametrize("nq,nk", LENGTHS, ids=lambda v: "-".join(map(str, v)))
+def test_lengths(dev, nq, nk, heads, kv, dim, dtype, causal):
+    q, k, v = make(dev, nq, nk, heads, kv, dim, dtype)
+    qo, ko = offsets(nq, dev), offsets(nk, dev)
+    check(packed_attention(q, k, v, qo, ko, causal=causal), q, k, v, qo, ko, causal=causal)
+
+
+@pytest.mark.parametrize("dim", [8, 16, 24, 32, 40, 56, 72, 88, 104, 112, 120])
+@pytest.mark.parametrize("nq,nk", [([1, 1], [45, 200]), ([70], [130])])
+def test_head_dimensions(dev, dim, nq, nk):
+    for dtype in (BF16, F16):
+        q, k, v = make(dev, nq, nk, 4, 2, dim, dtype)
+        qo, ko = offsets(nq, dev), offsets(nk, dev)
+        check(packed_attention(q, k, v, qo, ko, causal=True), q, k, v, qo, ko, causal=True)
+
+
+@pytest.mark.parametrize("heads,kv", [(1, 1), (16, 1), (17, 1), (40, 1), (71, 1), (150, 1), (16, 16), (24, 8), (5, 5)])
+@pytest.mark.parametrize("nq,nk", [([1, 1, 1], [3, 400, 90]), ([37], [150])])
+def test_groups(dev, heads, kv, nq, nk):
+    q, k, v = make(dev, nq, nk, heads, kv, 64, BF16)
+    qo, ko = offsets(nq, dev), offsets(nk, dev)
+    check(packed_attention(q, k, v, qo, ko, causal=True), q, k, v, qo, ko, causal=True)
+
+
+@pytest.mark.parametrize("nq", [1, 3, 90])
+def test_cache_with_room(dev, nq):
+    # What lies past a sequence's keys (infinities, NaN) is another's; nothing of it may show.
+    lengths, room = [1, 64, 200, 0, 777], 800
+    for heads, kv, dim in ((8, 2, 128), (4, 4, 64)):
+        q, k, v = make(dev, [nq] * 5, [room] * 5, heads, kv, dim, BF16)
+        for i, n in enumerate(lengths):
+            k[i * room + n:(i + 1) * room] = torch.inf
+            v[i * room + n:(i + 1) * room] = torch.nan
+        qo = offsets([nq] * 5, dev)
+        ko = torch.arange(5, device=dev) * room
+        kl = torch.tensor(lengths, device=dev)
+        for causal in (False, True):
+            got = packed_attention(q, k, v, qo, ko, k_lengths=kl, causal=causal)
+            check(got, q, k, v, qo, ko, k_lengths=kl, causal=causal)
+        # Sequences may share rows.
+        ko = torch.zeros(5, dtype=torch.int64, device=dev)
+        kl = torch.ones(5, dtype=torch.int64, device=dev)
+        check(packed_attention(q, k, v, qo, ko, k_lengths=kl), q, k, v, qo, ko, k_lengths=kl)
+
+
+def test_masked_keys_have_no_weight(dev):
+    # Keys that no query sees, or that later queries see, hold infinities and NaN.
+    q, k, v = make(dev, [50], [50], 4, 2, 64, BF16)
+    qo = offsets([50], dev)
+    want = packed_attention(q, k, v, qo, qo, causal=True)
+    k[30:] = torch.nan
+    got = packed_attention(q, k, v, qo, qo, causal=True)
+    assert torch.equal(got[:30], want[:30]) and bool(torch.isnan(got[30:]).all())
+
+
+def test_rows_outside_every_sequence_are_zeros(dev):
+    q, k, v = make(dev, [400], [300], 8, 2, 128, BF16)
+    for nq in ([13, 200], [1, 1]):
+        qo = torch.tensor([7, 7 + nq[0], 7 + nq[0] + nq[1]], device=dev)
+        ko = torch.tensor([0, 100, 300], device=dev)
+        got = packed_attention(q, k, v, qo, ko)
+        check(got, q, k, v, qo, ko)
+        assert not got[:7].any() and not got[7 + sum(nq):].any()
+
+
+@pytest.mark.parametrize("qo,ko,kl", [
+    ([0, -5, 1 << 40], [0, 50, 1 << 40], None), ([0, 60, 30], [-9, 1 << 62, -(1 << 62)], None),
+    ([50, 0, 90], [400, 3], [1 << 50, -1]), ([-(1 << 63), 0, (1 << 63) - 1], [299, -4], [5, 1 << 33]),
+])
+def test_bad_offsets_stay_inside(dev, qo, ko, kl):
+    q, k, v = make(dev, [90], [300], 4, 2, 64, BF16)
+    t = lambda x: None if x is None else torch.tensor(x, dtype=torch.int64, device=dev)
+    got = packed_attention(q, k, v, t(qo), t(ko), k_lengths=t(kl), causal=True)
+    torch.cuda.synchronize()
+    assert got.shape == q.shape
+
+
+@pytest.mark.parametrize("layout", ["merged", "heads first", "expanded", "odd strides", "offset"])
+@pytest.mark.parametrize("nq", [1, 150])
+def test_layouts(dev, layout, nq):
+    n, heads, kv, dim = 3, 8, 2, 64
+    q, k, v = make(dev, [nq] * n, [nq] * n, heads, kv, dim, F16)
+    t = nq * n
+    if layout == "merged":
+        q, k, v = torch.cat((q, k, v), 1).split((heads, kv, kv), 1)
+    elif layout == "heads first":
+        q, k, v = (x.transpose(0, 1).contiguous().transpose(0, 1) for x in (q, k, v))
+    elif layout == "expanded":
+        k, v = k[:1].expand(t, kv, dim), v[:, :1].expand(t, kv, dim)
+    elif layout == "odd strides":
+        q, k, v = (torch.nn.functional.pad(x, (0, 3))[..., :dim] for x in (q, k, v))
+    else:
+        q, k, v = (torch.cat((x.reshape(-1)[:3], x.reshape(-1)))[3:].view(x.shape) for x in (q, k, v))
+    qo = offsets([nq] * n, dev)
+    check(packed_attention(q, k, v, qo, qo, causal=True), q, k, v, qo, qo, causal=True)
+
+
+def test_scale_and_large_scores(dev):
+    q, k, v = make(dev, [1, 70], [600, 70], 4, 2, 128, BF16, std=30.0)
+    qo, ko = offsets([1, 70], dev), offsets([600, 70], dev)
+    for scale in (1e-6, 0.03, 1.0):
+        check(packed_attention(q, k, v, qo, ko, scale=scale), q, k, v, qo, ko, scale=scale)
+    # Exponents past binary32's range: the largest score's value alone.
+    q = torch.full((1, 1, 64), 1e18, device=dev, dtype=BF16)
+    k = torch.ones((200, 1, 64), device=dev, dtype=BF16) * -1.0
+    k[123] = -0.5
+    v = torch.randn((200, 1, 64), device=dev).to(BF16)
+    got = packed_attention(q, k, v, offsets([1], dev), offsets([200], dev))
+    assert torch.equal(got[0], v[123])
+
+
+def test_binary16_keeps_small_probabilities(dev):
+    # One score 17 above 60000 equal ones: each of these weighs 2^-24.5, together 2.5e-3.
+    n = 60000
+    q = torch.zeros((1, 1, 64), device=dev, dtype=F16)
+    q[..., 0] = 1.0
+    k = torch.zeros((n, 1, 64), device=dev, dtype=F16)
+    k[4, 0, 0] = 17.0
+    v = torch.ones((n, 1, 64), device=dev, dtype=F16)
+    v[4] = 0
+    qo, ko = offsets([1], dev), offsets([n], dev)
+    check(packed_attention(q, k, v, qo, ko, scale=1.0), q, k, v, qo, ko, scale=1.0)
+
+
+def test_many_sequences(dev):
+    # More sequences than a wave has lanes, long ones among short.
+    g = torch.Generator().manual_seed(3)
+    for nq in ([1] * 200, torch.randint(0, 40, (150,), generator=g).tolist()):
+        nk = [n + (2000 if i % 50 == 7 else i % 9) for i, n in enumerate(nq)]
+        q, k, v = make(dev, nq, nk, 4, 2, 64, BF16)
+        qo, ko = offsets(nq, dev), offsets(nk, dev)
+        check(packed_attention(q, k, v, qo, ko, causal=True), q, k, v, qo, ko, causal=True)
+
+
+def test_cache_past_32_bit_offsets(dev):
+    rows, kv, dim = (1 << 31) // 256 + 5000, 2, 128  # elements pass 2^31 before the last rows
+    k = torch.empty((rows, kv, dim), device=dev, dtype=BF16)
+    v = torch.empty_like(k)
+    for nq in (1, 40):
+        q, k[-3000:], v[-3000:] = make(dev, [nq], [3000], 4, kv, dim, BF16)
+        qo = offsets([nq], dev)
+        got = packed_attention(q, k, v, qo, torch.tensor([rows - 3000], device=dev),
+                               k_lengths=torch.tensor([3000], device=dev), causal=True)
+        check(got, q, k[-3000:], v[-3000:], qo, torch.tensor([0, 3000]), causal=True)
+
+
+def test_repeated_calls_and_other_streams_agree(dev):
+    for nq, nk in (([1] * 3, [5000, 20, 900]), ([300, 4], [4000, 4])):
+        q, k, v = make(dev, nq, nk, 8, 2, 128, BF16)
+        qo, ko = offsets(nq, dev), offsets(nk, dev)
+        want = packed_attention(q, k, v, qo, ko, causal=True)
+        side = torch.cuda.Stream(dev)
+        side.wait_stream(torch.cuda.current_stream(dev))
+        with torch.cuda.stream(side):
+            got = packed_attention(q, k, v, qo, ko, causal=True)
+        torch.cuda.current_stream(dev).wait_stream(side)
+        assert torch.equal(got, want)
+        for _ in range(5):
+            assert torch.equal(packed_attention(q, k, v, qo, ko, causal=True), want)
+
+
+def test_graph_replays_other_lengths(dev):
+    # The lengths are read on the device: a captured call serves others.
+    q, k, v = make(dev, [1] * 4, [1000] * 4, 8, 2, 128, BF16)
+    qo, ko = offsets([1] * 4, dev), torch.arange(4, device=dev) * 1000
+    kl = torch.tensor([1000, 1, 30, 500], device=dev)
+    side = torch.cuda.Stream(dev)
+    side.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(side):
+        packed_attention(q, k, v, qo, ko, k_lengths=kl)
+    torch.cuda.current_stream(dev).wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = packed_attention(q, k, v, qo, ko, k_lengths=kl)
+    for lengths in ([1000, 1, 30, 500], [3, 999, 0, 64], [1000] * 4):
+        kl.copy_(torch.tensor(lengths, device=dev))
+        q.normal_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, packed_attention(q, k, v, qo, ko, k_lengths=kl))
+
+
+def test_no_rows(dev):
+    q, k, v = make(dev, [0], [9], 4, 2, 64, BF16)
+    zero = torch.zeros(2, dtype=torch.int64, device=dev)
+    assert packed_attention(q, k, v, zero, zero).shape == (0, 4, 64)
+    q, k, v = make(dev, [5], [0], 4, 2, 64, BF16)
+    assert not packed_attention(q, k, v, offsets([5], dev), zero).any()
+    assert not packed_attention(q, k, v, zero[:1], zero[:1]).any()  # no sequence at all

@@ -99,6 +99,12 @@ SIGNATURES: dict[str, tuple[list, object]] = {
         [_P, _I32, _I64, _I64, _I64, _P, _P, _I64, _P, _I64, _P, _P, _P],
         _I32,
     ),
+    "vflash_packed_attention_workspace": ([_I64, _I64, _I64, _I64, _I64, _I64], _I64),
+    "vflash_packed_attention": (
+        [_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I32, _I64, _I64, _I64, _I64, _I64, _P, _P, _P,
+         _I64, _I32, _F32, _P, _I64, _I64, _P, _I64, _P],
+        _I32,
+    ),
     "vflash_nvfp4_w4a4_linear": (
         [_P, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _P, _P, _I64, _P],
         _I32,

@@ -1,0 +1,204 @@
+// Packed attention for gfx950: tiles of up to 16 rows (a token or a few per sequence).
+//
+// Bound by the bytes of K and V, each read once per key head.  The products are those of
+// attention.hip with v_mfma_f32_16x16x32: S^T = K Q^T for 16 keys at a time, O^T = V^T P^T for 32,
+// where K position (lane row g, j) stands for key 4 g + j of the first 16 keys (j < 4) or
+// 4 g + j - 4 of the second, which is where the scores lie.
+//
+// Each wave takes every fourth block of 32 keys of the item and keeps a ring of two in LDS, which
+// its own DMA fills: 128 KB a CU in flight or in use, no barrier before the end, where the four
+// waves' sums are added up.
+#include "attention.h"
+
+namespace vfa {
+
+template <int DP>
+struct AttentionSteps {
+  static constexpr int PITCH = DP <= 64 ? 128 : 256, CHUNKS = PITCH / 16, ROWS = 1024 / PITCH;
+  static constexpr int KEYS = 32, TILE = KEYS * PITCH, SLOT = 2 * TILE, NS = 2, WAVES = 4;
+  static constexpr int DMA = SLOT / 1024;  // instructions per stage
+  static constexpr int ACC = DP * 4 + 16;  // bytes of a row's sums in LDS
+};
+template <int PITCH>
+__device__ __forceinline__ int step_k_swizzle(int r) {
+  return PITCH == 256 ? r & 15 : lds_swizzle(r);
+}
+// Eight rows x two chunks of a half wave's transposing read take different slots.
+template <int PITCH>
+__device__ __forceinline__ int step_v_swizzle(int r) {
+  return PITCH == 256 ? (r & 7) << 1 : (r >> 1 & 3) << 1;
+}
+
+template <bool F16, int DP>
+__global__ void __launch_bounds__(256, 1) attention_step(const AttentionParams p) {
+  using L = AttentionSteps<DP>;
+  constexpr int QS = (DP + 31) / 32, DB = DP / 16;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[L::WAVES * L::NS * L::SLOT];
+  __shared__ float stat[L::WAVES][16][2];
+  static_assert(L::WAVES * 16 * L::ACC <= L::WAVES * L::NS * L::SLOT && (L::NS - 1) * L::DMA < 64, "LDS, vmcnt");
+  const AttentionItem it = attention_item<false>(p, blockIdx.x);
+  if (!it.live) return;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int lane = (int)threadIdx.x & 63;
+  const int fr = lane & 15, fg = lane >> 4;
+  uint8_t* ring = lds + wave * (L::NS * L::SLOT);
+  const uint32_t ring_lds = __builtin_amdgcn_readfirstlane(lds_addr(ring));
+
+  const AttentionRow row = attention_row(p, it, fr);
+  const int key_head = it.head_block / p.parts;
+  const int last_token = min(it.seq.nq, (it.tile + 1) * p.tile_tokens) - 1;
+  const int tile_limit = attention_limit(p, it.seq, last_token);
+  const int first = it.split * it.chunk;
+  const int last = (int)min((int64_t)tile_limit, (int64_t)first + it.chunk);
+  const int limit = row.live ? min(attention_limit(p, it.seq, row.token), last) : last;
+  // Keys that every row sees.
+  const int open = min(attention_limit(p, it.seq, min(it.tile * p.tile_tokens, it.seq.nq)), last);
+
+  const uint8_t* kb = reinterpret_cast<const uint8_t*>(p.k + (int64_t)it.seq.k0 * p.k_ts + (int64_t)key_head * p.k_hs);
+  const uint8_t* vb = reinterpret_cast<const uint8_t*>(p.v + (int64_t)it.seq.k0 * p.v_ts + (int64_t)key_head * p.v_hs);
+  const uint32_t kts = (uint32_t)p.k_ts * 2, vts = (uint32_t)p.v_ts * 2;
+  const int drow = lane / L::CHUNKS, dslot = lane % L::CHUNKS;
+  auto issue = [&](int buf, int key0) {
+    const int left = last - key0;  // none: every lane reads zeros
+    const __amdgpu_buffer_rsrc_t rk = make_rsrc(kb + (int64_t)key0 * kts, 0x7fffffffu);
+    const __amdgpu_buffer_rsrc_t rv = make_rsrc(vb + (int64_t)key0 * vts, 0x7fffffffu);
+    const uint32_t dst = ring_lds + buf * L::SLOT;
+    static_for<L::DMA / 2>([&](auto i) {
+      const int r = drow + i * L::ROWS;
+      const int c = dslot ^ step_k_swizzle<L::PITCH>(r);
+      lds_dma16(rk, dst + i * 1024, r < left && c * 8 < p.dim ? (uint32_t)r * kts + c * 16 : VFA_OOB);
+    });
+    static_for<L::DMA / 2>([&](auto i) {
+      const int r = drow + i * L::ROWS;
+      const int c = dslot ^ step_v_swizzle<L::PITCH>(r);
+      lds_dma16(rv, dst + L::TILE + i * 1024, r < left && c * 8 < p.dim ? (uint32_t)r * vts + c * 16 : VFA_OOB);
+    });
+  };
+  constexpr int STRIDE = L::WAVES * L::KEYS;
+  const int start = first + wave * L::KEYS;
+  static_for<L::NS>([&](auto i) { issue(i, start + i * STRIDE); });
+
+  v4i q[QS];
+  {
+    const uint16_t* src = p.q + (int64_t)(it.seq.q0 + row.token) * p.q_ts + (int64_t)row.head * p.q_hs;
+    static_for<QS>([&](auto s) {
+      const int d = s * 32 + fg * 8;
+      q[s] = row.live && d < p.dim ? *reinterpret_cast<const v4i*>(src + d) : v4i{};
+    });
+  }
+  v4f o[DB];
+  static_for<DB>([&](auto i) { o[i] = v4f{}; });
+  float m = VFA_LOWEST, l = 0;
+  bool far = false;
+  const uint8_t* krow = ring + fr * L::PITCH;
+  const int ksw = step_k_swizzle<L::PITCH>(fr);
+  const int vr = 4 * fg + ((lane >> 2) & 3);
+  const int vc = (lane & 3) >> 1;
+  const uint8_t* vrow = ring + L::TILE + vr * L::PITCH + (lane & 1) * 8;
+  const int vsw = step_v_swizzle<L::PITCH>(vr);
+
+  int buf = 0;
+  for (int key0 = start; key0 < last; key0 += STRIDE, buf = buf + 1 == L::NS ? 0 : buf + 1) {
+    wait_vmcnt<(L::NS - 1) * L::DMA, false>();
+    asm volatile("" ::: "memory");
+    v4f s[2];
+    static_for<2>([&](auto kbk) {
+      s[kbk] = v4f{};
+      static_for<QS>([&](auto st) {
+        const v4i a = *reinterpret_cast<const v4i*>(krow + buf * L::SLOT + kbk * 16 * L::PITCH +
+                                                    (((4 * st + fg) ^ ksw) << 4));
+        s[kbk] = mfma16<F16>(a, q[st], s[kbk]);
+      });
+    });
+    if (key0 + L::KEYS > open) {
+      const int lim = limit - key0 - 4 * fg;
+      static_for<2>([&](auto kbk) {
+        static_for<4>([&](auto r) { s[kbk][(int)r] = kbk * 16 + r < lim ? s[kbk][(int)r] : -__builtin_inff(); });
+      });
+    }
+    float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                     fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+    mx = max_across32(max_across16(mx));
+    if (__builtin_amdgcn_ballot_w64(mx * p.c > m * p.c + kAttentionSlack)) {
+      const float next = fmaxf(m, mx), f = __builtin_amdgcn_exp2f((m - next) * p.c);
+      static_for<DB>([&](auto i) { static_for<4>([&](auto r) { o[i][(int)r] *= f; }); });
+      l *= f;
+      m = next;
+      far = __builtin_amdgcn_ballot_w64(fabsf(m * p.c) >= kAttentionFar && m > VFA_LOWEST) != 0;
+    }
+    const float ref = kAttentionShift<F16> - m * p.c;
+    v4i pk;
+    auto weights = [&](auto far_rows) {
+      static_for<4>([&](auto j) {
+        constexpr int r = (j % 2) * 2;
+        const float a = attention_weight<F16, far_rows>(s[j / 2][r], p.c, m, ref);
+        const float b = attention_weight<F16, far_rows>(s[j / 2][r + 1], p.c, m, ref);
+        l += a;
+        l += b;
+        pk[(int)j] = pack2<F16>(a, b);
+      });
+    };
+    if (far) weights(std::true_type{});
+    else weights(std::false_type{});
+    static_for<DB>([&](auto db) {
+      const uint8_t* src = vrow + buf * L::SLOT + (((2 * db + vc) ^ vsw) << 4);
+      const v2i lo = lds_read_tr16(src), hi = lds_read_tr16(src + 16 * L::PITCH);
+      o[db] = mfma16<F16>(v4i{lo[0], lo[1], hi[0], hi[1]}, pk, o[db]);
+    });
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the slot is read
+    asm volatile("" ::: "memory");
+    issue(buf, key0 + L::NS * STRIDE);
+  }
+  l = sum_across32(sum_across16(l));
+  wait_vmcnt<0, true>();
+  asm volatile("" ::: "memory");
+  __syncthreads();  // every ring is done with
+  static_for<DB>([&](auto db) {
+    *reinterpret_cast<v4f*>(lds + (wave * 16 + fr) * L::ACC + (db * 16 + 4 * fg) * 4) = o[db];
+  });
+  if (fg == 0) {
+    stat[wave][fr][0] = attention_top(m, p.c);
+    stat[wave][fr][1] = l;
+  }
+  __syncthreads();
+  // Thread t: row t / 16, the d of t % 16 in runs of four.
+  const int r = (int)threadIdx.x >> 4, e = (int)threadIdx.x & 15;
+  const AttentionRow mine = attention_row(p, it, r);
+  if (!mine.live) return;
+  float top = stat[0][r][0], sum = 0, f[L::WAVES];
+  static_for<L::WAVES - 1>([&](auto w) { top = fmaxf(top, stat[w + 1][r][0]); });
+  static_for<L::WAVES>([&](auto w) {
+    f[w] = __builtin_amdgcn_exp2f(stat[w][r][0] - top);
+    sum += f[w] * stat[w][r][1];
+  });
+  const bool split = it.splits > 1;
+  if (split && first >= tile_limit) return;  // attention_join does not read it
+  const int64_t at = (int64_t)(it.slot + it.split) * 16 + r;
+  if (split && e == 0) *reinterpret_cast<v2f*>(p.part_ml + at * 2) = v2f{top, sum};
+  const float inv = split ? 1.0f : 1.0f / sum;
+  uint16_t* dst = p.out + (int64_t)(it.seq.q0 + mine.token) * p.o_ts + (int64_t)mine.head * p.o_hs;
+  for (int d = 4 * e; d < p.dim; d += 64) {
+    v4f x = v4f{};
+    static_for<L::WAVES>([&](auto w) { x += *reinterpret_cast<const v4f*>(lds + (w * 16 + r) * L::ACC + d * 4) * f[w]; });
+    x = sum == 0 ? v4f{} : x * inv;
+    if (split) {
+      *reinterpret_cast<v4f*>(p.part + at * p.dim + d) = x;
+    } else {
+      typedef int v2i_ __attribute__((ext_vector_type(2)));
+      *reinterpret_cast<v2i_*>(dst + d) = v2i_{pack2<F16>(x[0], x[1]), pack2<F16>(x[2], x[3])};
+    }
+  }
+}
+
+void launch_attention_step(const AttentionParams& p, bool f16, int64_t grid, hipStream_t s) {
+  const dim3 g((unsigned)grid), b(256);
+  if (p.dim <= 64) {
+    if (f16) attention_step<true, 64><<<g, b, 0, s>>>(p);
+    else attention_step<false, 64><<<g, b, 0, s>>>(p);
+  } else {
+    if (f16) attention_step<true, 128><<<g, b, 0, s>>>(p);
+    else attention_step<false, 128><<<g, b, 0, s>>>(p);
+  }
+}
+
+}  // namespace vfa

@@ -7,6 +7,7 @@
 #include <hip/hip_runtime.h>
 
 #include "../../include/vflash_amd.h"
+#include "attention_params.h"
 #include "common.h"
 #include "gemm_params.h"
 
@@ -35,6 +36,9 @@ hipError_t launch_restore_rows(const uint8_t*, const float*, int64_t, int64_t, i
 hipError_t launch_nvfp4(const uint8_t*, const float*, int64_t, const uint8_t*, const uint8_t*,
                         const float*, int64_t, int64_t, int64_t, const uint16_t*, uint16_t*, int64_t,
                         int, hipStream_t);
+int64_t attention_workspace(const AttentionParams&);
+bool attention_fits(const AttentionParams&);
+hipError_t launch_attention(const AttentionParams&, bool, void*, hipStream_t);
 }  // namespace vfa
 
 namespace {
@@ -137,6 +141,22 @@ bool out_args_ok(const void* out, int64_t ldo, int64_t m, int64_t n, int64_t pla
   if (plane_cols < 16 || plane_cols % 16 || n % plane_cols) return false;
   if (ldo < plane_cols || plane_stride % 4) return false;
   return plane_stride >= (m - 1) * ldo + plane_cols;  // planes may not overlap
+}
+
+// Sizes of a packed attention call.
+bool attention_sizes(vfa::AttentionParams& p, int64_t tokens, int64_t keys, int64_t batch, int64_t heads,
+                     int64_t key_heads, int64_t dim) {
+  constexpr int64_t LIMIT = int64_t(1) << 31;
+  if (tokens < 1 || tokens >= LIMIT || keys < 0 || keys >= LIMIT || batch < 0 || batch >= LIMIT) return false;
+  if (key_heads < 1 || heads < key_heads || heads % key_heads || heads >= LIMIT / 2) return false;
+  if (dim < 8 || dim > 128 || dim % 8) return false;
+  p.tokens = (int)tokens;
+  p.keys = (int)keys;
+  p.batch = batch;
+  p.heads = (int)heads;
+  p.group = (int)(heads / key_heads);
+  p.dim = (int)dim;
+  return vfa::attention_fits(p);
 }
 
 }  // namespace
@@ -466,6 +486,54 @@ int vflash_nvfp4_w4a4_linear(const void* a, int64_t lda, const void* a_scales, c
       static_cast<const uint8_t*>(w_packed), static_cast<const uint8_t*>(w_scales), alpha, m, n, k,
       static_cast<const uint16_t*>(bias), static_cast<uint16_t*>(out), ldo, FP4_GROUP_M,
       static_cast<hipStream_t>(stream)));
+}
+
+int64_t vflash_packed_attention_workspace(int64_t tokens, int64_t keys, int64_t batch, int64_t heads,
+                                          int64_t key_heads, int64_t dim) {
+  vfa::AttentionParams p{};
+  if (!attention_sizes(p, tokens, keys, batch, heads, key_heads, dim)) return VFLASH_EINVAL;
+  return vfa::attention_workspace(p);
+}
+
+int vflash_packed_attention(const void* q, int64_t q_ts, int64_t q_hs, const void* k, int64_t k_ts, int64_t k_hs,
+                            const void* v, int64_t v_ts, int64_t v_hs, int f16, int64_t tokens, int64_t keys,
+                            int64_t heads, int64_t key_heads, int64_t dim, const int64_t* q_offsets,
+                            const int64_t* k_offsets, const int64_t* k_lengths, int64_t batch, int causal,
+                            float scale, void* out, int64_t o_ts, int64_t o_hs, void* workspace,
+                            int64_t workspace_bytes, void* stream) {
+  vfa::AttentionParams p{};
+  if (!attention_sizes(p, tokens, keys, batch, heads, key_heads, dim)) return VFLASH_EINVAL;
+  if (!q || !out || !q_offsets || !aligned(q_offsets, 8) || !aligned(k_offsets, 8) || !aligned(k_lengths, 8))
+    return VFLASH_EINVAL;
+  if ((keys && (!k || !v)) || (batch && !k_offsets)) return VFLASH_EINVAL;
+  if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 16)) return VFLASH_EINVAL;
+  for (int64_t stride : {q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, o_ts, o_hs})
+    if (stride < 0 || stride % 8) return VFLASH_EINVAL;
+  // Offsets inside a block of 64 keys must stay below 2^31 bytes; an output element has one place.
+  if (k_ts >= (int64_t(1) << 23) || v_ts >= (int64_t(1) << 23)) return VFLASH_EINVAL;
+  if (!(o_hs >= dim && o_ts >= (heads - 1) * o_hs + dim) && !(o_ts >= dim && o_hs >= (tokens - 1) * o_ts + dim))
+    return VFLASH_EINVAL;
+  if (!(scale > 0.0f) || scale > 3.4e38f) return VFLASH_EINVAL;  // rejects NaN and infinity
+  const int64_t need = vfa::attention_workspace(p);
+  if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16))) return VFLASH_EINVAL;
+  p.q = static_cast<const uint16_t*>(q);
+  p.k = static_cast<const uint16_t*>(k);
+  p.v = static_cast<const uint16_t*>(v);
+  p.out = static_cast<uint16_t*>(out);
+  p.q_ts = q_ts;
+  p.q_hs = q_hs;
+  p.k_ts = k_ts;
+  p.k_hs = k_hs;
+  p.v_ts = v_ts;
+  p.v_hs = v_hs;
+  p.o_ts = o_ts;
+  p.o_hs = o_hs;
+  p.q_offsets = q_offsets;
+  p.k_offsets = k_offsets;
+  p.k_lengths = k_lengths;
+  p.causal = causal != 0;
+  p.c = scale * 1.4426950408889634f;
+  return status(vfa::launch_attention(p, f16 != 0, workspace, static_cast<hipStream_t>(stream)));
 }
 
 }  // extern "C"

@@ -656,3 +656,34 @@ def nvfp4_w4a4_gemm(codes, act_scales, packed, block_scales, alpha, rows, bias=N
              ptr(block_scales), ptr(alpha), rows, n, k, ptr(bias), ptr(out), out.stride(0),
              stream_of(device))
     return out
+
+
+def _attention_rows(t):
+    """``t`` [rows, heads, dim] as the attention kernels read it: unit stride in d, other
+    strides multiples of 8, 16-byte aligned; copied where it is not."""
+    if (t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16
+            or t.stride(0) >= 1 << 23):
+        return t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def packed_attention(q, k, v, q_offsets, k_offsets, k_lengths, causal, scale):
+    """softmax(scale q k^T) v over packed sequences (operands as ``attention.packed_attention``
+    checks them)."""
+    device = require_device(q, k, v, q_offsets, k_offsets, k_lengths)
+    q, k, v = _attention_rows(q), _attention_rows(k), _attention_rows(v)
+    tokens, heads, dim = q.shape
+    keys, key_heads = k.shape[:2]
+    batch = q_offsets.numel() - 1
+    out = torch.empty((tokens, heads, dim), device=device, dtype=q.dtype)
+    if not tokens:
+        return out
+    size = _lib.library().vflash_packed_attention_workspace(tokens, keys, batch, heads, key_heads, dim)
+    if size < 0:
+        raise ValueError("packed attention: more rows than a call takes")
+    workspace = torch.empty(size, device=device, dtype=torch.uint8) if size else None
+    call("vflash_packed_attention", ptr(q), q.stride(0), q.stride(1), ptr(k), k.stride(0), k.stride(1),
+         ptr(v), v.stride(0), v.stride(1), int(q.dtype == torch.float16), tokens, keys, heads, key_heads, dim,
+         ptr(q_offsets), ptr(k_offsets), ptr(k_lengths), batch, int(causal), scale, ptr(out), out.stride(0),
+         out.stride(1), ptr(workspace), size, stream_of(device))
+    return out
