@@ -433,6 +433,20 @@ int vflash_nvfp4_w4a4_linear(const void* a, int64_t lda, const void* a_scales, c
                              int64_t k, const void* bias, void* out, int64_t ldo, void* stream);
 
 /*
+ * NVFP4-weight linear with unquantized activations (weight-only).  No reference counterpart: the
+ * reference's module always quantizes its activations.
+ *   x        bf16 [m, k] (f16 when x_is_f16), row stride ldx
+ *   w_packed, w_scales, alpha, bias, out as vflash_nvfp4_linear
+ *   out = bf16(alpha * sum_k x * e2m1(w) * e4m3(s_blk) + bias[n]); the products' weight factors are
+ *   exact, the sum and the last two operations are binary32, with one rounding to bf16
+ *   Requires n % 128 == 0, k % 64 == 0, ldx % 8 == 0, ldo % 8 == 0, 512 ldx and 128 k < 2^31, n < 2^25,
+ *   and x, w_packed, w_scales, bias and out 16-byte aligned.
+ */
+int vflash_nvfp4_w16_linear(const void* x, int x_is_f16, int64_t ldx, const void* w_packed, const void* w_scales,
+                            const float* alpha, int64_t m, int64_t n, int64_t k, const void* bias, void* out,
+                            int64_t ldo, void* stream);
+
+/*
  * Packed attention: softmax(scale q k^T) v for sequences that lie one after another, with grouped
  * heads (query head h reads key head h / (heads / key_heads)).  No reference counterpart: the
  * reference's attention is a torch call.

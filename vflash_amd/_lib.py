@@ -99,6 +99,10 @@ SIGNATURES: dict[str, tuple[list, object]] = {
         [_P, _I32, _I64, _I64, _I64, _P, _P, _I64, _P, _I64, _P, _P, _P],
         _I32,
     ),
+    "vflash_nvfp4_w16_linear": (
+        [_P, _I32, _I64, _P, _P, _P, _I64, _I64, _I64, _P, _P, _I64, _P],
+        _I32,
+    ),
     "vflash_packed_attention_workspace": ([_I64, _I64, _I64, _I64, _I64, _I64], _I64),
     "vflash_packed_attention": (
         [_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I32, _I64, _I64, _I64, _I64, _I64, _P, _P, _P,

@@ -36,6 +36,7 @@ hipError_t launch_restore_rows(const uint8_t*, const float*, int64_t, int64_t, i
 hipError_t launch_nvfp4(const uint8_t*, const float*, int64_t, const uint8_t*, const uint8_t*,
                         const float*, int64_t, int64_t, int64_t, const uint16_t*, uint16_t*, int64_t,
                         int, hipStream_t);
+hipError_t launch_nvfp4_w16(const GemmParams&, bool, hipStream_t);
 int64_t attention_workspace(const AttentionParams&);
 bool attention_fits(const AttentionParams&);
 hipError_t launch_attention(const AttentionParams&, bool, void*, hipStream_t);
@@ -486,6 +487,25 @@ int vflash_nvfp4_w4a4_linear(const void* a, int64_t lda, const void* a_scales, c
       static_cast<const uint8_t*>(w_packed), static_cast<const uint8_t*>(w_scales), alpha, m, n, k,
       static_cast<const uint16_t*>(bias), static_cast<uint16_t*>(out), ldo, FP4_GROUP_M,
       static_cast<hipStream_t>(stream)));
+}
+
+int vflash_nvfp4_w16_linear(const void* x, int x_is_f16, int64_t ldx, const void* w_packed, const void* w_scales,
+                            const float* alpha, int64_t m, int64_t n, int64_t k, const void* bias, void* out,
+                            int64_t ldo, void* stream) {
+  if (!x || !w_packed || !w_scales || !alpha || !out || m < 1 || n < 128 || n % 128 || k < 64 || k % 64)
+    return VFLASH_EINVAL;
+  if (ldx < k || ldx % 8 || ldo < n || ldo % 8) return VFLASH_EINVAL;
+  if (!aligned(x, 16) || !aligned(w_packed, 16) || !aligned(w_scales, 16) || !aligned(out, 16) || !aligned(alpha, 4) ||
+      (bias && !aligned(bias, 16)))
+    return VFLASH_EINVAL;
+  // Offsets inside a tile stay below 2^31 bytes, and a grid holds the tiles.
+  if (512 * ldx >= (int64_t(1) << 31) || 256 * (k / 2) >= (int64_t(1) << 31)) return VFLASH_EINVAL;
+  if (n >= (int64_t(1) << 25) || m >= (int64_t(1) << 31) || (m + 127) / 128 * ((n + 255) / 256) >= (int64_t(1) << 24))
+    return VFLASH_EINVAL;
+  vfa::GemmParams p = base_params(x, nullptr, 2 * ldx, w_packed, alpha, k / 2, m, n, k, bias, out, ldo);
+  p.sw_step = 0;
+  p.wsb = static_cast<const uint8_t*>(w_scales);
+  return status(vfa::launch_nvfp4_w16(p, x_is_f16 != 0, static_cast<hipStream_t>(stream)));
 }
 
 int64_t vflash_packed_attention_workspace(int64_t tokens, int64_t keys, int64_t batch, int64_t heads,

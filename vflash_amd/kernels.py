@@ -658,6 +658,38 @@ def nvfp4_w4a4_gemm(codes, act_scales, packed, block_scales, alpha, rows, bias=N
     return out
 
 
+def nvfp4_w16_gemm(matrix, packed, block_scales, alpha, bias=None):
+    """Weight-only NVFP4 GEMM: out[rows, N] = bf16(alpha * x . w^T + bias), x bf16 or f16."""
+    if matrix.dtype not in (torch.bfloat16, torch.float16) or matrix.ndim != 2 or matrix.stride(1) != 1:
+        raise ValueError("the weight-only NVFP4 GEMM requires a 2-D BF16/F16 matrix with unit column stride")
+    if packed.dtype != torch.uint8 or block_scales.dtype != torch.uint8:
+        raise ValueError("NVFP4 weights and block scales must be uint8")
+    if packed.ndim != 2 or not packed.is_contiguous():
+        raise ValueError("NVFP4 packed weights must be a contiguous uint8 [N, K/2] matrix")
+    n, half_k = packed.shape
+    rows, k = matrix.shape
+    if k != 2 * half_k:
+        raise ValueError("NVFP4 activation width differs from the weight")
+    if block_scales.shape != (n, k // 16) or not block_scales.is_contiguous():
+        raise ValueError("NVFP4 block scales must be a contiguous uint8 [N, K/16] matrix")
+    if alpha.dtype != torch.float32 or alpha.numel() != 1:
+        raise ValueError("NVFP4 alpha must be an fp32 scalar tensor")
+    if bias is not None and (bias.dtype != torch.bfloat16 or bias.shape != (n,)):
+        raise ValueError("NVFP4 bias must be a BF16 vector of the output width")
+    device = require_device(matrix, packed, block_scales, alpha, bias)
+    # The kernels read 16-byte vectors.
+    if matrix.stride(0) % 8 or matrix.data_ptr() % 16:
+        matrix = matrix.clone(memory_format=torch.contiguous_format)
+    packed, block_scales = (t.clone() if t.data_ptr() % 16 else t for t in (packed, block_scales))
+    if bias is not None and (bias.data_ptr() % 16 or not bias.is_contiguous()):
+        bias = bias.clone(memory_format=torch.contiguous_format)
+    out = torch.empty((rows, n), device=device, dtype=torch.bfloat16)
+    if rows:
+        call("vflash_nvfp4_w16_linear", ptr(matrix), int(matrix.dtype == torch.float16), matrix.stride(0), ptr(packed),
+             ptr(block_scales), ptr(alpha), rows, n, k, ptr(bias), ptr(out), out.stride(0), stream_of(device))
+    return out
+
+
 def _attention_rows(t):
     """``t`` [rows, heads, dim] as the attention kernels read it: unit stride in d, other
     strides multiples of 8, 16-byte aligned; copied where it is not."""

@@ -18,6 +18,13 @@ to bf16, and the bias is added with a second bf16 rounding
 activations (the FP8 path's quantizer) times the same weights, ``sa[m] *
 alpha`` in the epilogue; ``input_scale`` is then not used.  It is the more
 accurate arithmetic, not the reference's.
+
+``NVFP4Execution(activations="unquantized")`` is the weight-only form: BF16 or
+F16 activations enter the GEMM as they are (FP32 ones as BF16), the weight's
+E2M1 values and block scales multiply exactly, and ``alpha * sum + bias`` is
+rounded to bf16 once.  It reads a weight's half byte per value whatever the
+rows, so single tokens and small batches run at the weight's bytes;
+``input_scale`` is not used.
 """
 
 from __future__ import annotations
@@ -77,14 +84,20 @@ def _require_device(device):
 class NVFP4Execution:
     """NVFP4 execution on gfx950 (W4A4 by default); host counters remain diagnostic."""
 
-    contract = "nvfp4-e2m1-block16-128x4-w4a4-gfx950-v1"
+    contracts = {
+        "nvfp4": "nvfp4-e2m1-block16-128x4-w4a4-gfx950-v1",
+        "e4m3": "nvfp4-e2m1-block16-128x4-w4a8-gfx950-v1",
+        "unquantized": "nvfp4-e2m1-block16-128x4-w4a16-gfx950-v1",
+    }
+    contract = contracts["nvfp4"]
 
     def __init__(self, activations: str = "nvfp4"):
-        if activations not in ("nvfp4", "e4m3"):
-            raise ValueError("NVFP4 activations are 'nvfp4' (W4A4) or 'e4m3' (W4A8)")
+        if activations not in self.contracts:
+            raise ValueError(
+                "NVFP4 activations are 'nvfp4' (W4A4), 'e4m3' (W4A8) or 'unquantized' (weight-only)"
+            )
         self.activations = activations
-        if activations == "e4m3":
-            self.contract = "nvfp4-e2m1-block16-128x4-w4a8-gfx950-v1"
+        self.contract = self.contracts[activations]
         self.calls = 0
         self.rows = 0
 
@@ -122,6 +135,8 @@ class NVFP4Execution:
             output = kernels.nvfp4_w4a4_gemm(
                 codes, scales, weight.packed, weight.scales, alpha, matrix.shape[0], bias
             )
+        elif self.activations == "unquantized":
+            output = kernels.nvfp4_w16_gemm(matrix, weight.packed, weight.scales, weight.alpha, bias)
         else:
             codes, act_scale = kernels.quantize_rows(matrix)
             output = kernels.nvfp4_gemm(
