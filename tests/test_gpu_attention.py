@@ -141,6 +141,27 @@ def test_scale_and_large_scores(dev):
     assert torch.equal(got[0], v[123])
 
 
+def test_rows_without_keys_at_large_scales(dev):
+    for nq, nk in (([60, 1], [20, 0]), ([1, 2], [300, 1])):
+        for dtype in (BF16, F16):
+            q, k, v = make(dev, nq, nk, 4, 2, 64, dtype, std=0.2)
+            qo, ko = offsets(nq, dev), offsets(nk, dev)
+            for scale in (1.0, 40.0):
+                check(packed_attention(q, k, v, qo, ko, causal=True, scale=scale), q, k, v, qo, ko, causal=True, scale=scale)
+
+
+def test_scores_that_rise_and_fall(dev):
+    # Later keys far above and far below the first ones, in both types' ranges.
+    n = 700
+    for dtype, step in ((BF16, 3.0), (F16, 0.1)):
+        for sign in (1, -1):
+            for nq in (1, 90):
+                q, k, v = make(dev, [nq], [n], 2, 1, 64, dtype, std=0.5)
+                q[..., 0], k[:, 0, 0] = 1.0, (torch.arange(n, device=dev) * sign * step).to(dtype)
+                qo, ko = offsets([nq], dev), offsets([n], dev)
+                check(packed_attention(q, k, v, qo, ko, scale=1.0), q, k, v, qo, ko, scale=1.0)
+
+
 def test_binary16_keeps_small_probabilities(dev):
     # One score 17 above 60000 equal ones: each of these weighs 2^-24.5, together 2.5e-3.
     n = 60000

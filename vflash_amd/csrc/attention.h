@@ -23,13 +23,17 @@ namespace vfa {
 
 typedef _Float16 v8hf __attribute__((ext_vector_type(8)));
 typedef _Float16 v2hf __attribute__((ext_vector_type(2)));
+typedef __bf16 v2bf16s __attribute__((ext_vector_type(2)));
 typedef short v4s16 __attribute__((ext_vector_type(4)));
 
 // Below every finite exponent: 2^(x - m) is 0 for a masked x = -inf, with no inf - inf.
 #define VFA_LOWEST (-3.4028234663852886e38f)
-// The running maximum follows the scores only once they pass it by 2^8, so that the sums are
-// rarely rescaled; p is then at most 2^8 and, in binary16, carries 2^6 more, which keeps 30
-// binary orders below the largest p out of the format's subnormals.
+// m follows the scores only where the weights of a block of keys would pass a bound: 2^15 keeps
+// binary16 from overflowing, and bfloat16 has binary32's range.  A rounding is relative, so a
+// weight above 1 loses nothing; in binary16 it carries 2^6 more, which keeps 20 binary orders
+// below m out of the format's subnormals.
+template <bool F16>
+constexpr float kAttentionBound = F16 ? 32768.0f : 1152921504606846976.0f;  // 2^60
 constexpr float kAttentionSlack = 8.0f;
 constexpr float kAttentionFar = 4194304.0f;  // 2^22: a rounding of 1/4
 template <bool F16>
@@ -39,6 +43,14 @@ constexpr float kAttentionShift = F16 ? 6.0f : 0.0f;
 template <bool F16, bool FAR>
 __device__ __forceinline__ float attention_weight(float s, float c, float m, float ref) {
   return __builtin_amdgcn_exp2f(FAR ? (s - m) * c + kAttentionShift<F16> : __builtin_fmaf(s, c, ref));
+}
+// l plus the two weights of a packed pair, as they were rounded: the sum that normalises them.
+template <bool F16>
+__device__ __forceinline__ float attention_sum2(int pair, float l) {
+  if constexpr (F16)
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(v2hf, pair), v2hf{(_Float16)1.0f, (_Float16)1.0f}, l, false);
+  else
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf16s, pair), v2bf16s{(__bf16)1.0f, (__bf16)1.0f}, l, false);
 }
 // A row's maximum as its statistics carry it: scaled, and finite where it saw nothing.
 __device__ __forceinline__ float attention_top(float m, float c) { return fmaxf(m * c, VFA_LOWEST); }
@@ -111,19 +123,38 @@ __device__ __forceinline__ int wave_scan(int v, int lane, int& total) {
   return v;
 }
 
+// Inclusive prefix maximum of values that are not negative.
+__device__ __forceinline__ int wave_scan_max(int v, int lane) {
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true));
+  const int r0 = __builtin_amdgcn_readlane(v, 15), r1 = __builtin_amdgcn_readlane(v, 31);
+  const int r2 = __builtin_amdgcn_readlane(v, 47);
+  return max(v, lane < 16 ? 0 : lane < 32 ? r0 : lane < 48 ? max(r0, r1) : max(r0, max(r1, r2)));
+}
+
 struct AttentionSeq {
   int q0, k0, nq, nk;
 };
-// Sequence s of 0 .. batch + 1 (0 and batch + 1: the rows outside the offsets).
-__device__ __forceinline__ AttentionSeq attention_sequence(const AttentionParams& p, int64_t s) {
+// This lane's sequence, base + lane of 0 .. batch + 1 (0 and batch + 1: the rows outside the
+// offsets).  Sequences begin where the one before ends, at the running maximum of the offsets, so
+// that they cover every row once whatever these hold; `reached` carries it from base to base.
+__device__ __forceinline__ AttentionSeq attention_sequence(const AttentionParams& p, int64_t base, int& reached) {
   auto clamp = [](int64_t v, int lo, int hi) { return (int)(v < lo ? lo : v > hi ? hi : v); };
+  const int lane = (int)threadIdx.x & 63;
+  const int64_t s = base + lane;
   AttentionSeq r{0, 0, 0, 0};
-  if (s > p.batch + 1) return r;
-  r.q0 = s == 0 ? 0 : clamp(p.q_offsets[s - 1], 0, p.tokens);
-  r.nq = (s > p.batch ? p.tokens : clamp(p.q_offsets[s], r.q0, p.tokens)) - r.q0;
-  if (s == 0 || s > p.batch) return r;
-  r.k0 = clamp(p.k_offsets[s - 1], 0, p.keys);
-  r.nk = p.k_lengths ? clamp(p.k_lengths[s - 1], 0, p.keys - r.k0) : clamp(p.k_offsets[s], r.k0, p.keys) - r.k0;
+  const bool real = s > 0 && s <= p.batch;
+  const int64_t from = s == 0 || s > p.batch + 1 ? 0 : p.q_offsets[s - 1];
+  const int64_t to = s > p.batch ? p.tokens : p.q_offsets[s];
+  const int64_t k0 = real ? p.k_offsets[s - 1] : 0;
+  const int64_t nk = !real ? 0 : p.k_lengths ? p.k_lengths[s - 1] : p.k_offsets[s];
+  r.q0 = max(reached, wave_scan_max(clamp(from, 0, p.tokens), lane));
+  r.nq = s > p.batch + 1 ? 0 : clamp(to, r.q0, p.tokens) - r.q0;
+  r.k0 = clamp(k0, 0, p.keys);
+  if (real) r.nk = p.k_lengths ? clamp(nk, 0, p.keys - r.k0) : clamp(nk, r.k0, p.keys) - r.k0;
+  reached = __builtin_amdgcn_readlane(r.q0 + r.nq, 63);
   return r;
 }
 
@@ -147,6 +178,7 @@ __device__ __forceinline__ AttentionItem attention_item(const AttentionParams& p
   };
   auto blocks_of = [](const AttentionSeq& s) { return ((uint32_t)s.nk + 63) >> 6; };
   AttentionSeq mine{};
+  int reached = 0;
   // Keys of a split, in blocks of 64: the whole sequence where the tiles fill the GPU, else as
   // many as make about p.target items.
   uint32_t chunk = 1u << 25;
@@ -154,7 +186,7 @@ __device__ __forceinline__ AttentionItem attention_item(const AttentionParams& p
   if (p.target) {
     float work = 0;
     for (int64_t base = 0; base < n; base += 64) {
-      mine = attention_sequence(p, base + lane);
+      mine = attention_sequence(p, base, reached);
       int t = tiles_of(mine), sum;
       wave_scan(t, lane, sum);
       tiles += sum;
@@ -169,8 +201,9 @@ __device__ __forceinline__ AttentionItem attention_item(const AttentionParams& p
   // Units and slots per head block; the grid's order needs them before the search.  A split
   // sequence has more keys than a chunk, so the slots are at most 2 p.target.
   int units = 0, slots = 0;
+  reached = 0;
   for (int64_t base = 0; base < n; base += 64) {
-    if (!p.target || n > 64) mine = attention_sequence(p, base + lane);
+    if (!p.target || n > 64) mine = attention_sequence(p, base, reached);
     const int t = tiles_of(mine), sp = splits_of(mine);
     int sum;
     wave_scan(t * sp, lane, sum);
@@ -186,20 +219,27 @@ __device__ __forceinline__ AttentionItem attention_item(const AttentionParams& p
   if constexpr (JOIN) total = tiles;
   // Workgroup b runs on XCD b % 8.  Where the head blocks divide among the XCDs, each XCD
   // takes whole ones, one after another, so that its L2 holds their keys.
+  // Causal tiles differ in length: a head goes from its longest to its shortest and the next one
+  // back, so that the tiles that meet on a CU are long and short, and the last ones are short.
   int x;
+  bool turn = false;
   if (p.head_blocks % 8 == 0) {
-    const int i = (int)(index >> 3);
-    if (total == 0 || i >= total * (p.head_blocks / 8)) return it;
-    it.head_block = (int)(index & 7) + 8 * (i / total);
-    x = i % total;
+    const int i = (int)(index >> 3), each = p.head_blocks / 8;
+    if (total == 0 || i >= total * each) return it;
+    const int local = i / total;
+    it.head_block = (int)(index & 7) + 8 * local;
+    x = i - local * total;
+    turn = (each - 1 - local) % 2 != 0;
   } else {
     it.head_block = (int)(index % (uint32_t)p.head_blocks);
     x = (int)(index / (uint32_t)p.head_blocks);
     if (x >= total) return it;
   }
+  if (p.causal && turn) x = total - 1 - x;
   int before = 0, slots_before = 0;
+  reached = 0;
   for (int64_t base = 0; base < n; base += 64) {
-    if (n > 64) mine = attention_sequence(p, base + lane);
+    if (n > 64) mine = attention_sequence(p, base, reached);
     const int t = tiles_of(mine), sp = splits_of(mine), own = JOIN ? t : t * sp;
     int sum, slot_sum;
     const int incl = wave_scan(own, lane, sum);
@@ -243,6 +283,81 @@ __device__ __forceinline__ AttentionRow attention_row(const AttentionParams& p, 
 // Keys that the token sees.
 __device__ __forceinline__ int attention_limit(const AttentionParams& p, const AttentionSeq& s, int token) {
   return p.causal ? max(0, min(s.nk, s.nk - s.nq + token + 1)) : s.nk;
+}
+
+// The schedule of attention_step.  Every tile is a number of units (p.unit_keys keys each, one at
+// least), the units of all tiles of a head block form a line, the head blocks' lines one after
+// another a longer one, and each workgroup takes the next p.grid-th part of that: equal work whatever
+// the lengths.  A workgroup whose part ends inside a tile leaves a partial sum, of which it has at
+// most two: one of a tile begun by an earlier workgroup (slot 2 b), one of a tile that a later one ends
+// (slot 2 b + 1).  On one XCD's workgroups lie whole head blocks where these divide among the XCDs.
+struct AttentionLine {
+  uint32_t units;       // per head block
+  uint32_t quota, end;  // of a workgroup; of the line
+  uint32_t unit_keys;
+  int xcds;             // 8: the line is one XCD's
+  AttentionSeq mine;    // of this lane, where there are at most 64 sequences
+};
+struct AttentionSegment {
+  AttentionItem it;  // seq, tile, head_block
+  uint32_t first, count, of;  // units: the segment's first in its tile, its own, the tile's
+};
+
+__device__ __forceinline__ uint32_t attention_tiles_of(const AttentionParams& p, const AttentionSeq& s) {
+  return ((uint32_t)s.nq + (uint32_t)p.tile_tokens - 1) / (uint32_t)p.tile_tokens;
+}
+__device__ __forceinline__ uint32_t attention_units_of(const AttentionLine& l, const AttentionSeq& s) {
+  return max(1u, ((uint32_t)s.nk + l.unit_keys - 1) / l.unit_keys);
+}
+
+__device__ __forceinline__ AttentionLine attention_line(const AttentionParams& p, int grid) {
+  const int lane = (int)threadIdx.x & 63;
+  AttentionLine l{};
+  l.unit_keys = (uint32_t)p.unit_keys;
+  int reached = 0;
+  for (int64_t base = 0; base < p.batch + 2; base += 64) {
+    l.mine = attention_sequence(p, base, reached);
+    int sum;
+    wave_scan((int)(attention_tiles_of(p, l.mine) * attention_units_of(l, l.mine)), lane, sum);
+    l.units += (uint32_t)sum;
+  }
+  l.xcds = p.head_blocks % 8 == 0 ? 8 : 1;
+  l.end = l.units * (uint32_t)(p.head_blocks / l.xcds);
+  const uint32_t parts = (uint32_t)(grid / l.xcds);
+  l.quota = max(1u, (l.end + parts - 1) / parts);
+  return l;
+}
+
+// The rest of the tile at unit `pos` (< line.end) of workgroup b's line, up to unit `stop`.
+__device__ __forceinline__ AttentionSegment attention_segment(const AttentionParams& p, const AttentionLine& line, int b,
+                                                              uint32_t pos, uint32_t stop) {
+  const int lane = (int)threadIdx.x & 63;
+  const int64_t n = p.batch + 2;
+  AttentionSegment g{};
+  const uint32_t local = pos / line.units, x = pos - local * line.units;
+  g.it.head_block = line.xcds == 8 ? (b & 7) + 8 * (int)local : (int)local;
+  uint32_t before = 0;
+  int reached = 0;
+  for (int64_t base = 0; base < n; base += 64) {
+    const AttentionSeq mine = n > 64 ? attention_sequence(p, base, reached) : line.mine;
+    const uint32_t u = attention_units_of(line, mine), own = attention_tiles_of(p, mine) * u;
+    int sum;
+    const uint32_t incl = (uint32_t)wave_scan((int)own, lane, sum);
+    if (x < before + (uint32_t)sum) {
+      const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(before + incl > x));
+      auto pick = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
+      g.it.seq = AttentionSeq{pick(mine.q0), pick(mine.k0), pick(mine.nq), pick(mine.nk)};
+      g.of = (uint32_t)pick((int)u);
+      const uint32_t in = x - before - (uint32_t)pick((int)(incl - own));
+      g.it.tile = (int)(in / g.of);
+      g.first = in - (uint32_t)g.it.tile * g.of;
+      g.count = min(g.of - g.first, stop - pos);
+      g.it.live = true;
+      return g;
+    }
+    before += (uint32_t)sum;
+  }
+  return g;
 }
 
 }  // namespace vfa

@@ -8,9 +8,8 @@
 // V^T is read from the row-major tile by transposing LDS reads, four keys at a time.
 //
 // A workgroup's waves, 32 rows each, share tiles of 64 keys in LDS, which DMA fills one tile
-// ahead.  Probabilities are rounded to the operands' type for the second product (half a step,
-// 2^-9 or 2^-12 of each), as the matrix instruction takes them; their sum is of the unrounded
-// ones in binary32.
+// ahead.  Weights are rounded to the operands' type (half a step, 2^-9 or 2^-12 of each), as the
+// matrix instruction takes them, and so does the binary32 sum that normalises them.
 #include "attention.h"
 
 namespace vfa {
@@ -18,7 +17,7 @@ namespace vfa {
 template <int DP>
 struct AttentionTiles {
   static constexpr int PITCH = DP <= 64 ? 128 : 256, CHUNKS = PITCH / 16, ROWS = 1024 / PITCH;
-  static constexpr int KEYS = 64, TILE = KEYS * PITCH, SLOT = 2 * TILE;
+  static constexpr int KEYS = 64, KB = KEYS / 32, TILE = KEYS * PITCH, SLOT = 2 * TILE;
 };
 // The 16-byte chunk c of row r lies in slot c ^ key.  K: the 16 rows of a ds_read_b128 phase take
 // different slots.  V: the four rows x four chunks that a half wave's transposing read takes do.
@@ -32,7 +31,7 @@ __device__ __forceinline__ int v_swizzle(int r) {
 }
 
 template <bool F16, int DP, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES, 2) attention_tiles(const AttentionParams p) {
+__global__ void __launch_bounds__(64 * WAVES, DP <= 64 ? 4 : 2) attention_tiles(const AttentionParams p) {
   using L = AttentionTiles<DP>;
   constexpr int QS = DP / 16, DB = DP / 32;            // contraction steps, blocks of 32 d
   constexpr int BLOCKS = L::TILE / 1024 / WAVES;       // DMA instructions per wave for K, and for V
@@ -116,10 +115,10 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attention_tiles(const Attention
     asm volatile("" ::: "memory");
     if (key0 + L::KEYS < last) issue(buf ^ 1, key0 + L::KEYS);
     if (key0 >= end) continue;
-    v16f s[2];
-    static_for<2>([&](auto kbk) {
-      s[kbk] = v16f{};
-      static_for<QS>([&](auto st) {
+    v16f s[L::KB];
+    static_for<L::KB>([&](auto kbk) { s[kbk] = v16f{}; });
+    static_for<QS>([&](auto st) {
+      static_for<L::KB>([&](auto kbk) {
         const v4i a = *reinterpret_cast<const v4i*>(krow + buf * L::SLOT + kbk * 32 * L::PITCH +
                                                     (((2 * st + fh) ^ ksw) << 4));
         s[kbk] = mfma32<F16>(a, q[st], s[kbk]);
@@ -127,40 +126,43 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attention_tiles(const Attention
     });
     if (key0 + L::KEYS > open) {  // some row of the wave masks some key
       const int lim = limit - key0 - 4 * fh;
-      static_for<2>([&](auto kbk) {
+      static_for<L::KB>([&](auto kbk) {
         static_for<16>([&](auto r) {
           const int key = kbk * 32 + 8 * (r / 4) + r % 4;
           s[kbk][(int)r] = key < lim ? s[kbk][(int)r] : -__builtin_inff();
         });
       });
     }
-    float mx = s[0][0];
-    static_for<31>([&](auto r) { mx = fmaxf(mx, s[(r + 1) / 16][(int)((r + 1) % 16)]); });
-    mx = max_across32(mx);
-    if (__builtin_amdgcn_ballot_w64(mx * p.c > m * p.c + kAttentionSlack)) {
-      const float next = fmaxf(m, mx), f = __builtin_amdgcn_exp2f((m - next) * p.c);
-      static_for<DB>([&](auto i) { static_for<16>([&](auto r) { o[i][(int)r] *= f; }); });
-      l *= f;
-      m = next;
-      far = __builtin_amdgcn_ballot_w64(fabsf(m * p.c) >= kAttentionFar && m > VFA_LOWEST) != 0;
-    }
-    const float ref = kAttentionShift<F16> - m * p.c;
-    v4i pk[4];
+    v4i pk[2 * L::KB];
+    float sum;
     auto weights = [&](auto far_rows) {
-      static_for<4>([&](auto st) {
+      const float ref = kAttentionShift<F16> - attention_top(m, p.c);
+      sum = 0;
+      static_for<2 * L::KB>([&](auto st) {
         static_for<4>([&](auto j) {
           constexpr int r = (st % 2) * 8 + 2 * j;
-          const float a = attention_weight<F16, far_rows>(s[st / 2][r], p.c, m, ref);
-          const float b = attention_weight<F16, far_rows>(s[st / 2][r + 1], p.c, m, ref);
-          l += a;
-          l += b;
-          pk[st][(int)j] = pack2<F16>(a, b);
+          pk[st][(int)j] = pack2<F16>(attention_weight<F16, far_rows>(s[st / 2][r], p.c, m, ref),
+                                      attention_weight<F16, far_rows>(s[st / 2][r + 1], p.c, m, ref));
+          sum = attention_sum2<F16>(pk[st][(int)j], sum);
         });
       });
     };
     if (far) weights(std::true_type{});
     else weights(std::false_type{});
-    static_for<4>([&](auto st) {
+    if (__builtin_amdgcn_ballot_w64(!(sum <= kAttentionBound<F16>))) {
+      // The first keys that a row sees, or scores far above those before.
+      float mx = s[0][0];
+      static_for<16 * L::KB - 1>([&](auto r) { mx = fmaxf(mx, s[(r + 1) / 16][(int)((r + 1) % 16)]); });
+      const float next = fmaxf(m, max_across32(mx)), f = __builtin_amdgcn_exp2f((m - next) * p.c);
+      static_for<DB>([&](auto i) { static_for<16>([&](auto r) { o[i][(int)r] *= f; }); });
+      l *= f;
+      m = next;
+      far = __builtin_amdgcn_ballot_w64(fabsf(m * p.c) >= kAttentionFar && m > VFA_LOWEST) != 0;
+      if (far) weights(std::true_type{});
+      else weights(std::false_type{});
+    }
+    l += sum;
+    static_for<2 * L::KB>([&](auto st) {
       static_for<DB>([&](auto db) {
         const uint8_t* src = vrow + buf * L::SLOT + st * 16 * L::PITCH + (((4 * db + vc) ^ vsw) << 4);
         const v2i lo = lds_read_tr16(src), hi = lds_read_tr16(src + 8 * L::PITCH);
@@ -242,7 +244,7 @@ __global__ void __launch_bounds__(256) attention_join(const AttentionParams p, i
 
 // ---------------------------------------------------------------------------
 int compute_units();
-void launch_attention_step(const AttentionParams&, bool, int64_t, hipStream_t);
+void launch_attention_step(const AttentionParams&, bool, int, bool, hipStream_t);
 
 namespace {
 
@@ -269,9 +271,23 @@ AttentionPlan attention_plan(AttentionParams& p) {
   int64_t tiles = p.tokens / p.tile_tokens + p.batch + 2;
   if (tiles > p.tokens) tiles = p.tokens;
   const int64_t blocks = ((int64_t)p.keys + 63) / 64;
+  if (plan.step) {
+    // A CU holds one workgroup of dimension 128, two of 64.  Splitting pays a second launch: not
+    // where the sequences are short, or the cache holds few keys for each.
+    const bool split = p.keys > 1024 && p.keys > 256 * p.batch;
+    p.unit_keys = split ? 128 : INT32_MAX;
+    auto bound = [&] { return tiles * p.head_blocks * (((int64_t)p.keys + p.unit_keys - 1) / p.unit_keys + 1); };
+    while (bound() >= int64_t(1) << 30 && p.unit_keys < 1 << 29) p.unit_keys *= 2;  // the kernel counts in 32 bits
+    const int64_t units = bound();
+    plan.grid = (cus + 7) / 8 * 8 * (p.dim <= 64 ? 2 : 1);
+    if (units < plan.grid) plan.grid = (units + 7) / 8 * 8;
+    plan.join = split;
+    p.slots = split ? 2 * plan.grid : 0;
+    return plan;
+  }
   p.target = (int)(2 * cus);
-  p.min_chunk = plan.step ? 4 : 4;
-  if (blocks <= p.min_chunk || (!plan.step && (int64_t)p.tokens / p.tile_tokens * p.head_blocks >= 4 * cus)) p.target = 0;
+  p.min_chunk = 4;
+  if (blocks <= p.min_chunk || (int64_t)p.tokens / p.tile_tokens * p.head_blocks >= 4 * cus) p.target = 0;
   p.slots = p.target ? 2 * p.target + p.head_blocks : 0;
   plan.join = p.target ? tiles * p.head_blocks : 0;
   plan.grid = tiles * p.head_blocks + (p.target ? p.slots : 0);
@@ -300,7 +316,8 @@ int64_t attention_workspace(const AttentionParams& params) {
 // false: the grid would pass HIP's limit.
 bool attention_fits(const AttentionParams& params) {
   AttentionParams p = params;
-  return attention_plan(p).grid < (int64_t(1) << 24);
+  const AttentionPlan plan = attention_plan(p);
+  return plan.grid < (int64_t(1) << 24) && plan.join < (int64_t(1) << 24);
 }
 
 hipError_t launch_attention(const AttentionParams& params, bool f16, void* workspace, hipStream_t s) {
@@ -308,12 +325,12 @@ hipError_t launch_attention(const AttentionParams& params, bool f16, void* works
   const AttentionPlan plan = attention_plan(p);
   p.part = static_cast<float*>(workspace);
   p.part_ml = p.part + p.slots * plan.rows * p.dim;
-  if (plan.step)
-    launch_attention_step(p, f16, plan.grid, s);
-  else if (f16)
-    launch_tiles<true>(p, plan.grid, s);
-  else
-    launch_tiles<false>(p, plan.grid, s);
+  if (plan.step) {
+    launch_attention_step(p, f16, (int)plan.grid, plan.join != 0, s);
+    return hipGetLastError();
+  }
+  if (f16) launch_tiles<true>(p, plan.grid, s);
+  else launch_tiles<false>(p, plan.grid, s);
   if (plan.join) {
     const dim3 g((unsigned)plan.join, (unsigned)(plan.rows / 4 < 8 ? plan.rows / 4 : 8));
     if (f16) attention_join<true><<<g, dim3(256), 0, s>>>(p, plan.rows);

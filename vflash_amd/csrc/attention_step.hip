@@ -36,20 +36,24 @@ __global__ void __launch_bounds__(256, 1) attention_step(const AttentionParams p
   __shared__ __attribute__((aligned(1024))) uint8_t lds[L::WAVES * L::NS * L::SLOT];
   __shared__ float stat[L::WAVES][16][2];
   static_assert(L::WAVES * 16 * L::ACC <= L::WAVES * L::NS * L::SLOT && (L::NS - 1) * L::DMA < 64, "LDS, vmcnt");
-  const AttentionItem it = attention_item<false>(p, blockIdx.x);
-  if (!it.live) return;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int lane = (int)threadIdx.x & 63;
   const int fr = lane & 15, fg = lane >> 4;
   uint8_t* ring = lds + wave * (L::NS * L::SLOT);
   const uint32_t ring_lds = __builtin_amdgcn_readfirstlane(lds_addr(ring));
 
+  const AttentionLine line = attention_line(p, gridDim.x);
+  const uint32_t begin = (blockIdx.x / line.xcds) * line.quota, stop = min(begin + line.quota, line.end);
+  for (uint32_t pos = begin; pos < stop;) {
+  const AttentionSegment seg = attention_segment(p, line, blockIdx.x, pos, stop);
+  const AttentionItem& it = seg.it;
+  if (!it.live) return;
   const AttentionRow row = attention_row(p, it, fr);
   const int key_head = it.head_block / p.parts;
   const int last_token = min(it.seq.nq, (it.tile + 1) * p.tile_tokens) - 1;
   const int tile_limit = attention_limit(p, it.seq, last_token);
-  const int first = it.split * it.chunk;
-  const int last = (int)min((int64_t)tile_limit, (int64_t)first + it.chunk);
+  const int first = (int)min(seg.first * (uint64_t)line.unit_keys, (uint64_t)INT32_MAX);
+  const int last = (int)min((uint64_t)tile_limit, (seg.first + seg.count) * (uint64_t)line.unit_keys);
   const int limit = row.live ? min(attention_limit(p, it.seq, row.token), last) : last;
   // Keys that every row sees.
   const int open = min(attention_limit(p, it.seq, min(it.tile * p.tile_tokens, it.seq.nq)), last);
@@ -126,7 +130,7 @@ __global__ void __launch_bounds__(256, 1) attention_step(const AttentionParams p
       m = next;
       far = __builtin_amdgcn_ballot_w64(fabsf(m * p.c) >= kAttentionFar && m > VFA_LOWEST) != 0;
     }
-    const float ref = kAttentionShift<F16> - m * p.c;
+    const float ref = kAttentionShift<F16> - attention_top(m, p.c);
     v4i pk;
     auto weights = [&](auto far_rows) {
       static_for<4>([&](auto j) {
@@ -164,33 +168,89 @@ __global__ void __launch_bounds__(256, 1) attention_step(const AttentionParams p
   // Thread t: row t / 16, the d of t % 16 in runs of four.
   const int r = (int)threadIdx.x >> 4, e = (int)threadIdx.x & 15;
   const AttentionRow mine = attention_row(p, it, r);
-  if (!mine.live) return;
-  float top = stat[0][r][0], sum = 0, f[L::WAVES];
-  static_for<L::WAVES - 1>([&](auto w) { top = fmaxf(top, stat[w + 1][r][0]); });
-  static_for<L::WAVES>([&](auto w) {
-    f[w] = __builtin_amdgcn_exp2f(stat[w][r][0] - top);
-    sum += f[w] * stat[w][r][1];
-  });
-  const bool split = it.splits > 1;
-  if (split && first >= tile_limit) return;  // attention_join does not read it
-  const int64_t at = (int64_t)(it.slot + it.split) * 16 + r;
-  if (split && e == 0) *reinterpret_cast<v2f*>(p.part_ml + at * 2) = v2f{top, sum};
-  const float inv = split ? 1.0f : 1.0f / sum;
-  uint16_t* dst = p.out + (int64_t)(it.seq.q0 + mine.token) * p.o_ts + (int64_t)mine.head * p.o_hs;
-  for (int d = 4 * e; d < p.dim; d += 64) {
-    v4f x = v4f{};
-    static_for<L::WAVES>([&](auto w) { x += *reinterpret_cast<const v4f*>(lds + (w * 16 + r) * L::ACC + d * 4) * f[w]; });
-    x = sum == 0 ? v4f{} : x * inv;
-    if (split) {
-      *reinterpret_cast<v4f*>(p.part + at * p.dim + d) = x;
-    } else {
-      typedef int v2i_ __attribute__((ext_vector_type(2)));
-      *reinterpret_cast<v2i_*>(dst + d) = v2i_{pack2<F16>(x[0], x[1]), pack2<F16>(x[2], x[3])};
+  if (mine.live) {
+    float top = stat[0][r][0], sum = 0, f[L::WAVES];
+    static_for<L::WAVES - 1>([&](auto w) { top = fmaxf(top, stat[w + 1][r][0]); });
+    static_for<L::WAVES>([&](auto w) {
+      f[w] = __builtin_amdgcn_exp2f(stat[w][r][0] - top);
+      sum += f[w] * stat[w][r][1];
+    });
+    const bool whole = seg.count == seg.of;
+    const int64_t at = (2 * (int64_t)blockIdx.x + (seg.first == 0)) * 16 + r;
+    if (!whole && e == 0) *reinterpret_cast<v2f*>(p.part_ml + at * 2) = v2f{top, sum};
+    const float inv = whole ? 1.0f / sum : 1.0f;
+    uint16_t* dst = p.out + (int64_t)(it.seq.q0 + mine.token) * p.o_ts + (int64_t)mine.head * p.o_hs;
+    for (int d = 4 * e; d < p.dim; d += 64) {
+      v4f x = v4f{};
+      static_for<L::WAVES>(
+          [&](auto w) { x += *reinterpret_cast<const v4f*>(lds + (w * 16 + r) * L::ACC + d * 4) * f[w]; });
+      x = sum == 0 ? v4f{} : x * inv;
+      if (whole) *reinterpret_cast<v2i*>(dst + d) = v2i{pack2<F16>(x[0], x[1]), pack2<F16>(x[2], x[3])};
+      else *reinterpret_cast<v4f*>(p.part + at * p.dim + d) = x;
     }
+  }
+  pos += seg.count;
+  if (pos < stop) __syncthreads();  // the sums are read: the rings may be filled again
   }
 }
 
-void launch_attention_step(const AttentionParams& p, bool f16, int64_t grid, hipStream_t s) {
+// The sum over a tile's segments: out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s.  Workgroup b
+// takes the tile that workgroup b of attention_step began and did not end.  Thread t: d 4 (t % 16) and
+// 64 more, one row, every SG-th segment; the segments' sums of a row meet in LDS.
+template <bool F16>
+__global__ void __launch_bounds__(256) attention_step_join(const AttentionParams p) {
+  const AttentionLine line = attention_line(p, gridDim.x);
+  const int part = blockIdx.x / line.xcds;
+  const uint32_t begin = part * line.quota, stop = min(begin + line.quota, line.end);
+  if (begin >= stop) return;
+  const AttentionSegment seg = attention_segment(p, line, blockIdx.x, stop - 1, line.end);
+  const uint32_t tile_begin = stop - 1 - seg.first, tile_end = tile_begin + seg.of;
+  if (!seg.it.live || tile_begin < begin || tile_end <= stop) return;
+  const int segments = (int)((tile_end - 1) / line.quota) - part + 1;
+  // Segment s lies in workgroup blockIdx.x + xcds s, slot 1 for the first, 0 for the others.
+  auto slot = [&](int s) { return 2 * ((int64_t)blockIdx.x + line.xcds * s) + (s == 0); };
+  const int tokens = min(p.tile_tokens, seg.it.seq.nq - seg.it.tile * p.tile_tokens);
+  const int rows = min(16, tokens * p.heads_per_tile);
+  const int pow = rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 4 ? 4 : rows <= 8 ? 8 : 16;
+  const int e = (int)threadIdx.x & 15, r = (int)threadIdx.x / 16 % pow, sg = (int)threadIdx.x / 16 / pow, groups = 16 / pow;
+  __shared__ float sums[16][132];
+  float top = VFA_LOWEST;
+  for (int s = e; s < segments; s += 16) top = fmaxf(top, p.part_ml[(slot(s) * 16 + r) * 2]);
+  for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+  v4f x[2] = {v4f{}, v4f{}};
+  float l = 0;
+#pragma unroll 4
+  for (int s = sg; s < segments; s += groups) {
+    const int64_t at = slot(s) * 16 + r;
+    const v2f ml = *reinterpret_cast<const v2f*>(p.part_ml + at * 2);
+    const float f = __builtin_amdgcn_exp2f(ml[0] - top);
+    l += f * ml[1];
+    static_for<2>([&](auto h) {
+      const int d = 4 * e + 64 * h;
+      if (d < p.dim) x[h] += *reinterpret_cast<const v4f*>(p.part + at * p.dim + d) * f;
+    });
+  }
+  float* mine = sums[(int)threadIdx.x / 16];
+  static_for<2>([&](auto h) { *reinterpret_cast<v4f*>(mine + 4 * e + 64 * h) = x[h]; });
+  if (e == 0) mine[128] = l;
+  __syncthreads();
+  const AttentionRow row = attention_row(p, seg.it, r);
+  if (sg || !row.live) return;
+  for (int q = 1; q < groups; ++q) {
+    const float* other = sums[q * pow + r];
+    static_for<2>([&](auto h) { x[h] += *reinterpret_cast<const v4f*>(other + 4 * e + 64 * h); });
+    l += other[128];
+  }
+  const float inv = 1.0f / l;
+  uint16_t* dst = p.out + (int64_t)(seg.it.seq.q0 + row.token) * p.o_ts + (int64_t)row.head * p.o_hs;
+  static_for<2>([&](auto h) {
+    const int d = 4 * e + 64 * h;
+    const v4f y = l == 0 ? v4f{} : x[h] * inv;
+    if (d < p.dim) *reinterpret_cast<v2i*>(dst + d) = v2i{pack2<F16>(y[0], y[1]), pack2<F16>(y[2], y[3])};
+  });
+}
+
+void launch_attention_step(const AttentionParams& p, bool f16, int grid, bool join, hipStream_t s) {
   const dim3 g((unsigned)grid), b(256);
   if (p.dim <= 64) {
     if (f16) attention_step<true, 64><<<g, b, 0, s>>>(p);
@@ -199,6 +259,9 @@ void launch_attention_step(const AttentionParams& p, bool f16, int64_t grid, hip
     if (f16) attention_step<true, 128><<<g, b, 0, s>>>(p);
     else attention_step<false, 128><<<g, b, 0, s>>>(p);
   }
+  if (!join) return;
+  if (f16) attention_step_join<true><<<g, b, 0, s>>>(p);
+  else attention_step_join<false><<<g, b, 0, s>>>(p);
 }
 
 }  // namespace vfa
