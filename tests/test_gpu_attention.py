@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from tests.attention_reference import check
+from vflash_amd import _lib, kernels
 from vflash_amd.attention import packed_attention
 
 pytestmark = pytest.mark.gpu
@@ -231,6 +232,29 @@ def test_graph_replays_other_lengths(dev):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, packed_attention(q, k, v, qo, ko, k_lengths=kl))
+
+
+def test_native_host_path(dev):
+    # The same bits as the Python wrapper's; None for what that one has to decide.
+    host = _lib.host()
+    q, k, v = make(dev, [1, 60], [90, 60], 8, 2, 64, BF16)
+    qo, ko = offsets([1, 60], dev), offsets([90, 60], dev)
+    kl = torch.tensor([90, 60], device=dev)
+    for causal, scale in ((True, None), (False, 0.3)):
+        want = kernels.packed_attention(q, k, v, qo, ko, None, causal, 0.125 if scale is None else scale)
+        assert torch.equal(host.packed_attention(q, k, v, qo, ko, None, causal, scale), want)
+        assert torch.equal(host.packed_attention(q, k, v, qo, ko[:2], kl, causal, scale), want)
+    p = torch.nn.Parameter(q)
+    assert host.packed_attention(p, k, v, qo, ko, None, True, None) is None
+    with torch.no_grad():
+        assert torch.equal(packed_attention(p, k, v, qo, ko), packed_attention(q, k, v, qo, ko))
+    for args in ((q.cpu(), k, v, qo, ko, None, True, None), (q, k, v, qo.int(), ko, None, True, None),
+                 (q, k, v, qo, ko, kl, True, None), (q, k, v[..., :32], qo, ko, None, True, None),
+                 (q, k, v, qo.cpu(), ko, None, True, None), (q, k, v, qo, ko, None, 1, None),
+                 (q, k, v, qo, ko, None, True, -1.0), (q, k, v, qo, ko, None, True, 1),
+                 (q[:, :3], k, v, qo, ko, None, True, None), (q[:0], k, v, qo, ko, None, True, None),
+                 (q.float(), k.float(), v.float(), qo, ko, None, True, None)):
+        assert host.packed_attention(*args) is None
 
 
 def test_no_rows(dev):

@@ -3,6 +3,7 @@
 import pytest
 import torch
 
+from vflash_amd import _lib, kernels
 from vflash_amd.nvfp4_linear import NVFP4Execution, NVFP4Weight
 from vflash_amd.prepare import quantize_nvfp4_weight
 
@@ -137,6 +138,22 @@ def test_repeated_calls_other_streams_and_graphs(dev):
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(out, ex.linear(x, weight, b))
+
+
+def test_native_host_path(dev):
+    # The same bits as the Python wrapper's; None for what that one has to decide.
+    host = _lib.host()
+    for m in (1, 30, 300):
+        x, w, b = make(dev, m, 256, 192, F16)
+        for bias in (b, None):
+            want = kernels.nvfp4_w16_gemm(x, w.packed, w.scales, w.alpha, bias)
+            assert torch.equal(host.nvfp4_w16_linear(x, w.packed, w.scales, w.alpha, bias), want)
+        assert host.nvfp4_w16_linear(x.reshape(1, m, 192), w.packed, w.scales, w.alpha, b).shape == (1, m, 256)
+    for args in ((x.float(), w.packed, w.scales, w.alpha, b), (x[:, :64], w.packed, w.scales, w.alpha, b),
+                 (x.cpu(), w.packed, w.scales, w.alpha, b), (x, w.packed, w.scales, w.alpha, b[:8]),
+                 (x, w.packed, w.scales, w.alpha.cpu(), b), (x.clone().requires_grad_(), w.packed, w.scales, w.alpha, b),
+                 (x[:0], w.packed, w.scales, w.alpha, b), (x, w.packed[:64], w.scales[:64], w.alpha, None)):
+        assert host.nvfp4_w16_linear(*args) is None
 
 
 def test_refusals(dev):

@@ -115,6 +115,9 @@ SIGNATURES: dict[str, tuple[list, object]] = {
     ),
 }
 
+# What the native host path (csrc/host.cpp) serves.
+HOST_CALLS = ("w8a8_linear", "w8a8_linear_lora", "nvfp4_w16_linear", "packed_attention")
+
 
 class KernelError(RuntimeError):
     """The HIP runtime refused a launch."""
@@ -164,6 +167,10 @@ def host():
     try:
         library()
         from vflash_amd import _host
+
+        missing = [name for name in HOST_CALLS if not hasattr(_host, name)]
+        if missing:
+            raise ImportError(f"_host.so is older than this package (it has no {missing[0]})")
     except ImportError as e:
         warnings.warn(f"the native host path is off ({e}); `python -m vflash_amd.build` builds it for this "
                       "Python and torch", RuntimeWarning, stacklevel=2)

@@ -15,7 +15,7 @@ import math
 
 import torch
 
-from vflash_amd import kernels
+from vflash_amd import _lib, kernels
 
 
 def packed_attention(q, k, v, q_offsets, k_offsets, *, k_lengths=None, causal=False, scale=None):
@@ -37,6 +37,13 @@ def packed_attention(q, k, v, q_offsets, k_offsets, *, k_lengths=None, causal=Fa
 
     Offsets are read on the device, clamped to the operands.  Inference only.
     """
+    if isinstance(q, torch.Tensor) and q.is_cuda:
+        # The whole call in native code; None sends any other layout, and every refusal, on from here.
+        host = _lib.host()
+        if host is not None:
+            out = host.packed_attention(q, k, v, q_offsets, k_offsets, k_lengths, causal, scale)
+            if out is not None:
+                return out
     tensors = (q, k, v)
     if any(t.ndim != 3 for t in tensors):
         raise ValueError("packed attention takes [rows, heads, dim] queries, keys and values")

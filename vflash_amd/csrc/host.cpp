@@ -1,4 +1,4 @@
-// The host side of the two W8A8 linears that users call most, natively: checks,
+// The host side of the calls that are short on the GPU, natively: checks,
 // allocations and launches of one call without a round trip through Python for
 // each of them.
 //
@@ -15,10 +15,12 @@
 
 #include <ATen/ATen.h>
 #include <ATen/hip/HIPContext.h>
+#include <c10/core/GradMode.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <cmath>
 #include <cstring>
 
 #include "../../include/vflash_amd.h"
@@ -155,10 +157,105 @@ PyObject* w8a8_linear_lora(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+bool records(const at::Tensor& t) { return t.requires_grad() && c10::GradMode::is_enabled(); }
+
+bool aligned16(const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
+
+// nvfp4_w16_linear(values, packed, scales, alpha, bias): the weight-only NVFP4 linear.
+PyObject* nvfp4_w16_linear(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 5) Py_RETURN_NONE;
+  const at::Tensor *x = plain(a[0]), *w = plain(a[1]), *ws = plain(a[2]), *alpha = plain(a[3]);
+  const at::Tensor* b = a[4] == Py_None ? nullptr : plain(a[4]);
+  if (!x || !w || !ws || !alpha || (a[4] != Py_None && !b) || records(*x)) Py_RETURN_NONE;
+  const bool f16 = x->scalar_type() == at::kHalf;
+  if ((!f16 && x->scalar_type() != at::kBFloat16) || w->scalar_type() != at::kByte || ws->scalar_type() != at::kByte ||
+      alpha->scalar_type() != at::kFloat || alpha->numel() != 1)
+    Py_RETURN_NONE;
+  if (x->dim() < 1 || !x->is_contiguous() || w->dim() != 2 || !w->is_contiguous() || !ws->is_contiguous() || x->numel() == 0)
+    Py_RETURN_NONE;
+  const int64_t n = w->size(0), k = 2 * w->size(1);
+  if (x->size(-1) != k || ws->dim() != 2 || ws->size(0) != n || ws->size(1) != k / 16) Py_RETURN_NONE;
+  const c10::Device d = x->device();
+  if (w->device() != d || ws->device() != d || alpha->device() != d || !gfx950(d.index())) Py_RETURN_NONE;
+  if (b && (b->dim() != 1 || b->size(0) != n || b->scalar_type() != at::kBFloat16 || b->device() != d || !b->is_contiguous()))
+    Py_RETURN_NONE;
+  at::Tensor out;
+  int status;
+  {
+    const NoGil nogil;
+    c10::SmallVector<int64_t, 5> shape(x->sizes().begin(), x->sizes().end());
+    shape.back() = n;
+    out = at::empty(shape, x->options().dtype(at::kBFloat16).requires_grad(false));
+    // Alignments and limits are the entry's to refuse.
+    status = vflash_nvfp4_w16_linear(x->data_ptr(), f16, k, w->data_ptr(), ws->data_ptr(),
+                                     static_cast<float*>(alpha->data_ptr()), x->numel() / k, n, k,
+                                     b ? b->data_ptr() : nullptr, out.data_ptr(), n,
+                                     c10::hip::getCurrentHIPStream(d.index()).stream());
+  }
+  if (status != VFLASH_OK) Py_RETURN_NONE;
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// The offsets or lengths of `count` sequences (any number where it is negative).
+const int64_t* indices(const at::Tensor* t, c10::Device d, int64_t count) {
+  if (!t || t->scalar_type() != at::kLong || t->dim() != 1 || !t->is_contiguous() || t->device() != d ||
+      (count >= 0 && t->numel() != count))
+    return nullptr;
+  return static_cast<const int64_t*>(t->data_ptr());
+}
+
+// packed_attention(q, k, v, q_offsets, k_offsets, k_lengths, causal, scale): with a causal of True
+// or False and a scale of None or a float.
+PyObject* packed_attention(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 8 || !PyBool_Check(a[6]) || (a[7] != Py_None && !PyFloat_CheckExact(a[7]))) Py_RETURN_NONE;
+  const at::Tensor *q = plain(a[0]), *k = plain(a[1]), *v = plain(a[2]), *qo = plain(a[3]), *ko = plain(a[4]);
+  const at::Tensor* kl = a[5] == Py_None ? nullptr : plain(a[5]);
+  if (!q || !k || !v || !qo || !ko || (a[5] != Py_None && !kl)) Py_RETURN_NONE;
+  if (records(*q) || records(*k) || records(*v)) Py_RETURN_NONE;
+  const auto type = q->scalar_type();
+  if ((type != at::kBFloat16 && type != at::kHalf) || k->scalar_type() != type || v->scalar_type() != type) Py_RETURN_NONE;
+  if (q->dim() != 3 || k->dim() != 3 || k->sizes() != v->sizes() || q->size(2) != k->size(2)) Py_RETURN_NONE;
+  const c10::Device d = q->device();
+  if (k->device() != d || v->device() != d || !gfx950(d.index()) || qo->numel() < 1) Py_RETURN_NONE;
+  for (const at::Tensor* t : {q, k, v})
+    if (t->stride(2) != 1 || !aligned16(*t)) Py_RETURN_NONE;
+  const int64_t tokens = q->size(0), heads = q->size(1), dim = q->size(2), keys = k->size(0), key_heads = k->size(1);
+  const int64_t batch = qo->numel() - 1;
+  const int64_t *q_offsets = indices(qo, d, -1), *k_offsets = indices(ko, d, kl ? batch : batch + 1);
+  const int64_t* k_lengths = kl ? indices(kl, d, batch) : nullptr;
+  if (!q_offsets || !k_offsets || (kl && !k_lengths) || tokens == 0) Py_RETURN_NONE;
+  const int64_t bytes = vflash_packed_attention_workspace(tokens, keys, batch, heads, key_heads, dim);
+  if (bytes < 0) Py_RETURN_NONE;
+  const double scale = a[7] == Py_None ? 1.0 / std::sqrt((double)dim) : PyFloat_AS_DOUBLE(a[7]);
+  const bool causal = a[6] == Py_True;
+  at::Tensor out;
+  int status;
+  {
+    const NoGil nogil;
+    out = at::empty({tokens, heads, dim}, q->options().requires_grad(false));
+    const at::Tensor workspace = bytes ? at::empty({bytes}, q->options().dtype(at::kByte).requires_grad(false)) : at::Tensor();
+    status = vflash_packed_attention(
+        q->data_ptr(), q->stride(0), q->stride(1), k->data_ptr(), k->stride(0), k->stride(1), v->data_ptr(),
+        v->stride(0), v->stride(1), type == at::kHalf, tokens, keys, heads, key_heads, dim, q_offsets, k_offsets,
+        k_lengths, batch, causal, (float)scale, out.data_ptr(), heads * dim, dim, bytes ? workspace.data_ptr() : nullptr,
+        bytes, c10::hip::getCurrentHIPStream(d.index()).stream());
+  }
+  if (status != VFLASH_OK) Py_RETURN_NONE;
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef kMethods[] = {
     {"w8a8_linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(w8a8_linear)),
      METH_FASTCALL, nullptr},
     {"w8a8_linear_lora", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(w8a8_linear_lora)),
+     METH_FASTCALL, nullptr},
+    {"nvfp4_w16_linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(nvfp4_w16_linear)),
+     METH_FASTCALL, nullptr},
+    {"packed_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(packed_attention)),
      METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, kMethods,

@@ -102,6 +102,16 @@ class NVFP4Execution:
         self.rows = 0
 
     def linear(self, values, weight: NVFP4Weight, bias=None):
+        if self.activations == "unquantized" and isinstance(values, torch.Tensor) and values.is_cuda:
+            # The whole call in native code; None sends any other layout, and every refusal, on from here.
+            host = _lib.host()
+            output = None
+            if host is not None:
+                output = host.nvfp4_w16_linear(values, weight.packed, weight.scales, weight.alpha, bias)
+            if output is not None:
+                self.calls += 1
+                self.rows += values.numel() // weight.in_features
+                return output
         if (
             values.ndim < 1
             or values.shape[-1] != weight.in_features
