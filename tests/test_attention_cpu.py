@@ -82,8 +82,8 @@ def test_every_tile_has_a_workgroup(tmp_path):
     calls = []
     for tokens, keys, batch, heads, kv, dim in PLANS:
         # Sized for the stand-in's device of 256 compute units, on which the workspace is at
-        # most 2 x 512 + head blocks slots of 128 rows.
-        size = (2 * 512 + heads) * 128 * (dim + 2) * 4
+        # most 2 x 768 + head blocks slots of 128 rows.
+        size = (2 * 768 + heads) * 128 * (dim + 2) * 4
         calls.append(("vflash_packed_attention",
                       [P, heads * dim, dim, P, kv * dim, dim, P, kv * dim, dim, 0, tokens, keys, heads, kv, dim, P, P,
                        None, batch, 1, 0.5, P, heads * dim, dim, P, size, None]))
@@ -102,6 +102,6 @@ def test_every_tile_has_a_workgroup(tmp_path):
             assert x % 8 == 0 and x <= 512 and y == z == 1 and threads == 256, plan
         if len(run) == 2:
             name, (jx, jy, _), threads = run[1]
-            assert threads == 256
+            assert threads == (256 if rows == 128 else 1024)
             assert name.startswith("attention_join") and jx >= worst if rows == 128 else jx == x, plan
     assert lib.vflash_packed_attention_workspace(0, 1, 1, 4, 2, 64) == _lib.VFLASH_EINVAL

@@ -141,26 +141,36 @@ struct AttentionSeq {
 // offsets).  Sequences begin where the one before ends, at the running maximum of the offsets, so
 // that they cover every row once whatever these hold; `reached` carries it from base to base.
 __device__ __forceinline__ AttentionSeq attention_sequence(const AttentionParams& p, int64_t base, int& reached) {
-  auto clamp = [](int64_t v, int lo, int hi) { return (int)(v < lo ? lo : v > hi ? hi : v); };
-  const int lane = (int)threadIdx.x & 63;
-  const int64_t s = base + lane;
-  AttentionSeq r{0, 0, 0, 0};
+  // Clamped to [0, hi] through the 32 bits that are left when the others say which side.
+  auto clamp = [](int64_t v, int hi) { return v < 0 ? 0 : (uint64_t)v > (uint64_t)hi ? hi : (int)v; };
+  const int64_t s = base + (threadIdx.x & 63);
   const bool real = s > 0 && s <= p.batch;
-  const int64_t from = s == 0 || s > p.batch + 1 ? 0 : p.q_offsets[s - 1];
-  const int64_t to = s > p.batch ? p.tokens : p.q_offsets[s];
-  const int64_t k0 = real ? p.k_offsets[s - 1] : 0;
-  const int64_t nk = !real ? 0 : p.k_lengths ? p.k_lengths[s - 1] : p.k_offsets[s];
-  r.q0 = max(reached, wave_scan_max(clamp(from, 0, p.tokens), lane));
-  r.nq = s > p.batch + 1 ? 0 : clamp(to, r.q0, p.tokens) - r.q0;
-  r.k0 = clamp(k0, 0, p.keys);
-  if (real) r.nk = p.k_lengths ? clamp(nk, 0, p.keys - r.k0) : clamp(nk, r.k0, p.keys) - r.k0;
+  // Every lane loads, from a place that exists, so that no load waits for another.
+  const int64_t at = s < 1 ? 0 : s > p.batch ? p.batch : s, before = at > 0 ? at - 1 : 0;
+  const int64_t from = p.q_offsets[before], to = p.q_offsets[at];
+  int64_t k0 = 0, kn = 0;
+  if (p.batch) {
+    k0 = p.k_offsets[before];
+    kn = (p.k_lengths ? p.k_lengths : p.k_offsets + 1)[before];
+  }
+  // Sequence batch + 1 begins where the offsets end; later ones are empty.
+  const int first = s == 0 ? 0 : clamp(s > p.batch ? to : from, p.tokens);
+  AttentionSeq r;
+  r.q0 = max(reached, wave_scan_max(first, (int)threadIdx.x & 63));
+  r.nq = s > p.batch + 1 ? 0 : max(0, (s > p.batch ? p.tokens : clamp(to, p.tokens)) - r.q0);
+  r.k0 = clamp(k0, p.keys);
+  r.nk = !real ? 0 : p.k_lengths ? clamp(kn, p.keys - r.k0) : max(0, clamp(kn, p.keys) - r.k0);
   reached = __builtin_amdgcn_readlane(r.q0 + r.nq, 63);
   return r;
 }
 
+__device__ __forceinline__ uint32_t attention_tiles_of(const AttentionParams& p, const AttentionSeq& s) {
+  return (uint32_t)(((uint64_t)((uint32_t)s.nq + (uint32_t)p.tile_tokens - 1) * p.tile_mul) >> p.tile_shift);
+}
+
 struct AttentionItem {
   AttentionSeq seq;  // all uniform
-  int tile, tiles;   // of the sequence
+  int tile;          // of the sequence
   int split, splits;
   int chunk;         // keys of a split
   int slot;          // of the tile's split 0, where it has several
@@ -168,100 +178,135 @@ struct AttentionItem {
   bool live;
 };
 
+// Which of `total` units of which head block workgroup `index` takes; false: none.
+// Workgroup b runs on XCD b % 8.  Where the head blocks divide among the XCDs, each XCD takes whole
+// ones, one after another, so that its L2 holds their keys.  Causal tiles differ in length: a
+// head goes from its longest to its shortest and the next one back, so that the tiles that meet on
+// a CU are long and short, and the last ones are short.
+__device__ __forceinline__ bool attention_place(const AttentionParams& p, uint32_t index, int total, int& head_block, int& x) {
+  if (total == 0) return false;
+  if (p.head_blocks % 8 == 0) {
+    const int i = (int)(index >> 3), each = p.head_blocks / 8;
+    const int local = (int)((uint32_t)i / (uint32_t)total);
+    if (local >= each) return false;
+    head_block = (int)(index & 7) + 8 * local;
+    x = i - local * total;
+    if (p.causal && (each - 1 - local) % 2) x = total - 1 - x;
+    return true;
+  }
+  x = (int)(index / (uint32_t)p.head_blocks);
+  head_block = (int)index - x * p.head_blocks;
+  return x < total;
+}
+
 // The unit `index` of the launch: an item, or with JOIN a tile (all its splits).
 template <bool JOIN>
-__device__ __forceinline__ AttentionItem attention_item(const AttentionParams& p, uint32_t index) {
+__device__ __forceinline__ AttentionItem attention_find(const AttentionParams& p, uint32_t index) {
   const int lane = (int)threadIdx.x & 63;
   const int64_t n = p.batch + 2;
-  auto tiles_of = [&](const AttentionSeq& s) {
-    return (int)(((uint32_t)s.nq + (uint32_t)p.tile_tokens - 1) / (uint32_t)p.tile_tokens);
+  int reached = 0, x;
+  AttentionItem it{};
+  AttentionSeq mine = attention_sequence(p, 0, reached);
+  auto take = [&](int l) {
+    auto pick = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
+    it.seq = AttentionSeq{pick(mine.q0), pick(mine.k0), pick(mine.nq), pick(mine.nk)};
+    it.live = true;
   };
+  if (!p.target && n <= 64) {  // no split, and the sequences are in the lanes
+    const int t = (int)attention_tiles_of(p, mine);
+    int total;
+    const int incl = wave_scan(t, lane, total);
+    if (!attention_place(p, index, total, it.head_block, x)) return it;
+    const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(incl > x));
+    take(l);
+    it.tile = __builtin_amdgcn_readlane(incl, l) - 1 - x;  // from the last to the first: longest first
+    it.splits = 1;
+    it.chunk = INT32_MAX;
+    return it;
+  }
   auto blocks_of = [](const AttentionSeq& s) { return ((uint32_t)s.nk + 63) >> 6; };
-  AttentionSeq mine{};
-  int reached = 0;
   // Keys of a split, in blocks of 64: the whole sequence where the tiles fill the GPU, else as
   // many as make about p.target items.
   uint32_t chunk = 1u << 25;
   int tiles = 0;
+  auto each = [&](auto&& f) {  // f(tiles) for every 64 sequences, in `mine`, until it returns true
+    reached = 0;
+    for (int64_t base = 0; base < n; base += 64) {
+      if (n > 64) mine = attention_sequence(p, base, reached);
+      if (f((int)attention_tiles_of(p, mine))) return;
+    }
+  };
   if (p.target) {
     float work = 0;
-    for (int64_t base = 0; base < n; base += 64) {
-      mine = attention_sequence(p, base, reached);
-      int t = tiles_of(mine), sum;
+    each([&](int t) {
+      int sum;
       wave_scan(t, lane, sum);
       tiles += sum;
       work += wave_sum((float)t * (float)blocks_of(mine));
-    }
+      return false;
+    });
     work = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(work)));
     chunk = max((uint32_t)p.min_chunk, (uint32_t)fminf(ceilf(work * (float)p.head_blocks / (float)p.target), 33554432.0f));
   }
   auto splits_of = [&](const AttentionSeq& s) { return (int)max(1u, (blocks_of(s) + chunk - 1) / chunk); };
   auto slots_of = [](int t, int sp) { return sp > 1 ? t * sp : 0; };
-  AttentionItem it{};
   // Units and slots per head block; the grid's order needs them before the search.  A split
   // sequence has more keys than a chunk, so the slots are at most 2 p.target.
   int units = 0, slots = 0;
-  reached = 0;
-  for (int64_t base = 0; base < n; base += 64) {
-    if (!p.target || n > 64) mine = attention_sequence(p, base, reached);
-    const int t = tiles_of(mine), sp = splits_of(mine);
+  each([&](int t) {
+    const int sp = splits_of(mine);
     int sum;
     wave_scan(t * sp, lane, sum);
     units += sum;
     wave_scan(slots_of(t, sp), lane, sum);
     slots += sum;
-  }
+    return false;
+  });
   if (p.target && (int64_t)slots * p.head_blocks > p.slots) {  // not reached: a bound on the memory
     chunk = 1u << 25;
     units = tiles;
   }
-  int total = units;  // of what `index` counts
-  if constexpr (JOIN) total = tiles;
-  // Workgroup b runs on XCD b % 8.  Where the head blocks divide among the XCDs, each XCD
-  // takes whole ones, one after another, so that its L2 holds their keys.
-  // Causal tiles differ in length: a head goes from its longest to its shortest and the next one
-  // back, so that the tiles that meet on a CU are long and short, and the last ones are short.
-  int x;
-  bool turn = false;
-  if (p.head_blocks % 8 == 0) {
-    const int i = (int)(index >> 3), each = p.head_blocks / 8;
-    if (total == 0 || i >= total * each) return it;
-    const int local = i / total;
-    it.head_block = (int)(index & 7) + 8 * local;
-    x = i - local * total;
-    turn = (each - 1 - local) % 2 != 0;
-  } else {
-    it.head_block = (int)(index % (uint32_t)p.head_blocks);
-    x = (int)(index / (uint32_t)p.head_blocks);
-    if (x >= total) return it;
-  }
-  if (p.causal && turn) x = total - 1 - x;
+  if (!attention_place(p, index, JOIN ? tiles : units, it.head_block, x)) return it;
   int before = 0, slots_before = 0;
-  reached = 0;
-  for (int64_t base = 0; base < n; base += 64) {
-    if (n > 64) mine = attention_sequence(p, base, reached);
-    const int t = tiles_of(mine), sp = splits_of(mine), own = JOIN ? t : t * sp;
+  each([&](int t) {
+    const int sp = splits_of(mine), own = JOIN ? t : t * sp;
     int sum, slot_sum;
     const int incl = wave_scan(own, lane, sum);
     const int slot_incl = wave_scan(slots_of(t, sp), lane, slot_sum);
     if (x < before + sum) {
       const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(before + incl > x));
-      auto pick = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
-      it.seq = AttentionSeq{pick(mine.q0), pick(mine.k0), pick(mine.nq), pick(mine.nk)};
-      it.tiles = pick(t);
-      it.splits = pick(sp);
-      const int in = x - before - pick(incl - own);
-      const int back = JOIN ? in : in / it.splits;  // tiles from the last to the first: longest first
-      it.split = JOIN ? 0 : in % it.splits;
-      it.tile = it.tiles - 1 - back;
+      take(l);
+      it.splits = __builtin_amdgcn_readlane(sp, l);
+      const int in = x - before - __builtin_amdgcn_readlane(incl - own, l);
+      const int back = JOIN ? in : in / it.splits;
+      it.split = JOIN ? 0 : in - back * it.splits;
+      it.tile = __builtin_amdgcn_readlane(t, l) - 1 - back;
       it.chunk = (int)min((uint64_t)chunk * 64, (uint64_t)INT32_MAX);
-      it.slot = it.head_block * slots + slots_before + pick(slot_incl - slots_of(t, sp)) + back * it.splits;
-      it.live = true;
-      return it;
+      it.slot = it.head_block * slots + slots_before + __builtin_amdgcn_readlane(slot_incl - slots_of(t, sp), l) +
+                back * it.splits;
+      return true;
     }
     before += sum;
     slots_before += slot_sum;
-  }
+    return false;
+  });
+  return it;
+}
+
+// The same in scalar registers, where the compiler does not see that the search is uniform.
+template <bool JOIN>
+__device__ __forceinline__ AttentionItem attention_item(const AttentionParams& p, uint32_t index) {
+  auto u = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+  const AttentionItem f = attention_find<JOIN>(p, index);
+  AttentionItem it;
+  it.seq = AttentionSeq{u(f.seq.q0), u(f.seq.k0), u(f.seq.nq), u(f.seq.nk)};
+  it.tile = u(f.tile);
+  it.split = u(f.split);
+  it.splits = u(f.splits);
+  it.chunk = u(f.chunk);
+  it.slot = u(f.slot);
+  it.head_block = u(f.head_block);
+  it.live = u(f.live) != 0;
   return it;
 }
 
@@ -270,14 +315,24 @@ struct AttentionRow {
   int token, head;
   bool live;
 };
+// Row r's token of the tile: r / heads_per_tile, for r < 512.
+__device__ __forceinline__ int attention_token_of(const AttentionParams& p, int r) { return (r * p.row_mul) >> 16; }
 __device__ __forceinline__ AttentionRow attention_row(const AttentionParams& p, const AttentionItem& it, int r) {
-  const int in = (int)((uint32_t)r / (uint32_t)p.heads_per_tile);
+  const int in = attention_token_of(p, r);
   const int h = it.head_block % p.parts * p.heads_per_tile + r - in * p.heads_per_tile;
   AttentionRow row;
   row.token = it.tile * p.tile_tokens + in;
   row.head = it.head_block / p.parts * p.group + h;
   row.live = in < p.tile_tokens && row.token < it.seq.nq && h < p.group;
   return row;
+}
+
+// Eight d of the row, zeros past the head's dimension and for a row that is none.  Always a load, from
+// a place that exists.
+__device__ __forceinline__ v4i attention_query(const AttentionParams& p, const AttentionItem& it, const AttentionRow& row, int d) {
+  const uint16_t* src = row.live ? p.q + (int64_t)(it.seq.q0 + row.token) * p.q_ts + (int64_t)row.head * p.q_hs : p.q;
+  const v4i v = *reinterpret_cast<const v4i*>(src + min(d, p.dim - 8));
+  return row.live && d < p.dim ? v : v4i{};
 }
 
 // Keys that the token sees.
@@ -303,9 +358,6 @@ struct AttentionSegment {
   uint32_t first, count, of;  // units: the segment's first in its tile, its own, the tile's
 };
 
-__device__ __forceinline__ uint32_t attention_tiles_of(const AttentionParams& p, const AttentionSeq& s) {
-  return ((uint32_t)s.nq + (uint32_t)p.tile_tokens - 1) / (uint32_t)p.tile_tokens;
-}
 __device__ __forceinline__ uint32_t attention_units_of(const AttentionLine& l, const AttentionSeq& s) {
   return max(1u, ((uint32_t)s.nk + l.unit_keys - 1) / l.unit_keys);
 }

@@ -17,7 +17,7 @@ namespace vfa {
 template <int DP>
 struct AttentionTiles {
   static constexpr int PITCH = DP <= 64 ? 128 : 256, CHUNKS = PITCH / 16, ROWS = 1024 / PITCH;
-  static constexpr int KEYS = 64, KB = KEYS / 32, TILE = KEYS * PITCH, SLOT = 2 * TILE;
+  static constexpr int KEYS = DP <= 64 ? 64 : 32, KB = KEYS / 32, TILE = KEYS * PITCH, SLOT = 2 * TILE;
 };
 // The 16-byte chunk c of row r lies in slot c ^ key.  K: the 16 rows of a ds_read_b128 phase take
 // different slots.  V: the four rows x four chunks that a half wave's transposing read takes do.
@@ -31,7 +31,7 @@ __device__ __forceinline__ int v_swizzle(int r) {
 }
 
 template <bool F16, int DP, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES, DP <= 64 ? 4 : 2) attention_tiles(const AttentionParams p) {
+__global__ void __launch_bounds__(64 * WAVES, DP <= 64 ? 4 : 3) attention_tiles(const AttentionParams p) {
   using L = AttentionTiles<DP>;
   constexpr int QS = DP / 16, DB = DP / 32;            // contraction steps, blocks of 32 d
   constexpr int BLOCKS = L::TILE / 1024 / WAVES;       // DMA instructions per wave for K, and for V
@@ -53,8 +53,8 @@ __global__ void __launch_bounds__(64 * WAVES, DP <= 64 ? 4 : 2) attention_tiles(
   const int last = (int)min((int64_t)tile_limit, (int64_t)first + it.chunk);
   const int limit = row.live ? attention_limit(p, it.seq, row.token) : last;
   // Of this wave: the keys before which no row masks anything, and after which all do.
-  const int wave_first_token = min(it.tile * p.tile_tokens + wave * 32 / p.heads_per_tile, it.seq.nq);
-  const int wave_last_token = min(it.tile * p.tile_tokens + min((wave * 32 + 31) / p.heads_per_tile, p.tile_tokens - 1),
+  const int wave_first_token = min(it.tile * p.tile_tokens + attention_token_of(p, wave * 32), it.seq.nq);
+  const int wave_last_token = min(it.tile * p.tile_tokens + min(attention_token_of(p, wave * 32 + 31), p.tile_tokens - 1),
                                   it.seq.nq - 1);
   const int open = min(attention_limit(p, it.seq, wave_first_token), last);
   const int end = min(attention_limit(p, it.seq, wave_last_token), last);
@@ -86,13 +86,7 @@ __global__ void __launch_bounds__(64 * WAVES, DP <= 64 ? 4 : 2) attention_tiles(
 
   if (first < last) issue(0, first);
   v4i q[QS];
-  {
-    const uint16_t* src = p.q + (int64_t)(it.seq.q0 + row.token) * p.q_ts + (int64_t)row.head * p.q_hs;
-    static_for<QS>([&](auto s) {
-      const int d = s * 16 + fh * 8;
-      q[s] = row.live && d < p.dim ? *reinterpret_cast<const v4i*>(src + d) : v4i{};
-    });
-  }
+  static_for<QS>([&](auto s) { q[s] = attention_query(p, it, row, s * 16 + fh * 8); });
   v16f o[DB];
   static_for<DB>([&](auto i) { o[i] = v16f{}; });
   float m = VFA_LOWEST, l = 0;
@@ -208,37 +202,35 @@ __global__ void __launch_bounds__(64 * WAVES, DP <= 64 ? 4 : 2) attention_tiles(
 }
 
 // The sum over a tile's splits: out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s.  A workgroup
-// per tile, ROWS of its rows at a time; 64 lanes of a wave take a row's d two by two.
+// takes every eighth row of a tile, half a wave a row, four d a lane.
 template <bool F16>
 __global__ void __launch_bounds__(256) attention_join(const AttentionParams p, int rows) {
   const AttentionItem it = attention_item<true>(p, blockIdx.x);
   if (!it.live || it.splits == 1) return;
-  const int wave = (int)threadIdx.x >> 6, lane = (int)threadIdx.x & 63;
+  const int d = 4 * ((int)threadIdx.x & 31);
   const int last_token = min(it.seq.nq, (it.tile + 1) * p.tile_tokens) - 1;
   const int tile_limit = attention_limit(p, it.seq, last_token);
   const int splits = (int)(((uint32_t)tile_limit + (uint32_t)it.chunk - 1) / (uint32_t)it.chunk);
-  for (int r = blockIdx.y * 4 + wave; r < rows; r += 4 * gridDim.y) {
+#pragma unroll 2
+  for (int r = blockIdx.y * 8 + ((int)threadIdx.x >> 5); r < rows; r += 8 * gridDim.y) {
     const AttentionRow row = attention_row(p, it, r);
-    if (!row.live) continue;
-    float top = VFA_LOWEST;
-    for (int s = lane; s < splits; s += 64) top = fmaxf(top, p.part_ml[((int64_t)(it.slot + s) * rows + r) * 2]);
-    top = wave_max(top);
-    float a = 0, b = 0, l = 0;
+    float top = VFA_LOWEST, l = 0;
+    v4f x = v4f{};
+#pragma unroll 4
     for (int s = 0; s < splits; ++s) {
       const int64_t at = (int64_t)(it.slot + s) * rows + r;
       const v2f ml = *reinterpret_cast<const v2f*>(p.part_ml + at * 2);
-      const float f = __builtin_amdgcn_exp2f(ml[0] - top);
-      l += f * ml[1];
-      if (2 * lane < p.dim) {
-        const v2f x = *reinterpret_cast<const v2f*>(p.part + at * p.dim + 2 * lane);
-        a += f * x[0];
-        b += f * x[1];
-      }
+      const v4f y = d < p.dim ? *reinterpret_cast<const v4f*>(p.part + at * p.dim + d) : v4f{};
+      const float next = fmaxf(top, ml[0]);
+      const float old = __builtin_amdgcn_exp2f(top - next), f = __builtin_amdgcn_exp2f(ml[0] - next);
+      top = next;
+      l = l * old + f * ml[1];
+      x = x * old + y * f;
     }
-    const float inv = 1.0f / l;
-    if (2 * lane < p.dim)
-      *reinterpret_cast<int*>(p.out + (int64_t)(it.seq.q0 + row.token) * p.o_ts + (int64_t)row.head * p.o_hs + 2 * lane) =
-          l == 0 ? 0 : pack2<F16>(a * inv, b * inv);
+    x = l == 0 ? v4f{} : x * (1.0f / l);
+    if (row.live && d < p.dim)
+      *reinterpret_cast<v2i*>(p.out + (int64_t)(it.seq.q0 + row.token) * p.o_ts + (int64_t)row.head * p.o_hs + d) =
+          v2i{pack2<F16>(x[0], x[1]), pack2<F16>(x[2], x[3])};
   }
 }
 
@@ -260,6 +252,7 @@ struct AttentionPlan {
 AttentionPlan attention_plan(AttentionParams& p) {
   const int64_t cus = compute_units();
   AttentionPlan plan{};
+  p.tile_shift = 31;
   const int few = p.group < kStepRows ? p.group : kStepRows;
   plan.step = (int64_t)p.tokens * few <= p.batch * kStepRows;
   plan.rows = plan.step ? kStepRows : kTileRows;
@@ -267,6 +260,10 @@ AttentionPlan attention_plan(AttentionParams& p) {
   p.parts = (p.group + p.heads_per_tile - 1) / p.heads_per_tile;
   p.head_blocks = p.heads / p.group * p.parts;
   p.tile_tokens = plan.rows / p.heads_per_tile;
+  // Divisions by these two as products: exact below 2^31 and 2^9.
+  while ((1 << (p.tile_shift - 31)) < p.tile_tokens) ++p.tile_shift;
+  p.tile_mul = (uint32_t)(((uint64_t(1) << p.tile_shift) + p.tile_tokens - 1) / p.tile_tokens);
+  p.row_mul = (65536 + p.heads_per_tile - 1) / p.heads_per_tile;
   // At most a tile per token, or whole tiles and one partial tile per sequence.
   int64_t tiles = p.tokens / p.tile_tokens + p.batch + 2;
   if (tiles > p.tokens) tiles = p.tokens;
@@ -285,9 +282,9 @@ AttentionPlan attention_plan(AttentionParams& p) {
     p.slots = split ? 2 * plan.grid : 0;
     return plan;
   }
-  p.target = (int)(2 * cus);
+  p.target = (int)(3 * cus);
   p.min_chunk = 4;
-  if (blocks <= p.min_chunk || (int64_t)p.tokens / p.tile_tokens * p.head_blocks >= 4 * cus) p.target = 0;
+  if (blocks <= p.min_chunk || (int64_t)p.tokens / p.tile_tokens * p.head_blocks >= cus) p.target = 0;
   p.slots = p.target ? 2 * p.target + p.head_blocks : 0;
   plan.join = p.target ? tiles * p.head_blocks : 0;
   plan.grid = tiles * p.head_blocks + (p.target ? p.slots : 0);
@@ -332,7 +329,7 @@ hipError_t launch_attention(const AttentionParams& params, bool f16, void* works
   if (f16) launch_tiles<true>(p, plan.grid, s);
   else launch_tiles<false>(p, plan.grid, s);
   if (plan.join) {
-    const dim3 g((unsigned)plan.join, (unsigned)(plan.rows / 4 < 8 ? plan.rows / 4 : 8));
+    const dim3 g((unsigned)plan.join, 8);
     if (f16) attention_join<true><<<g, dim3(256), 0, s>>>(p, plan.rows);
     else attention_join<false><<<g, dim3(256), 0, s>>>(p, plan.rows);
   }

@@ -18,6 +18,8 @@ struct AttentionParams {
   int heads_per_tile;  // of a key head's group; a group of more than the tile's rows has `parts` blocks
   int parts, head_blocks;
   int tile_tokens;
+  uint32_t tile_mul;  // x / tile_tokens = x * tile_mul >> tile_shift
+  int tile_shift, row_mul;  // r / heads_per_tile = r * row_mul >> 16
   // Splitting of the keys, off where target is 0.
   int target, min_chunk;  // items, blocks of 64 keys
   int64_t slots;          // what the workspace holds

@@ -83,13 +83,7 @@ __global__ void __launch_bounds__(256, 1) attention_step(const AttentionParams p
   static_for<L::NS>([&](auto i) { issue(i, start + i * STRIDE); });
 
   v4i q[QS];
-  {
-    const uint16_t* src = p.q + (int64_t)(it.seq.q0 + row.token) * p.q_ts + (int64_t)row.head * p.q_hs;
-    static_for<QS>([&](auto s) {
-      const int d = s * 32 + fg * 8;
-      q[s] = row.live && d < p.dim ? *reinterpret_cast<const v4i*>(src + d) : v4i{};
-    });
-  }
+  static_for<QS>([&](auto s) { q[s] = attention_query(p, it, row, s * 32 + fg * 8); });
   v4f o[DB];
   static_for<DB>([&](auto i) { o[i] = v4f{}; });
   float m = VFA_LOWEST, l = 0;
@@ -196,9 +190,9 @@ __global__ void __launch_bounds__(256, 1) attention_step(const AttentionParams p
 
 // The sum over a tile's segments: out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s.  Workgroup b
 // takes the tile that workgroup b of attention_step began and did not end.  Thread t: d 4 (t % 16) and
-// 64 more, one row, every SG-th segment; the segments' sums of a row meet in LDS.
+// 64 more, one row, every groups-th segment under a maximum of its own; the groups meet in LDS.
 template <bool F16>
-__global__ void __launch_bounds__(256) attention_step_join(const AttentionParams p) {
+__global__ void __launch_bounds__(1024) attention_step_join(const AttentionParams p) {
   const AttentionLine line = attention_line(p, gridDim.x);
   const int part = blockIdx.x / line.xcds;
   const uint32_t begin = part * line.quota, stop = min(begin + line.quota, line.end);
@@ -212,34 +206,43 @@ __global__ void __launch_bounds__(256) attention_step_join(const AttentionParams
   const int tokens = min(p.tile_tokens, seg.it.seq.nq - seg.it.tile * p.tile_tokens);
   const int rows = min(16, tokens * p.heads_per_tile);
   const int pow = rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 4 ? 4 : rows <= 8 ? 8 : 16;
-  const int e = (int)threadIdx.x & 15, r = (int)threadIdx.x / 16 % pow, sg = (int)threadIdx.x / 16 / pow, groups = 16 / pow;
-  __shared__ float sums[16][132];
-  float top = VFA_LOWEST;
-  for (int s = e; s < segments; s += 16) top = fmaxf(top, p.part_ml[(slot(s) * 16 + r) * 2]);
-  for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+  const int groups = min(16, 64 / pow);
+  const int e = (int)threadIdx.x & 15, r = (int)threadIdx.x / 16 % pow, sg = (int)threadIdx.x / 16 / pow;
+  __shared__ float sums[64][132];
+  float top = VFA_LOWEST, l = 0;
   v4f x[2] = {v4f{}, v4f{}};
-  float l = 0;
 #pragma unroll 4
-  for (int s = sg; s < segments; s += groups) {
+  for (int s = sg; s < segments && sg < groups; s += groups) {
     const int64_t at = slot(s) * 16 + r;
     const v2f ml = *reinterpret_cast<const v2f*>(p.part_ml + at * 2);
-    const float f = __builtin_amdgcn_exp2f(ml[0] - top);
-    l += f * ml[1];
+    const float next = fmaxf(top, ml[0]);
+    const float old = __builtin_amdgcn_exp2f(top - next), f = __builtin_amdgcn_exp2f(ml[0] - next);
+    top = next;
+    l = l * old + f * ml[1];
     static_for<2>([&](auto h) {
       const int d = 4 * e + 64 * h;
-      if (d < p.dim) x[h] += *reinterpret_cast<const v4f*>(p.part + at * p.dim + d) * f;
+      if (d < p.dim) x[h] = x[h] * old + *reinterpret_cast<const v4f*>(p.part + at * p.dim + d) * f;
     });
   }
   float* mine = sums[(int)threadIdx.x / 16];
   static_for<2>([&](auto h) { *reinterpret_cast<v4f*>(mine + 4 * e + 64 * h) = x[h]; });
-  if (e == 0) mine[128] = l;
+  if (e == 0) {
+    mine[128] = l;
+    mine[129] = top;
+  }
   __syncthreads();
   const AttentionRow row = attention_row(p, seg.it, r);
   if (sg || !row.live) return;
+  float all = top;
+  for (int q = 1; q < groups; ++q) all = fmaxf(all, sums[q * pow + r][129]);
+  const float f0 = __builtin_amdgcn_exp2f(top - all);
+  l *= f0;
+  static_for<2>([&](auto h) { x[h] *= f0; });
   for (int q = 1; q < groups; ++q) {
     const float* other = sums[q * pow + r];
-    static_for<2>([&](auto h) { x[h] += *reinterpret_cast<const v4f*>(other + 4 * e + 64 * h); });
-    l += other[128];
+    const float f = __builtin_amdgcn_exp2f(other[129] - all);
+    static_for<2>([&](auto h) { x[h] += *reinterpret_cast<const v4f*>(other + 4 * e + 64 * h) * f; });
+    l += other[128] * f;
   }
   const float inv = 1.0f / l;
   uint16_t* dst = p.out + (int64_t)(seg.it.seq.q0 + row.token) * p.o_ts + (int64_t)row.head * p.o_hs;
@@ -260,8 +263,8 @@ void launch_attention_step(const AttentionParams& p, bool f16, int grid, bool jo
     else attention_step<false, 128><<<g, b, 0, s>>>(p);
   }
   if (!join) return;
-  if (f16) attention_step_join<true><<<g, b, 0, s>>>(p);
-  else attention_step_join<false><<<g, b, 0, s>>>(p);
+  if (f16) attention_step_join<true><<<g, dim3(1024), 0, s>>>(p);
+  else attention_step_join<false><<<g, dim3(1024), 0, s>>>(p);
 }
 
 }  // namespace vfa

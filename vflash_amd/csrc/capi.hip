@@ -147,7 +147,7 @@ bool out_args_ok(const void* out, int64_t ldo, int64_t m, int64_t n, int64_t pla
 // Sizes of a packed attention call.
 bool attention_sizes(vfa::AttentionParams& p, int64_t tokens, int64_t keys, int64_t batch, int64_t heads,
                      int64_t key_heads, int64_t dim) {
-  constexpr int64_t LIMIT = int64_t(1) << 31;
+  constexpr int64_t LIMIT = int64_t(1) << 30;
   if (tokens < 1 || tokens >= LIMIT || keys < 0 || keys >= LIMIT || batch < 0 || batch >= LIMIT) return false;
   if (key_heads < 1 || heads < key_heads || heads % key_heads || heads >= LIMIT / 2) return false;
   if (dim < 8 || dim > 128 || dim % 8) return false;

@@ -80,14 +80,14 @@ __global__ void __launch_bounds__(64 * WAVES) nvfp4_w16_few(const GemmParams p, 
   using L = W16Few<NB, MB, XR, KS, WAVES, NS>;
   constexpr int SUBS = 8 / NB;
   __shared__ __attribute__((aligned(1024))) uint8_t lds[L::LDS];
-  // A 128-row tile's workgroups run on one XCD, whose L2 then serves the scales and weights that
-  // they share.
-  const int per_tile = SUBS * blocks_m;
+  // The workgroups of a 128-row tile and a block of x rows run on one XCD, whose L2 then serves the
+  // scales and x rows that they share; the tiles and blocks go round the XCDs.
   const int xcd = (int)blockIdx.x & 7, j = (int)blockIdx.x >> 3;
-  const int64_t tile = (int64_t)(j / per_tile) * 8 + xcd;
-  if (tile >= p.n / 128) return;
-  const int sub = j % per_tile % SUBS;
-  const int64_t m0 = (int64_t)(j % per_tile / SUBS) * (16 * MB);
+  const int64_t group = (int64_t)(j / SUBS) * 8 + xcd, n_tiles = p.n / 128;
+  if (group >= n_tiles * blocks_m) return;
+  const int sub = j % SUBS;
+  const int64_t block = group / n_tiles, tile = group - block * n_tiles;
+  const int64_t m0 = block * (16 * MB);
   const int half = sub & 1, b0 = (sub >> 1) * NB;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int lane = (int)threadIdx.x & 63, i = lane & 15, g = lane >> 4;
@@ -353,9 +353,9 @@ namespace {
 template <bool F16, int NB, int MB, int XR, int KS, int WAVES, int NS>
 void launch_few(const GemmParams& p, hipStream_t s) {
   const int64_t blocks_m = (p.m + 16 * MB - 1) / (16 * MB);
-  const int64_t tiles = (p.n / 128 + 7) / 8 * 8;
+  const int64_t groups = (p.n / 128 * blocks_m + 7) / 8 * 8;
   nvfp4_w16_few<F16, NB, MB, XR, KS, WAVES, NS>
-      <<<dim3((unsigned)(tiles * (8 / NB) * blocks_m)), dim3(64 * WAVES), 0, s>>>(p, (int)blocks_m);
+      <<<dim3((unsigned)(groups * (8 / NB))), dim3(64 * WAVES), 0, s>>>(p, (int)blocks_m);
 }
 
 template <bool F16, int BM, int BN, int WGM, int NS>
