@@ -385,9 +385,9 @@ void launch_w16(const GemmParams& p, hipStream_t s) {
     if (p.n / 64 >= cus) launch_few<F16, 4, 1, 16, 128, 4, 2>(p, s);
     else launch_few<F16, 2, 1, 16, 128, 8, 3>(p, s);
   } else if (p.m <= 32) {
-    launch_few<F16, 4, 2, 32, 64, 8, 3>(p, s);
+    launch_few<F16, 4, 2, 32, 64, 8, 2>(p, s);
   } else if (!many_rows(p.m, p.n, cus)) {
-    launch_few<F16, 4, 4, 64, 64, 6, 2>(p, s);
+    launch_few<F16, 4, 4, 64, 64, 7, 2>(p, s);
   } else {
     launch_tile<F16, 128, 256, 1, 3>(p, s);
   }
