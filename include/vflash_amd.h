@@ -461,9 +461,9 @@ int vflash_nvfp4_w16_linear(const void* x, int x_is_f16, int64_t ldx, const void
  *        rows outside every sequence, are zeros.  Scores, softmax and sums are binary32;
  *        probabilities are rounded to the operands' type for their product with v.
  * Offsets and lengths are read on the device and clamped to the operands: values that decrease or
- * overlap give unspecified results, but nothing outside the operands is read or written.  A
- * masked key has no effect through k; its v enters with weight 0 if it lies in its sequence (0
- * times an infinity is NaN).
+ * overlap give unspecified results, but nothing outside the operands is read or written, and every
+ * row of out is.  A masked key has no effect through k; its v may enter with weight 0 if it lies in
+ * its sequence (0 times an infinity is NaN).  A row whose scores are all -inf is zeros.
  *   workspace  vflash_packed_attention_workspace(...) bytes (0: may be NULL), 16-byte aligned,
  *              without contents to keep; one call at a time
  *   Requires dim % 8 == 0, 8 <= dim <= 128, every stride a multiple of 8 and the pointers 16-byte

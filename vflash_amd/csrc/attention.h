@@ -21,9 +21,6 @@
 
 namespace vfa {
 
-typedef _Float16 v8hf __attribute__((ext_vector_type(8)));
-typedef _Float16 v2hf __attribute__((ext_vector_type(2)));
-typedef __bf16 v2bf16s __attribute__((ext_vector_type(2)));
 typedef short v4s16 __attribute__((ext_vector_type(4)));
 
 // Below every finite exponent: 2^(x - m) is 0 for a masked x = -inf, with no inf - inf.
@@ -50,25 +47,11 @@ __device__ __forceinline__ float attention_sum2(int pair, float l) {
   if constexpr (F16)
     return __builtin_amdgcn_fdot2(__builtin_bit_cast(v2hf, pair), v2hf{(_Float16)1.0f, (_Float16)1.0f}, l, false);
   else
-    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf16s, pair), v2bf16s{(__bf16)1.0f, (__bf16)1.0f}, l, false);
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, pair), v2bf{(__bf16)1.0f, (__bf16)1.0f}, l, false);
 }
 // A row's maximum as its statistics carry it: scaled, and finite where it saw nothing.
 __device__ __forceinline__ float attention_top(float m, float c) { return fmaxf(m * c, VFA_LOWEST); }
 
-template <bool F16>
-__device__ __forceinline__ v16f mfma32(v4i a, v4i b, v16f c) {
-  if constexpr (F16)
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8hf, a), __builtin_bit_cast(v8hf, b), c, 0, 0, 0);
-  else
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
-}
-template <bool F16>
-__device__ __forceinline__ v4f mfma16(v4i a, v4i b, v4f c) {
-  if constexpr (F16)
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8hf, a), __builtin_bit_cast(v8hf, b), c, 0, 0, 0);
-  else
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
-}
 // Two values to the operand type, to nearest even.  Not pack_bf16x2: the values come from
 // v_exp_f32, whose result the next instruction may not read yet, and the compiler places the wait
 // states for its own instructions only.

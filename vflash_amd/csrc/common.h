@@ -260,4 +260,26 @@ __device__ __forceinline__ uint32_t f32_to_e2m1(float f) {
   return c | ((__float_as_uint(f) >> 28) & 8u);
 }
 
+// D = A B + C of 16-bit operands, binary16 or bfloat16: 32x32 outputs over 16 K, 16x16 over 32.
+typedef _Float16 v2hf __attribute__((ext_vector_type(2)));
+typedef _Float16 v8hf __attribute__((ext_vector_type(8)));
+template <bool F16>
+__device__ __forceinline__ v16f mfma32(v4i a, v4i b, v16f c) {
+  if constexpr (F16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8hf, a), __builtin_bit_cast(v8hf, b), c, 0,
+                                                  0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0,
+                                                  0, 0);
+}
+template <bool F16>
+__device__ __forceinline__ v4f mfma16(v4i a, v4i b, v4f c) {
+  if constexpr (F16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8hf, a), __builtin_bit_cast(v8hf, b), c, 0,
+                                                  0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0,
+                                                  0, 0);
+}
+
 }  // namespace vfa

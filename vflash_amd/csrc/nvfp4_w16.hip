@@ -18,9 +18,6 @@
 
 namespace vfa {
 
-typedef _Float16 w16_v2h __attribute__((ext_vector_type(2)));
-typedef _Float16 w16_v8h __attribute__((ext_vector_type(8)));
-
 // The eight values of packed word d times their block scale, as an MFMA operand.
 template <bool F16>
 __device__ __forceinline__ v4i w16_restore(uint32_t d, float s) {
@@ -28,7 +25,7 @@ __device__ __forceinline__ v4i w16_restore(uint32_t d, float s) {
   static_for<4>([&](auto i) {
     if constexpr (F16) {
       const _Float16 h = (_Float16)s;  // exact, as every E4M3 value
-      o[(int)i] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(d, 1.0f, (int)i) * w16_v2h{h, h});
+      o[(int)i] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(d, 1.0f, (int)i) * v2hf{h, h});
     } else {
       const v2f y = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(d, 1.0f, (int)i);
       const float a = y[0] * s, b = y[1] * s;
@@ -38,21 +35,6 @@ __device__ __forceinline__ v4i w16_restore(uint32_t d, float s) {
   return o;
 }
 
-template <bool F16>
-__device__ __forceinline__ v16f w16_mfma32(v4i a, v4i b, v16f c) {
-  if constexpr (F16)
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(w16_v8h, a), __builtin_bit_cast(w16_v8h, b), c, 0, 0, 0);
-  else
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
-}
-template <bool F16>
-__device__ __forceinline__ v4f w16_mfma16(v4i a, v4i b, v4f c) {
-  if constexpr (F16)
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(w16_v8h, a), __builtin_bit_cast(w16_v8h, b), c, 0, 0, 0);
-  else
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
-}
-
 // ---------------------------------------------------------------------------
 // Few rows.  A workgroup computes 16 MB rows of x times 16 NB rows of the weight.  Its waves take
 // every WAVES-th stage of KS K each, through an LDS ring of their own that DMA fills NS stages
@@ -60,6 +42,10 @@ __device__ __forceinline__ v4f w16_mfma16(v4i a, v4i b, v4f c) {
 // operands' lane order would do without LDS, but neighbouring lanes hold different rows there: at an
 // access per 16 bytes the vector cache alone took 20 us of the 31 that 64 x 5120 x 15360 then took.
 // The 16-row blocks of a workgroup lie 32 rows apart, as the scales of one 16-byte run do.
+//
+// Bound by the weight's bytes from one row to a few where it is large (1 x 5376 x 28672 in f16 16.7 us,
+// 5.2 TB/s), by one launch's latency where it is small (1 x 5120 x 5120 6.9), and at 64 rows by x,
+// which every workgroup takes through L2 and LDS (64 x 5120 x 15360 20.6, 2.3 TB/s of all bytes).
 //
 // Lane group g takes K g KS / 4 .. of a stage, so that it reads its packed values at once: step v of
 // 32 K multiplies K g KS / 4 + 8 v .. + 7 of each group.
@@ -156,7 +142,7 @@ __global__ void __launch_bounds__(64 * WAVES) nvfp4_w16_few(const GemmParams p, 
       });
       static_for<NB>([&](auto b) {
         const v4i o = w16_restore<F16>(w[b][v], sc[b][v / 2]);
-        static_for<MB>([&](auto m) { acc[b][m] = w16_mfma16<F16>(o, x[m], acc[b][m]); });
+        static_for<MB>([&](auto m) { acc[b][m] = mfma16<F16>(o, x[m], acc[b][m]); });
       });
     });
     __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the slot is read
@@ -195,7 +181,8 @@ __global__ void __launch_bounds__(64 * WAVES) nvfp4_w16_few(const GemmParams p, 
 // 512 bytes of scales per 128 weight rows) in an LDS ring that DMA fills NS - 1 stages ahead,
 // with one barrier a stage.  K goes to the lanes as in w8a16_gemm.hip: a lane reads 64 bytes of an
 // activation row and 16 of a packed row.  Four waves lie side by side along N where the tile is
-// wide, so that none restores another's weights.  Each of a stage's four steps multiplies while the
+// wide, so that none restores another's weights; 1021 x 5120 x 13824 126 us, 1.15 PFLOP/s on a grid that
+// fills 84 % of its two rounds.  Each of a stage's four steps multiplies while the
 // next one's operands are read and restored between its MFMAs.
 template <int BM, int BN, int NS>
 struct W16Tile {
@@ -284,7 +271,7 @@ __global__ void __launch_bounds__(256, 2) nvfp4_w16_pipe(const GemmParams p) {
   constexpr int VALU = (F16 ? 10 : 18) * NB / (NB * MB) + 1;
   auto multiply = [&](const Step& o) {
     static_for<NB>([&](auto nb) {
-      static_for<MB>([&](auto mb) { acc[nb][mb] = w16_mfma32<F16>(o.w[nb], o.a[mb], acc[nb][mb]); });
+      static_for<MB>([&](auto mb) { acc[nb][mb] = mfma32<F16>(o.w[nb], o.a[mb], acc[nb][mb]); });
     });
     static_for<NB * MB>([&](auto) {
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
