@@ -161,6 +161,15 @@ struct AttentionItem {
   bool live;
 };
 
+// a / b of values that a wave shares; most are small enough to go without the division.
+__device__ __forceinline__ uint32_t attention_quotient(uint32_t a, uint32_t b) {
+  return a < b ? 0 : a < 2 * b ? 1 : b == 1 ? a : a / b;
+}
+// The key head of a head block, and which of its parts this is.
+__device__ __forceinline__ int attention_key_head(const AttentionParams& p, int head_block) {
+  return p.parts == 1 ? head_block : head_block / p.parts;
+}
+
 // Which of `total` units of which head block workgroup `index` takes; false: none.
 // Workgroup b runs on XCD b % 8.  Where the head blocks divide among the XCDs, each XCD takes whole
 // ones, one after another, so that its L2 holds their keys.  Causal tiles differ in length: a
@@ -170,14 +179,14 @@ __device__ __forceinline__ bool attention_place(const AttentionParams& p, uint32
   if (total == 0) return false;
   if (p.head_blocks % 8 == 0) {
     const int i = (int)(index >> 3), each = p.head_blocks / 8;
-    const int local = (int)((uint32_t)i / (uint32_t)total);
+    const int local = (int)attention_quotient((uint32_t)i, (uint32_t)total);
     if (local >= each) return false;
     head_block = (int)(index & 7) + 8 * local;
     x = i - local * total;
     if (p.causal && (each - 1 - local) % 2) x = total - 1 - x;
     return true;
   }
-  x = (int)(index / (uint32_t)p.head_blocks);
+  x = (int)attention_quotient(index, (uint32_t)p.head_blocks);
   head_block = (int)index - x * p.head_blocks;
   return x < total;
 }
@@ -302,10 +311,11 @@ struct AttentionRow {
 __device__ __forceinline__ int attention_token_of(const AttentionParams& p, int r) { return (r * p.row_mul) >> 16; }
 __device__ __forceinline__ AttentionRow attention_row(const AttentionParams& p, const AttentionItem& it, int r) {
   const int in = attention_token_of(p, r);
-  const int h = it.head_block % p.parts * p.heads_per_tile + r - in * p.heads_per_tile;
+  const int key_head = attention_key_head(p, it.head_block);
+  const int h = (it.head_block - key_head * p.parts) * p.heads_per_tile + r - in * p.heads_per_tile;
   AttentionRow row;
   row.token = it.tile * p.tile_tokens + in;
-  row.head = it.head_block / p.parts * p.group + h;
+  row.head = key_head * p.group + h;
   row.live = in < p.tile_tokens && row.token < it.seq.nq && h < p.group;
   return row;
 }
@@ -323,7 +333,7 @@ __device__ __forceinline__ int attention_limit(const AttentionParams& p, const A
   return p.causal ? max(0, min(s.nk, s.nk - s.nq + token + 1)) : s.nk;
 }
 
-// The schedule of attention_step.  Every tile is a number of units (p.unit_keys keys each, one at
+// The schedule of attention_step.  Every tile is a number of units (2^p.unit_shift keys each, one at
 // least), the units of all tiles of a head block form a line, the head blocks' lines one after
 // another a longer one, and each workgroup takes the next p.grid-th part of that: equal work whatever
 // the lengths.  A workgroup whose part ends inside a tile leaves a partial sum, of which it has at
@@ -332,7 +342,7 @@ __device__ __forceinline__ int attention_limit(const AttentionParams& p, const A
 struct AttentionLine {
   uint32_t units;       // per head block
   uint32_t quota, end;  // of a workgroup; of the line
-  uint32_t unit_keys;
+  int unit_shift;
   int xcds;             // 8: the line is one XCD's
   AttentionSeq mine;    // of this lane, where there are at most 64 sequences
 };
@@ -342,13 +352,13 @@ struct AttentionSegment {
 };
 
 __device__ __forceinline__ uint32_t attention_units_of(const AttentionLine& l, const AttentionSeq& s) {
-  return max(1u, ((uint32_t)s.nk + l.unit_keys - 1) / l.unit_keys);
+  return max(1u, ((uint32_t)s.nk + (1u << l.unit_shift) - 1) >> l.unit_shift);
 }
 
 __device__ __forceinline__ AttentionLine attention_line(const AttentionParams& p, int grid) {
   const int lane = (int)threadIdx.x & 63;
   AttentionLine l{};
-  l.unit_keys = (uint32_t)p.unit_keys;
+  l.unit_shift = p.unit_shift;
   int reached = 0;
   for (int64_t base = 0; base < p.batch + 2; base += 64) {
     l.mine = attention_sequence(p, base, reached);
@@ -357,9 +367,10 @@ __device__ __forceinline__ AttentionLine attention_line(const AttentionParams& p
     l.units += (uint32_t)sum;
   }
   l.xcds = p.head_blocks % 8 == 0 ? 8 : 1;
-  l.end = l.units * (uint32_t)(p.head_blocks / l.xcds);
-  const uint32_t parts = (uint32_t)(grid / l.xcds);
-  l.quota = max(1u, (l.end + parts - 1) / parts);
+  const int shift = l.xcds == 8 ? 3 : 0;
+  l.end = l.units * (uint32_t)(p.head_blocks >> shift);
+  const uint32_t parts = (uint32_t)grid >> shift;
+  l.quota = max(1u, attention_quotient(l.end + parts - 1, parts));
   return l;
 }
 
@@ -369,7 +380,7 @@ __device__ __forceinline__ AttentionSegment attention_segment(const AttentionPar
   const int lane = (int)threadIdx.x & 63;
   const int64_t n = p.batch + 2;
   AttentionSegment g{};
-  const uint32_t local = pos / line.units, x = pos - local * line.units;
+  const uint32_t local = attention_quotient(pos, line.units), x = pos - local * line.units;
   g.it.head_block = line.xcds == 8 ? (b & 7) + 8 * (int)local : (int)local;
   uint32_t before = 0;
   int reached = 0;
@@ -384,7 +395,7 @@ __device__ __forceinline__ AttentionSegment attention_segment(const AttentionPar
       g.it.seq = AttentionSeq{pick(mine.q0), pick(mine.k0), pick(mine.nq), pick(mine.nk)};
       g.of = (uint32_t)pick((int)u);
       const uint32_t in = x - before - (uint32_t)pick((int)(incl - own));
-      g.it.tile = (int)(in / g.of);
+      g.it.tile = (int)attention_quotient(in, g.of);
       g.first = in - (uint32_t)g.it.tile * g.of;
       g.count = min(g.of - g.first, stop - pos);
       g.it.live = true;

@@ -51,7 +51,7 @@ __global__ void __launch_bounds__(64 * WAVES, DP <= 64 ? 4 : 3) attention_tiles(
   const uint32_t base_lds = __builtin_amdgcn_readfirstlane(lds_addr(lds));
 
   const AttentionRow row = attention_row(p, it, wave * 32 + fr);
-  const int part_head = it.head_block / p.parts;
+  const int part_head = attention_key_head(p, it.head_block);
   // Keys of this item: [first, last), last no further than the tile's last token sees.
   const int last_token = min(it.seq.nq, (it.tile + 1) * p.tile_tokens) - 1;
   const int tile_limit = attention_limit(p, it.seq, last_token);
@@ -293,9 +293,9 @@ AttentionPlan attention_plan(AttentionParams& p) {
   if (plan.step) {
     // A CU holds one workgroup of dimension 128, two of 64.
     const bool split = p.keys > 768 && p.keys > 512 * p.batch;
-    p.unit_keys = split ? 128 : INT32_MAX;
-    auto bound = [&] { return tiles * p.head_blocks * (((int64_t)p.keys + p.unit_keys - 1) / p.unit_keys + 1); };
-    while (bound() >= int64_t(1) << 30 && p.unit_keys < 1 << 29) p.unit_keys *= 2;  // the kernel counts in 32 bits
+    p.unit_shift = split ? 7 : 31;
+    auto bound = [&] { return tiles * p.head_blocks * (((int64_t)p.keys >> p.unit_shift) + 1); };
+    while (bound() >= int64_t(1) << 30 && p.unit_shift < 31) ++p.unit_shift;  // the kernel counts in 32 bits
     const int64_t units = bound();
     plan.grid = (cus + 7) / 8 * 8 * (p.dim <= 64 ? 2 : 1);
     if (units < plan.grid) plan.grid = (units + 7) / 8 * 8;

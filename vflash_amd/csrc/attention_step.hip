@@ -8,7 +8,7 @@
 // Each wave takes every fourth block of 32 keys of the item and keeps a ring of two in LDS, which
 // its own DMA fills: 128 KB a CU in flight or in use, no barrier before the end, where the four
 // waves' sums are added up.  131071 keys of 8 heads of 128: 107 us, 5.0 TB/s, what a copy of 1 GiB
-// reaches; 16 sequences of up to 8191: 64 us, 4.3 TB/s; 77 keys: 5.5 us on the GPU, latency alone.
+// reaches; 16 sequences of up to 8191: 64 us, 4.3 TB/s; 77 keys: 7.4 us a call, latency alone.
 #include "attention.h"
 
 namespace vfa {
@@ -44,17 +44,17 @@ __global__ void __launch_bounds__(256, 1) attention_step(const AttentionParams p
   const uint32_t ring_lds = __builtin_amdgcn_readfirstlane(lds_addr(ring));
 
   const AttentionLine line = attention_line(p, gridDim.x);
-  const uint32_t begin = (blockIdx.x / line.xcds) * line.quota, stop = min(begin + line.quota, line.end);
+  const uint32_t begin = (blockIdx.x >> (line.xcds == 8 ? 3 : 0)) * line.quota, stop = min(begin + line.quota, line.end);
   for (uint32_t pos = begin; pos < stop;) {
     const AttentionSegment seg = attention_segment(p, line, blockIdx.x, pos, stop);
     const AttentionItem& it = seg.it;
     if (!it.live) return;
     const AttentionRow row = attention_row(p, it, fr);
-    const int key_head = it.head_block / p.parts;
+    const int key_head = attention_key_head(p, it.head_block);
     const int last_token = min(it.seq.nq, (it.tile + 1) * p.tile_tokens) - 1;
     const int tile_limit = attention_limit(p, it.seq, last_token);
-    const int first = (int)min(seg.first * (uint64_t)line.unit_keys, (uint64_t)INT32_MAX);
-    const int last = (int)min((uint64_t)tile_limit, (seg.first + seg.count) * (uint64_t)line.unit_keys);
+    const int first = (int)min((uint64_t)seg.first << line.unit_shift, (uint64_t)INT32_MAX);
+    const int last = (int)min((uint64_t)tile_limit, (uint64_t)(seg.first + seg.count) << line.unit_shift);
     const int limit = row.live ? min(attention_limit(p, it.seq, row.token), last) : last;
     // Keys that every row sees.
     const int open = min(attention_limit(p, it.seq, min(it.tile * p.tile_tokens, it.seq.nq)), last);
@@ -195,7 +195,7 @@ __global__ void __launch_bounds__(256, 1) attention_step(const AttentionParams p
 template <bool F16>
 __global__ void __launch_bounds__(1024) attention_step_join(const AttentionParams p) {
   const AttentionLine line = attention_line(p, gridDim.x);
-  const int part = blockIdx.x / line.xcds;
+  const int part = blockIdx.x >> (line.xcds == 8 ? 3 : 0);
   const uint32_t begin = part * line.quota, stop = min(begin + line.quota, line.end);
   if (begin >= stop) return;
   const AttentionSegment seg = attention_segment(p, line, blockIdx.x, stop - 1, line.end);
