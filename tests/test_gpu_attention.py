@@ -163,6 +163,17 @@ def test_scores_that_rise_and_fall(dev):
                 check(packed_attention(q, k, v, qo, ko, scale=1.0), q, k, v, qo, ko, scale=1.0)
 
 
+def test_large_values_under_rising_scores(dev):
+    # Weights above 1 until the maximum follows: sums of large values stay in binary32.
+    n = 700
+    for nq in (1, 90):
+        q, k, v = make(dev, [nq], [n], 2, 1, 128, BF16, std=0.5)
+        q[..., 0], k[:, 0, 0] = 1.0, (torch.arange(n, device=dev) * 0.05).to(BF16)
+        v = (v.float() * 1e28).to(BF16)
+        qo, ko = offsets([nq], dev), offsets([n], dev)
+        check(packed_attention(q, k, v, qo, ko, scale=1.0), q, k, v, qo, ko, scale=1.0)
+
+
 def test_binary16_keeps_small_probabilities(dev):
     # One score 17 above 60000 equal ones: each of these weighs 2^-24.5, together 2.5e-3.
     n = 60000

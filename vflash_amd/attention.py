@@ -35,7 +35,9 @@ def packed_attention(q, k, v, q_offsets, k_offsets, *, k_lengths=None, causal=Fa
     and query ``i`` of ``nq`` sees the keys ``j <= i + nk - nq``.  Rows that see no key, and
     rows outside every sequence, are zeros.  ``scale`` defaults to ``dim ** -0.5``.
 
-    Offsets are read on the device, clamped to the operands.  Inference only.
+    Offsets are read on the device, clamped to the operands.  A masked key has no effect,
+    whatever it holds; infinities and NaN in its *value* may, as 0 times them is NaN, if it lies in its
+    sequence.  Inference only.
     """
     if isinstance(q, torch.Tensor) and q.is_cuda:
         # The whole call in native code; None sends any other layout, and every refusal, on from here.

@@ -26,11 +26,12 @@ typedef short v4s16 __attribute__((ext_vector_type(4)));
 // Below every finite exponent: 2^(x - m) is 0 for a masked x = -inf, with no inf - inf.
 #define VFA_LOWEST (-3.4028234663852886e38f)
 // m follows the scores only where the weights of a block of keys would pass a bound: 2^15 keeps
-// binary16 from overflowing, and bfloat16 has binary32's range.  A rounding is relative, so a
-// weight above 1 loses nothing; in binary16 it carries 2^6 more, which keeps 20 binary orders
-// below m out of the format's subnormals.
+// binary16 from overflowing, and 2^20 leaves the sums room for values to 2^100.  A rounding is
+// relative, so a weight above 1 loses nothing; in binary16 it carries 2^6 more, which keeps 20
+// binary orders below m out of the format's subnormals.  Tiles of few rows, which wait for their
+// keys, follow the maximum itself, once it is 2^8 above.
 template <bool F16>
-constexpr float kAttentionBound = F16 ? 32768.0f : 1152921504606846976.0f;  // 2^60
+constexpr float kAttentionBound = F16 ? 32768.0f : 1048576.0f;
 constexpr float kAttentionSlack = 8.0f;
 constexpr float kAttentionFar = 4194304.0f;  // 2^22: a rounding of 1/4
 template <bool F16>
