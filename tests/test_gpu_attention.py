@@ -1,5 +1,7 @@
 """Packed attention on the GPU against its definition in 64 bits."""
 
+import math
+
 import pytest
 import torch
 
@@ -185,6 +187,23 @@ def test_binary16_keeps_small_probabilities(dev):
     v[4] = 0
     qo, ko = offsets([1], dev), offsets([n], dev)
     check(packed_attention(q, k, v, qo, ko, scale=1.0), q, k, v, qo, ko, scale=1.0)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("n", [700, 5000])
+@pytest.mark.parametrize("nq", [1, 40])
+def test_weights_are_normalised_as_rounded(dev, nq, n, dtype):
+    # Every 32nd key weighs 1, the others just below the middle of two 16-bit numbers, so that all of them
+    # round down by half a step; a value that the keys share comes back exactly all the same.
+    half = torch.finfo(dtype).eps / 2
+    weight = 0.5 * (1 + half) * (1 - half / 16)
+    q = torch.zeros((nq, 1, 64), device=dev, dtype=dtype)
+    q[..., 0] = 1.0
+    k = torch.full((n, 1, 64), -1.0, device=dev, dtype=dtype)
+    k[::32] = 0.0
+    v = torch.full((n, 1, 64), 1.0, device=dev, dtype=dtype)
+    got = packed_attention(q, k, v, offsets([nq], dev), offsets([n], dev), scale=-math.log(weight))
+    assert torch.equal(got, torch.ones_like(got))
 
 
 def test_many_sequences(dev):

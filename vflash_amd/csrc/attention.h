@@ -42,7 +42,9 @@ template <bool F16, bool FAR>
 __device__ __forceinline__ float attention_weight(float s, float c, float m, float ref) {
   return __builtin_amdgcn_exp2f(FAR ? (s - m) * c + kAttentionShift<F16> : __builtin_fmaf(s, c, ref));
 }
-// l plus the two weights of a packed pair, as they were rounded: the sum that normalises them.
+// l plus the two weights of a packed pair, as they were rounded: the sum that normalises them, in
+// every kernel, so that what their roundings have in common cancels (a value that all keys share
+// comes back as it is).
 template <bool F16>
 __device__ __forceinline__ float attention_sum2(int pair, float l) {
   if constexpr (F16)

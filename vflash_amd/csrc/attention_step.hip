@@ -130,11 +130,9 @@ __global__ void __launch_bounds__(256, 1) attention_step(const AttentionParams p
       auto weights = [&](auto far_rows) {
         static_for<4>([&](auto j) {
           constexpr int r = (j % 2) * 2;
-          const float a = attention_weight<F16, far_rows>(s[j / 2][r], p.c, m, ref);
-          const float b = attention_weight<F16, far_rows>(s[j / 2][r + 1], p.c, m, ref);
-          l += a;
-          l += b;
-          pk[(int)j] = pack2<F16>(a, b);
+          pk[(int)j] = pack2<F16>(attention_weight<F16, far_rows>(s[j / 2][r], p.c, m, ref),
+                                  attention_weight<F16, far_rows>(s[j / 2][r + 1], p.c, m, ref));
+          l = attention_sum2<F16>(pk[(int)j], l);
         });
       };
       if (far) weights(std::true_type{});
