@@ -459,7 +459,8 @@ int vflash_nvfp4_w16_linear(const void* x, int x_is_f16, int64_t ldx, const void
  *   causal    query i of a sequence of nq queries and nk keys sees the keys j <= i + nk - nq
  *   out  [tokens, heads, dim] of the same type, elements at t * o_ts + h * o_hs + d.  Rows that see no key, and
  *        rows outside every sequence, are zeros.  Scores, softmax and sums are binary32;
- *        probabilities are rounded to the operands' type for their product with v.
+ *        probabilities are rounded to the operands' type for their product with v.  Every finite v
+ *        has its place in the sums; bf16 values below 2^-118 times `keys` may lose bits.
  * Offsets and lengths are read on the device and clamped to the operands: values that decrease or
  * overlap give unspecified results, but nothing outside the operands is read or written, and every
  * row of out is.  A masked key has no effect through k; its v may enter with weight 0 if it lies in

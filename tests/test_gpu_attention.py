@@ -176,6 +176,22 @@ def test_large_values_under_rising_scores(dev):
         check(packed_attention(q, k, v, qo, ko, scale=1.0), q, k, v, qo, ko, scale=1.0)
 
 
+@pytest.mark.parametrize("nq,n", [(1, 700), (90, 700), (1, 20000), (40, 20000), (300, 3000)])
+@pytest.mark.parametrize("step", [0.0, 0.05, -0.05])
+@pytest.mark.parametrize("size", [1e-30, 1e36, 3.3895e38], ids=str)
+def test_every_finite_value(dev, nq, n, step, size):
+    # The sum before its normalisation stays finite up to bf16's largest values, under equal, rising and
+    # falling scores, in one part and in several.
+    q, k, v = make(dev, [nq], [n], 2, 1, 128, BF16, std=0.5)
+    q[..., 0], k[:, 0, 0] = 1.0, ((torch.arange(n, device=dev) % 700) * step).to(BF16)
+    if step == 0.0:
+        q.zero_()
+    v = (v.sign() * size).to(BF16)
+    v[:, :, :8] = size
+    qo, ko = offsets([nq], dev), offsets([n], dev)
+    check(packed_attention(q, k, v, qo, ko, scale=1.0), q, k, v, qo, ko, scale=1.0)
+
+
 def test_binary16_keeps_small_probabilities(dev):
     # One score 17 above 60000 equal ones: each of these weighs 2^-24.5, together 2.5e-3.
     n = 60000

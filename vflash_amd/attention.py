@@ -37,7 +37,8 @@ def packed_attention(q, k, v, q_offsets, k_offsets, *, k_lengths=None, causal=Fa
 
     Offsets are read on the device, clamped to the operands.  A masked key has no effect,
     whatever it holds; infinities and NaN in its *value* may, as 0 times them is NaN, if it lies in its
-    sequence.  Inference only.
+    sequence.  No sum of finite values overflows; bf16 values below 2^-118 times the rows of ``k`` may
+    lose bits to binary32's subnormals.  Inference only.
     """
     if isinstance(q, torch.Tensor) and q.is_cuda:
         # The whole call in native code; None sends any other layout, and every refusal, on from here.

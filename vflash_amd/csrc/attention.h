@@ -25,22 +25,25 @@ typedef short v4s16 __attribute__((ext_vector_type(4)));
 
 // Below every finite exponent: 2^(x - m) is 0 for a masked x = -inf, with no inf - inf.
 #define VFA_LOWEST (-3.4028234663852886e38f)
-// m follows the scores only where the weights of a block of keys would pass a bound: 2^15 keeps
-// binary16 from overflowing, and 2^20 leaves the sums room for values to 2^100.  A rounding is
-// relative, so a weight above 1 loses nothing; in binary16 it carries 2^6 more, which keeps 20
-// binary orders below m out of the format's subnormals.  Tiles of few rows, which wait for their
-// keys, follow the maximum itself, once it is 2^8 above.
+// A weight carries 2^shift, and m follows the scores only where a block's weights would sum up to more
+// than a bound above that.  A rounding is relative, so a weight above that of m loses nothing.
+// bf16: 2^20 above, and a shift by which all keys at the bound sum up to 2^-1: no sum of finite values
+// overflows before it is normalised (values below 2^(-126 - shift) enter it as subnormals).  A bound of
+// 2^9 instead costs 5 % where the scores spread by 10 and 8 % where they rise by 0.05 a key (6000
+// tokens, 16 heads of 128: 300 and 306 us).  f16: 2^6 keeps 20 binary orders below m out of the weights'
+// subnormals, and 2^15 them from overflowing.  Tiles of few rows, which wait for their keys, follow the
+// maximum itself, once it is 2^8 above.
 template <bool F16>
-constexpr float kAttentionBound = F16 ? 32768.0f : 1048576.0f;
+__device__ __forceinline__ float attention_shift(const AttentionParams& p) { return F16 ? 6.0f : p.shift; }
+template <bool F16>
+__device__ __forceinline__ float attention_bound(const AttentionParams& p) { return F16 ? 32768.0f : p.bound; }
 constexpr float kAttentionSlack = 8.0f;
 constexpr float kAttentionFar = 4194304.0f;  // 2^22: a rounding of 1/4
-template <bool F16>
-constexpr float kAttentionShift = F16 ? 6.0f : 0.0f;
 
-// 2^(c (s - m)) times 2^shift, m the row's maximum before its scaling.
-template <bool F16, bool FAR>
-__device__ __forceinline__ float attention_weight(float s, float c, float m, float ref) {
-  return __builtin_amdgcn_exp2f(FAR ? (s - m) * c + kAttentionShift<F16> : __builtin_fmaf(s, c, ref));
+// 2^(c (s - m)) times 2^shift, m the row's maximum before its scaling (ref = shift - c m).
+template <bool FAR>
+__device__ __forceinline__ float attention_weight(float s, float c, float m, float ref, float shift) {
+  return __builtin_amdgcn_exp2f(FAR ? (s - m) * c + shift : __builtin_fmaf(s, c, ref));
 }
 // l plus the two weights of a packed pair, as they were rounded: the sum that normalises them, in
 // every kernel, so that what their roundings have in common cancels (a value that all keys share

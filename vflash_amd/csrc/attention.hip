@@ -136,20 +136,20 @@ __global__ void __launch_bounds__(64 * WAVES, DP <= 64 ? 4 : 3) attention_tiles(
     v4i pk[2 * L::KB];
     float sum;
     auto weights = [&](auto far_rows) {
-      const float ref = kAttentionShift<F16> - attention_top(m, p.c);
+      const float ref = attention_shift<F16>(p) - attention_top(m, p.c);
       sum = 0;
       static_for<2 * L::KB>([&](auto st) {
         static_for<4>([&](auto j) {
           constexpr int r = (st % 2) * 8 + 2 * j;
-          pk[st][(int)j] = pack2<F16>(attention_weight<F16, far_rows>(s[st / 2][r], p.c, m, ref),
-                                      attention_weight<F16, far_rows>(s[st / 2][r + 1], p.c, m, ref));
+          pk[st][(int)j] = pack2<F16>(attention_weight<far_rows>(s[st / 2][r], p.c, m, ref, attention_shift<F16>(p)),
+                                      attention_weight<far_rows>(s[st / 2][r + 1], p.c, m, ref, attention_shift<F16>(p)));
           sum = attention_sum2<F16>(pk[st][(int)j], sum);
         });
       });
     };
     if (far) weights(std::true_type{});
     else weights(std::false_type{});
-    if (__builtin_amdgcn_ballot_w64(!(sum <= kAttentionBound<F16>))) {
+    if (__builtin_amdgcn_ballot_w64(!(sum <= attention_bound<F16>(p)))) {
       // The first keys that a row sees, or scores far above those before.
       float mx = s[0][0];
       static_for<16 * L::KB - 1>([&](auto r) { mx = fmaxf(mx, s[(r + 1) / 16][(int)((r + 1) % 16)]); });
@@ -344,6 +344,10 @@ bool attention_fits(const AttentionParams& params) {
 hipError_t launch_attention(const AttentionParams& params, bool f16, void* workspace, hipStream_t s) {
   AttentionParams p = params;
   const AttentionPlan plan = attention_plan(p);
+  int log = 0;  // at most 2^log keys
+  while ((int64_t(1) << log) < p.keys) ++log;
+  p.shift = -(float)(21 + log);
+  p.bound = exp2f(20.0f + p.shift);
   p.part = static_cast<float*>(workspace);
   p.part_ml = p.part + p.slots * plan.rows * p.dim;
   if (plan.step) {

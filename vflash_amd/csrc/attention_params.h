@@ -14,6 +14,7 @@ struct AttentionParams {
   int heads, group, dim;  // group: query heads of a key head
   int causal;
   float c;  // scale * log2(e)
+  float shift, bound;  // of bf16 weights: attention_shift, attention_bound
   // The tiles' shape.
   int heads_per_tile;  // of a key head's group; a group of more than the tile's rows has `parts` blocks
   int parts, head_blocks;

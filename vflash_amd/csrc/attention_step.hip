@@ -125,13 +125,13 @@ __global__ void __launch_bounds__(256, 1) attention_step(const AttentionParams p
         m = next;
         far = __builtin_amdgcn_ballot_w64(fabsf(m * p.c) >= kAttentionFar && m > VFA_LOWEST) != 0;
       }
-      const float ref = kAttentionShift<F16> - attention_top(m, p.c);
+      const float ref = attention_shift<F16>(p) - attention_top(m, p.c);
       v4i pk;
       auto weights = [&](auto far_rows) {
         static_for<4>([&](auto j) {
           constexpr int r = (j % 2) * 2;
-          pk[(int)j] = pack2<F16>(attention_weight<F16, far_rows>(s[j / 2][r], p.c, m, ref),
-                                  attention_weight<F16, far_rows>(s[j / 2][r + 1], p.c, m, ref));
+          pk[(int)j] = pack2<F16>(attention_weight<far_rows>(s[j / 2][r], p.c, m, ref, attention_shift<F16>(p)),
+                                  attention_weight<far_rows>(s[j / 2][r + 1], p.c, m, ref, attention_shift<F16>(p)));
           l = attention_sum2<F16>(pk[(int)j], l);
         });
       };
