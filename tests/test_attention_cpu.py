@@ -4,6 +4,7 @@ import ctypes
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fw
 
 from tests.launches import LIBRARY, launches
 from vflash_amd import _lib
@@ -44,6 +45,20 @@ def test_refusals():
     for scale in (0.0, -1.0, float("inf"), float("nan")):
         refused("scale", a, scale=scale)
     refused("inference-only", [a[0].requires_grad_(), *a[1:]])
+
+
+def test_forward_mode_is_refused():
+    # A tangent that the kernel would drop, on each operand, gradients recorded or not.
+    for recorded in (True, False):
+        with torch.set_grad_enabled(recorded), fw.dual_level():
+            for i in range(3):
+                a = operands()
+                a[i] = fw.make_dual(a[i], torch.ones_like(a[i]))
+                with pytest.raises(ValueError, match="inference-only"):
+                    packed_attention(*a)
+    a = operands()
+    with pytest.raises(ValueError, match="inference-only"):
+        torch.func.jvp(lambda q: packed_attention(q, *a[1:]), (a[0],), (a[0],))
 
 
 def entry(**change):

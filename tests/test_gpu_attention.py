@@ -4,6 +4,7 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fw
 
 from tests.attention_reference import check
 from vflash_amd import _lib, kernels
@@ -301,6 +302,19 @@ def test_native_host_path(dev):
                  (q[:, :3], k, v, qo, ko, None, True, None), (q[:0], k, v, qo, ko, None, True, None),
                  (q.float(), k.float(), v.float(), qo, ko, None, True, None)):
         assert host.packed_attention(*args) is None
+
+
+def test_forward_mode_is_refused(dev):
+    q, k, v = make(dev, [4], [9], 4, 2, 64, BF16)
+    qo, ko = offsets([4], dev), offsets([9], dev)
+    with torch.no_grad(), fw.dual_level():
+        for i in range(3):
+            a = [q, k, v]
+            a[i] = fw.make_dual(a[i], torch.ones_like(a[i]))
+            assert _lib.host().packed_attention(*a, qo, ko, None, True, None) is None
+            with pytest.raises(ValueError, match="inference-only"):
+                packed_attention(*a, qo, ko, causal=True)
+        assert _lib.host().packed_attention(q, k, v, qo, ko, None, True, None) is not None
 
 
 def test_no_rows(dev):

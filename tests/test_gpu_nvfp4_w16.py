@@ -2,6 +2,7 @@
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fw
 
 from vflash_amd import _lib, kernels
 from vflash_amd.nvfp4_linear import NVFP4Execution, NVFP4Weight
@@ -164,3 +165,13 @@ def test_refusals(dev):
         with pytest.raises(ValueError):
             ex.linear(*args)
     assert ex.calls == 0 and ex.rows == 0
+
+
+def test_forward_mode_is_refused(dev):
+    x, weight, b = make(dev, 4, 128, 64, BF16)
+    ex = NVFP4Execution("unquantized")
+    with torch.no_grad(), fw.dual_level():
+        for values, bias in ((fw.make_dual(x, torch.ones_like(x)), b), (x, fw.make_dual(b, torch.ones_like(b)))):
+            with pytest.raises(ValueError, match="inference-only"):
+                ex.linear(values, weight, bias)
+    assert ex.calls == 0

@@ -4,6 +4,7 @@ import ctypes
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fw
 
 from tests.launches import LIBRARY, launches
 from vflash_amd import _lib
@@ -21,6 +22,18 @@ def test_names_and_refusals():
                          torch.ones(()), torch.ones(()))
     with pytest.raises(ValueError, match="gfx950"):
         ex.linear(torch.zeros((2, 64), dtype=torch.bfloat16), weight)
+    assert ex.calls == 0
+
+
+def test_forward_mode_is_refused():
+    weight = NVFP4Weight(torch.zeros((128, 32), dtype=torch.uint8), torch.zeros((128, 4), dtype=torch.uint8),
+                         torch.ones(()), torch.ones(()))
+    x, b = torch.zeros((2, 64), dtype=torch.bfloat16), torch.zeros(128, dtype=torch.bfloat16)
+    ex = NVFP4Execution("unquantized")
+    with torch.no_grad(), fw.dual_level():
+        for args in ((fw.make_dual(x, torch.ones_like(x)), weight, b), (x, weight, fw.make_dual(b, torch.ones_like(b)))):
+            with pytest.raises(ValueError, match="inference-only"):
+                ex.linear(*args)
     assert ex.calls == 0
 
 

@@ -60,7 +60,7 @@ def packed_attention(q, k, v, q_offsets, k_offsets, *, k_lengths=None, causal=Fa
         raise ValueError("query heads must be a multiple of the key heads")
     if dim % 8 or not 8 <= dim <= 128:
         raise ValueError("the head dimension must be a multiple of 8 from 8 to 128")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors) or kernels.has_tangent(*tensors):
         raise ValueError("packed attention is inference-only")
     batch = q_offsets.numel() - 1
     ends = batch if k_lengths is not None else batch + 1

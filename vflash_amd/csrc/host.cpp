@@ -157,7 +157,10 @@ PyObject* w8a8_linear_lora(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
-bool records(const at::Tensor& t) { return t.requires_grad() && c10::GradMode::is_enabled(); }
+// A gradient or a forward-mode tangent to carry: the wrappers refuse both.
+bool records(const at::Tensor& t) {
+  return (t.requires_grad() && c10::GradMode::is_enabled()) || t._fw_grad(0).defined();
+}
 
 bool aligned16(const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
 
@@ -167,7 +170,8 @@ PyObject* nvfp4_w16_linear(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   if (nargs != 5) Py_RETURN_NONE;
   const at::Tensor *x = plain(a[0]), *w = plain(a[1]), *ws = plain(a[2]), *alpha = plain(a[3]);
   const at::Tensor* b = a[4] == Py_None ? nullptr : plain(a[4]);
-  if (!x || !w || !ws || !alpha || (a[4] != Py_None && !b) || records(*x)) Py_RETURN_NONE;
+  if (!x || !w || !ws || !alpha || (a[4] != Py_None && !b)) Py_RETURN_NONE;
+  if (records(*x) || (b && b->_fw_grad(0).defined())) Py_RETURN_NONE;
   const bool f16 = x->scalar_type() == at::kHalf;
   if ((!f16 && x->scalar_type() != at::kBFloat16) || w->scalar_type() != at::kByte || ws->scalar_type() != at::kByte ||
       alpha->scalar_type() != at::kFloat || alpha->numel() != 1)

@@ -690,6 +690,11 @@ def nvfp4_w16_gemm(matrix, packed, block_scales, alpha, bias=None):
     return out
 
 
+def has_tangent(*tensors) -> bool:
+    """Whether a tensor carries a forward-mode tangent, which the kernels would drop."""
+    return any(t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def _attention_rows(t):
     """``t`` [rows, heads, dim] as the attention kernels read it: unit stride in d, other
     strides multiples of 8, 16-byte aligned; copied where it is not."""

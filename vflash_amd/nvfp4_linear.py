@@ -119,7 +119,9 @@ class NVFP4Execution:
             or values.device != weight.packed.device
         ):
             raise ValueError("NVFP4 input differs from its frozen matrix")
-        if torch.is_grad_enabled() and values.requires_grad:
+        if torch.is_grad_enabled() and values.requires_grad or (
+            self.activations == "unquantized" and kernels.has_tangent(values, bias)
+        ):
             raise ValueError("NVFP4 execution is inference-only")
         _require_device(values.device)
         if bias is not None and (
