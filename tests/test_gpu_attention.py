@@ -304,6 +304,16 @@ def test_native_host_path(dev):
         assert host.packed_attention(*args) is None
 
 
+def test_pending_signs(dev):
+    # torch._neg_view and the imaginary part of a conjugate: the memory holds the opposite sign.
+    q, k, v = make(dev, [1, 60], [90, 60], 8, 2, 64, BF16)
+    qo, ko = offsets([1, 60], dev), offsets([90, 60], dev)
+    for i in range(3):
+        a, b = [q, k, v], [q, k, v]
+        a[i], b[i] = torch._neg_view(a[i]), -a[i]
+        assert torch.equal(packed_attention(*a, qo, ko, causal=True), packed_attention(*b, qo, ko, causal=True))
+
+
 def test_forward_mode_is_refused(dev):
     q, k, v = make(dev, [4], [9], 4, 2, 64, BF16)
     qo, ko = offsets([4], dev), offsets([9], dev)

@@ -175,3 +175,13 @@ def test_forward_mode_is_refused(dev):
             with pytest.raises(ValueError, match="inference-only"):
                 ex.linear(values, weight, bias)
     assert ex.calls == 0
+
+
+@pytest.mark.parametrize("m", [1, 20, 300])
+def test_pending_signs(dev, m):
+    x, weight, b = make(dev, m, 256, 192, BF16)
+    ex = NVFP4Execution("unquantized")
+    assert torch.equal(ex.linear(torch._neg_view(x), weight, b), ex.linear(-x, weight, b))
+    assert torch.equal(ex.linear(x, weight, torch._neg_view(b)), ex.linear(x, weight, -b))
+    twice = NVFP4Weight(weight.packed, weight.scales, torch._neg_view(-weight.alpha), weight.input_scale)
+    assert torch.equal(ex.linear(x, twice, b), ex.linear(x, weight, b))

@@ -31,7 +31,8 @@ namespace {
 const at::Tensor* plain(PyObject* o) {
   if (!THPVariable_CheckExact(o)) return nullptr;
   const at::Tensor& t = THPVariable_Unpack(o);
-  return t.is_cuda() && t.layout() == at::kStrided ? &t : nullptr;
+  // A tensor with a pending sign (torch._neg_view) is not what its memory holds.
+  return t.is_cuda() && t.layout() == at::kStrided && !t.is_neg() ? &t : nullptr;
 }
 
 bool gfx950(c10::DeviceIndex index) {

@@ -677,6 +677,8 @@ def nvfp4_w16_gemm(matrix, packed, block_scales, alpha, bias=None):
     if bias is not None and (bias.dtype != torch.bfloat16 or bias.shape != (n,)):
         raise ValueError("NVFP4 bias must be a BF16 vector of the output width")
     device = require_device(matrix, packed, block_scales, alpha, bias)
+    matrix, alpha = matrix.resolve_neg(), alpha.resolve_neg()  # a pending sign is not in the memory
+    bias = None if bias is None else bias.resolve_neg()
     # The kernels read 16-byte vectors.
     if matrix.stride(0) % 8 or matrix.data_ptr() % 16:
         matrix = matrix.clone(memory_format=torch.contiguous_format)
@@ -697,7 +699,8 @@ def has_tangent(*tensors) -> bool:
 
 def _attention_rows(t):
     """``t`` [rows, heads, dim] as the attention kernels read it: unit stride in d, other
-    strides multiples of 8, 16-byte aligned; copied where it is not."""
+    strides multiples of 8, 16-byte aligned, no pending sign; copied where it is not."""
+    t = t.resolve_neg()
     if (t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16
             or t.stride(0) >= 1 << 23):
         return t.clone(memory_format=torch.contiguous_format)
