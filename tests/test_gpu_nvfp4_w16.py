@@ -185,3 +185,20 @@ def test_pending_signs(dev, m):
     assert torch.equal(ex.linear(x, weight, torch._neg_view(b)), ex.linear(x, weight, -b))
     twice = NVFP4Weight(weight.packed, weight.scales, torch._neg_view(-weight.alpha), weight.input_scale)
     assert torch.equal(ex.linear(x, twice, b), ex.linear(x, weight, b))
+
+
+@pytest.mark.parametrize("m", [2, 9, 20, 50, 300])
+def test_broadcast_overlapping_and_distant_rows(dev, m):
+    x, weight, b = make(dev, m, 256, 192, BF16)
+    ex = NVFP4Execution("unquantized")
+    flat = torch.randn(16 * m + 192, device=dev).to(BF16)
+    distant = torch.zeros(((m - 1) * (1 << 22) + 192,) if m < 20 else (1,), device=dev, dtype=BF16)
+    views = [x[:1].expand(m, 192), x[:1].half().expand(m, 192), x[:1].float().expand(m, 192), flat.as_strided((m, 192), (16, 1)),
+             x.as_strided((m, 192), (8, 1))]
+    if m < 20:
+        views.append(distant.as_strided((m, 192), (1 << 22, 1)))
+        views[-1].copy_(x)
+    for view in views:
+        assert torch.equal(ex.linear(view, weight, b), ex.linear(view.contiguous(), weight, b))
+    batched = x[:1].expand(m, 192).unflatten(0, (1, m))
+    assert torch.equal(ex.linear(batched, weight, b)[0], ex.linear(x[:1].repeat(m, 1), weight, b))

@@ -679,8 +679,8 @@ def nvfp4_w16_gemm(matrix, packed, block_scales, alpha, bias=None):
     device = require_device(matrix, packed, block_scales, alpha, bias)
     matrix, alpha = matrix.resolve_neg(), alpha.resolve_neg()  # a pending sign is not in the memory
     bias = None if bias is None else bias.resolve_neg()
-    # The kernels read 16-byte vectors.
-    if matrix.stride(0) % 8 or matrix.data_ptr() % 16:
+    # The kernels read 16-byte vectors of rows that lie apart, by less than 2^22 values.
+    if matrix.stride(0) % 8 or matrix.data_ptr() % 16 or not k <= matrix.stride(0) < 1 << 22:
         matrix = matrix.clone(memory_format=torch.contiguous_format)
     packed, block_scales = (t.clone() if t.data_ptr() % 16 else t for t in (packed, block_scales))
     if bias is not None and (bias.data_ptr() % 16 or not bias.is_contiguous()):
