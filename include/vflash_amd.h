@@ -468,7 +468,7 @@ int vflash_nvfp4_w16_linear(const void* x, int x_is_f16, int64_t ldx, const void
  *   workspace  vflash_packed_attention_workspace(...) bytes (0: may be NULL), 16-byte aligned,
  *              without contents to keep; one call at a time
  *   Requires dim % 8 == 0, 8 <= dim <= 128, every stride a multiple of 8 and the pointers 16-byte
- *   aligned, k_ts and v_ts < 2^23, tokens and keys < 2^30, scale positive and finite.
+ *   aligned, k_ts and v_ts < 2^23, tokens and keys < 2^30, scale and log2(e) scale positive and finite.
  */
 int64_t vflash_packed_attention_workspace(int64_t tokens, int64_t keys, int64_t batch, int64_t heads,
                                           int64_t key_heads, int64_t dim);

@@ -47,6 +47,16 @@ def test_refusals():
     refused("inference-only", [a[0].requires_grad_(), *a[1:]])
 
 
+def test_scales_past_binary32():
+    # What the kernels multiply by is log2(e) times the scale in binary32: neither infinite nor zero.
+    for scale in (2.4e38, 3.39e38, 1e-46):
+        assert entry(scale=scale) == _lib.VFLASH_EINVAL
+        with pytest.raises(ValueError, match="scale"):
+            packed_attention(*operands(), scale=scale)
+    with pytest.raises(ValueError, match="gfx950"):
+        packed_attention(*operands(), scale=2.35e38)
+
+
 def test_forward_mode_is_refused():
     # A tangent that the kernel would drop, on each operand, gradients recorded or not.
     for recorded in (True, False):

@@ -11,6 +11,7 @@ synchronizes and a captured call replays with other lengths of the same total.
 
 from __future__ import annotations
 
+import ctypes
 import math
 
 import torch
@@ -72,6 +73,7 @@ def packed_attention(q, k, v, q_offsets, k_offsets, *, k_lengths=None, causal=Fa
             raise ValueError(f"{name} must be a contiguous int64 vector of the sequences")
     if scale is None:
         scale = 1.0 / math.sqrt(dim)
-    elif not (0.0 < scale < 3.4e38):
-        raise ValueError("the scale must be positive and finite")
+    elif not (ctypes.c_float(scale).value > 0.0 and scale <= 2.358e38):
+        # times log2(e), in binary32
+        raise ValueError("the scale must be positive and finite, and so must log2(e) times it")
     return kernels.packed_attention(q, k, v, q_offsets, k_offsets, k_lengths, bool(causal), scale)

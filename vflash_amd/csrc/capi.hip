@@ -533,7 +533,8 @@ int vflash_packed_attention(const void* q, int64_t q_ts, int64_t q_hs, const voi
   if (k_ts >= (int64_t(1) << 23) || v_ts >= (int64_t(1) << 23)) return VFLASH_EINVAL;
   if (!(o_hs >= dim && o_ts >= (heads - 1) * o_hs + dim) && !(o_ts >= dim && o_hs >= (tokens - 1) * o_ts + dim))
     return VFLASH_EINVAL;
-  if (!(scale > 0.0f) || scale > 3.4e38f) return VFLASH_EINVAL;  // rejects NaN and infinity
+  p.c = scale * 1.4426950408889634f;
+  if (!(p.c > 0.0f) || p.c > 3.4028234663852886e38f) return VFLASH_EINVAL;  // rejects NaN and infinity too
   const int64_t need = vfa::attention_workspace(p);
   if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16))) return VFLASH_EINVAL;
   p.q = static_cast<const uint16_t*>(q);
@@ -552,7 +553,6 @@ int vflash_packed_attention(const void* q, int64_t q_ts, int64_t q_hs, const voi
   p.k_offsets = k_offsets;
   p.k_lengths = k_lengths;
   p.causal = causal != 0;
-  p.c = scale * 1.4426950408889634f;
   return status(vfa::launch_attention(p, f16 != 0, workspace, static_cast<hipStream_t>(stream)));
 }
 
