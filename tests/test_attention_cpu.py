@@ -57,6 +57,19 @@ def test_scales_past_binary32():
         packed_attention(*operands(), scale=2.35e38)
 
 
+@pytest.mark.parametrize("tokens,heads,key_heads,taken", [
+    (1 << 29, 9, 9, False), (477 * 10**6, 9, 9, False), (475 * 10**6, 9, 9, True), (1 << 29, 64, 64, False),
+    (1 << 29, 56, 56, True), (1 << 29, 7, 1, True), (1 << 29, 32 * 32, 32, False),
+])
+def test_single_tokens_are_counted_in_32_bits(tokens, heads, key_heads, taken):
+    # A tile per token and key head (per 16 heads of one), on one line or, for multiples of 8, on eight.
+    need = _lib.library().vflash_packed_attention_workspace(tokens, 6, tokens, heads, key_heads, 8)
+    assert need == (0 if taken else _lib.VFLASH_EINVAL)
+    if not taken:
+        change = dict(tokens=tokens, batch=tokens, heads=heads, key_heads=key_heads, dim=8, o_ts=heads * 64)
+        assert entry(**change) == _lib.VFLASH_EINVAL
+
+
 def test_forward_mode_is_refused():
     # A tangent that the kernel would drop, on each operand, gradients recorded or not.
     for recorded in (True, False):

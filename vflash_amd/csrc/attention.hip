@@ -252,6 +252,7 @@ struct AttentionPlan {
   bool step;
   int rows;            // of a tile
   int64_t grid, join;  // workgroups; 0: no split
+  int64_t line;        // step: units that a line may hold, counted in 32 bits
 };
 
 // The launch of a call, from its sizes alone: the lengths are on the device.  Measured as one side
@@ -297,6 +298,7 @@ AttentionPlan attention_plan(AttentionParams& p) {
     auto bound = [&] { return tiles * p.head_blocks * (((int64_t)p.keys >> p.unit_shift) + 1); };
     while (bound() >= int64_t(1) << 30 && p.unit_shift < 31) ++p.unit_shift;  // the kernel counts in 32 bits
     const int64_t units = bound();
+    plan.line = p.head_blocks % 8 ? units : units / 8;
     plan.grid = (cus + 7) / 8 * 8 * (p.dim <= 64 ? 2 : 1);
     if (units < plan.grid) plan.grid = (units + 7) / 8 * 8;
     plan.join = split;
@@ -334,11 +336,13 @@ int64_t attention_workspace(const AttentionParams& params) {
   return p.slots * plan.rows * (p.dim + 2) * 4;
 }
 
-// false: the grid would pass HIP's limit.
+// false: the grid would pass HIP's limit, or a line of attention_step 2^32 units (its workgroups'
+// parts end at most a grid past the line).
 bool attention_fits(const AttentionParams& params) {
   AttentionParams p = params;
   const AttentionPlan plan = attention_plan(p);
-  return plan.grid < (int64_t(1) << 24) && plan.join < (int64_t(1) << 24);
+  return plan.grid < (int64_t(1) << 24) && plan.join < (int64_t(1) << 24) &&
+         plan.line < (int64_t(1) << 32) - (int64_t(1) << 24);
 }
 
 hipError_t launch_attention(const AttentionParams& params, bool f16, void* workspace, hipStream_t s) {
