@@ -1,6 +1,7 @@
 """Packed attention on the GPU against its definition in 64 bits."""
 
 import math
+import random
 
 import pytest
 import torch
@@ -109,6 +110,54 @@ def test_bad_offsets_stay_inside(dev, qo, ko, kl):
     got = packed_attention(q, k, v, t(qo), t(ko), k_lengths=t(kl), causal=True)
     torch.cuda.synchronize()
     assert got.shape == q.shape
+
+
+@pytest.mark.parametrize("tokens,keys,batch,heads,kv", [
+    (90, 300, 80, 4, 2), (40, 5000, 5, 8, 4), (150, 100000, 200, 6, 3),  # tiles of 16 rows: whole, split
+    (900, 900, 2, 7, 1), (300, 4000, 3, 4, 2), (4000, 5000, 150, 4, 2),  # tiles of 128: whole, split, many sequences
+])
+def test_bad_offsets_write_every_row_and_no_other(dev, tokens, keys, batch, heads, kv):
+    # What lies around the operands is NaN, and must neither show in a row nor change.  The schedule is
+    # run on the CPU under the same kinds of offsets (test_attention_schedule_cpu.py).
+    dim, room = 64, 64
+    g = torch.Generator(device=dev).manual_seed(5)
+
+    def inside(rows, width):
+        buffer = torch.full((rows + 2 * room, width, dim), torch.nan, device=dev, dtype=BF16)
+        buffer[room:room + rows] = torch.randn((rows, width, dim), generator=g, device=dev).to(BF16)
+        return buffer, buffer[room:room + rows]
+
+    (_, q), (_, k), (_, v) = inside(tokens, heads), inside(keys, kv), inside(keys, kv)
+    size = _lib.library().vflash_packed_attention_workspace(tokens, keys, batch, heads, kv, dim)
+    workspace = torch.full((size // 4 + 256,), torch.nan, device=dev)
+    rng = random.Random(tokens)
+    for i in range(8):
+        def bad(n, hi):
+            good = sorted(rng.randint(0, hi) for _ in range(n))
+            if i % 4 == 0:
+                values = [rng.choice((-(1 << 63), -1, 0, hi, hi + 1, 1 << 32, (1 << 63) - 1, rng.randint(-hi, 2 * hi)))
+                          for _ in range(n)]
+            elif i % 4 == 1:
+                values = good[::-1]
+            elif i % 4 == 2:  # falls back once, past the first 64 where there are that many
+                values = good[:70] + [x // 2 for x in good[70:]] if n > 70 else good[:1] + [x // 2 for x in good[1:]]
+            else:
+                values = [x if rng.random() < 0.8 else rng.choice((-5, 3 * hi, rng.randint(0, hi))) for x in good]
+            return torch.tensor(values, dtype=torch.int64, device=dev)
+
+        qo, ko = bad(batch + 1, tokens), bad(batch + (i < 4), keys)
+        kl = None if i < 4 else bad(batch, keys)
+        around, out = inside(tokens, heads)
+        out.fill_(torch.nan)
+        workspace.fill_(torch.nan)
+        _lib.call("vflash_packed_attention", q.data_ptr(), heads * dim, dim, k.data_ptr(), kv * dim, dim, v.data_ptr(),
+                  kv * dim, dim, 0, tokens, keys, heads, kv, dim, qo.data_ptr(), ko.data_ptr(),
+                  None if kl is None else kl.data_ptr(), batch, i % 2, 0.125, out.data_ptr(), heads * dim, dim,
+                  workspace.data_ptr() if size else None, size, _lib.stream_of(dev))
+        torch.cuda.synchronize()
+        assert bool(torch.isfinite(out).all()), i
+        assert bool(around[:room].isnan().all()) and bool(around[room + tokens:].isnan().all()), i
+        assert bool(workspace[size // 4:].isnan().all()), i
 
 
 @pytest.mark.parametrize("layout", ["merged", "heads first", "expanded", "odd strides", "offset"])
