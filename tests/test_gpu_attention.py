@@ -272,6 +272,29 @@ def test_weights_are_normalised_as_rounded(dev, nq, n, dtype):
     assert torch.equal(got, torch.ones_like(got))
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("nq,n", [(1, 33), (1, 640), (1, 5000), (3, 16000), (1, 16383), (40, 5000), (130, 1100), (300, 4000)])
+def test_every_key_counts_once(dev, nq, n, dtype):
+    # Queries of zeros weigh all keys alike, and v marks key j by d = j % 128, a quarter of the keys for each
+    # key head: an output is a count over n, of at most 32 keys, so that one key more or less is 1 / 32 of
+    # it.  Off by its one rounding (half a step) and the sums' binary32.
+    heads, dim = 4, 128
+    q = torch.zeros((nq, heads, dim), device=dev, dtype=dtype)
+    k = torch.randn((n, heads, dim), device=dev).to(dtype)
+    j = torch.arange(n, device=dev)
+    v = torch.zeros((n, heads, dim), device=dev, dtype=dtype)
+    v[j, j * heads // n, j % dim] = 1.0
+    got = packed_attention(q, k, v, offsets([nq], dev), offsets([n], dev)).double()
+    want = (v.double().sum(0) / n).expand(nq, heads, dim)
+    half = torch.finfo(dtype).eps / 2
+    assert bool(((got - want).abs() <= (half + 2.0**-23 * 40) * want + torch.finfo(dtype).smallest_normal * half * 2).all())
+    # Causal: query i of nq sees n - nq + i + 1 keys.
+    got = packed_attention(q, k, v, offsets([nq], dev), offsets([n], dev), causal=True).double()
+    seen = torch.cumsum(v.double(), 0)[n - nq:]
+    want = seen / torch.arange(n - nq + 1, n + 1, device=dev)[:, None, None]
+    assert bool(((got - want).abs() <= (half + 2.0**-23 * 40) * want + torch.finfo(dtype).smallest_normal * half * 2).all())
+
+
 def test_many_sequences(dev):
     # More sequences than a wave has lanes, long ones among short.
     g = torch.Generator().manual_seed(3)
