@@ -342,7 +342,7 @@ __device__ __forceinline__ int attention_limit(const AttentionParams& p, const A
 // The schedule of attention_step.  Every tile is a number of units (2^p.unit_shift keys each, one at
 // least), the units of all tiles of a head block form a line, the head blocks' lines one after
 // another a longer one, and each workgroup takes the next p.grid-th part of that: equal work whatever
-// the lengths.  A workgroup whose part ends inside a tile leaves a partial sum, of which it has at
+// the lengths, where the plan splits keys (else a unit is a whole sequence).  A workgroup whose part ends inside a tile leaves a partial sum, of which it has at
 // most two: one of a tile begun by an earlier workgroup (slot 2 b), one of a tile that a later one ends
 // (slot 2 b + 1).  On one XCD's workgroups lie whole head blocks where these divide among the XCDs.
 struct AttentionLine {

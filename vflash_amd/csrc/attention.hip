@@ -8,14 +8,16 @@
 // V^T is read from the row-major tile by transposing LDS reads, four keys at a time.
 //
 // A workgroup's waves, 32 rows each, share tiles of 64 keys in LDS, which DMA fills one tile
-// ahead.  Weights are rounded to the operands' type (half a step, 2^-9 or 2^-12 of each), as the
-// matrix instruction takes them, and so does the binary32 sum that normalises them.
+// ahead.  Weights are rounded to the operands' type, as the matrix instruction takes them (by half a
+// step at most, 2^-8 of the value in bf16 and 2^-11 in f16), and the binary32 sum that normalises them
+// is that of the rounded ones: errors against 64 bits are 1.1 to 1.4 times those of weights in 32 bits.
 //
 // Bound by the softmax beside the MFMAs, and over milliseconds by the board's power: 32760 tokens
-// of 40 heads of 128, unmasked, 19.4 ms (1.13 PFLOP/s, MFMAs busy 0.60 of the cycles at 1.6 GHz); 8191
-// causal tokens of 16 heads of 64 0.163 ms (0.84 PFLOP/s, its VALU full); 24 causal prompts of up to
-// 1023 tokens, 28 heads over 4, 0.129 ms.  Blocks of 32 keys above dimension 64 let three workgroups
-// share a CU, 64 below four.
+// of 40 heads of 128, unmasked, 19.8 ms (1.11 PFLOP/s, MFMAs busy 0.60 of the cycles at 1.65 GHz, VALU
+// 0.50); 8191 causal tokens of 16 heads of 64 0.165 ms (0.83 PFLOP/s; VALU 0.54, MFMAs 0.38: a wave's
+// products and softmax follow each other, and the others' fill its gaps in part); 24 causal prompts of
+// up to 1023 tokens, 28 heads over 4, 0.126 ms (VALU 0.43, MFMAs 0.30).  Boxes differ by 5 %.  Blocks of
+// 32 keys above dimension 64 let three workgroups share a CU, 64 below four.
 #include "attention.h"
 #include "attention_plan.h"
 

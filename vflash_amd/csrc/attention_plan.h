@@ -28,6 +28,12 @@ struct AttentionPlan {
 //   for tiles of 128 where these number less than three quarters of the CUs (509 tokens after 2000
 //   over 8 heads: 28 split, 57 whole; 2000 tokens over 16 heads, 240 tiles: 56, 49), in chunks of at
 //   least 512 keys (400 tokens over 8 heads in chunks of 256: 18, whole 14).
+// They see rows and sequences, not lengths, and cost most where these differ most: one sequence of 60000
+// keys among 127 of one key, too few rows for a split, 664 (with 20000 rows of room, split, 126); 64
+// sequences that share 32768 rows, not split, 541; 77 keys 7.8 in a room of 768 rows and 10.4, split, in
+// one of 8192.  One kernel serves the whole call: 200 single tokens over 500 keys 108 and a prompt of
+// 500 17, in one call 153, in tiles of 16; 100 over 1000 keys 93 and a prompt of 2000 56, in one call
+// 137, in tiles of 128.
 inline AttentionPlan attention_plan(AttentionParams& p) {
   const int64_t cus = compute_units();
   AttentionPlan plan{};

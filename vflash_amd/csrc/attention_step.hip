@@ -8,7 +8,8 @@
 // Each wave takes every fourth block of 32 keys of the item and keeps a ring of two in LDS, which
 // its own DMA fills: 128 KB a CU in flight or in use, no barrier before the end, where the four
 // waves' sums are added up.  131071 keys of 8 heads of 128: 107 us, 5.0 TB/s, what a copy of 1 GiB
-// reaches; 16 sequences of up to 8191: 64 us, 4.3 TB/s; 77 keys: 7.4 us a call, latency alone.
+// reaches; 16 sequences of up to 8191: 65 us, 4.2 TB/s; 77 keys: 7.5 us a call, a chain of loads, search
+// and sums in one wave after another.
 #include "attention.h"
 
 namespace vfa {

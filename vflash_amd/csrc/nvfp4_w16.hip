@@ -353,7 +353,8 @@ void launch_tile(const GemmParams& p, hipStream_t s) {
 
 // Tiles of 64 x 64 (the few-row kernel) or 128 x 256, by the time of the busiest CU: 19 us a round of
 // the first at K = 5120 (128 x 5120 x 5120, 160 workgroups 20.9; 300 rows, 400 workgroups 38.8) and 64
-// of the second (300 rows, 60 tiles 65; 1021 x 5120 x 13824, 432 tiles 130), in proportion to K.
+// of the second (300 rows, 60 tiles 65; 1021 x 5120 x 13824, 432 tiles 126), in proportion to K.  A
+// round takes as long where it fills part of the CUs: 64 x 5120 x 5120, 80 workgroups, 19.6.
 bool many_rows(int64_t m, int64_t n, int64_t cus) {
   const int64_t few = (m + 63) / 64 * (n / 64), many = (m + 127) / 128 * ((n + 255) / 256);
   return 64 * ((many + cus - 1) / cus) < 19 * ((few + cus - 1) / cus);
@@ -363,8 +364,8 @@ template <bool F16>
 void launch_w16(const GemmParams& p, hipStream_t s) {
   const int64_t cus = compute_units();
   // Up to 16 rows a workgroup takes 64 weight rows where these fill the GPU and 32 where not:
-  // 1 x 5120 x 5120 7.7 us with 80 workgroups of twice the waves, 10.5 with 64 rows each, and
-  // 1 x 5376 x 28672 17.9 us.  x in stages of four rows where it has no more: a quarter of its LDS.
+  // 1 x 5120 x 5120 7.7 us with 160 workgroups of 32 rows and twice the waves, 10.5 with 80 of 64 rows,
+  // and 1 x 5376 x 28672 17.9 us.  x in stages of four rows where it has no more: a quarter of its LDS.
   if (p.m <= 4) {
     if (p.n / 64 >= cus) launch_few<F16, 4, 1, 4, 128, 4, 2>(p, s);
     else launch_few<F16, 2, 1, 4, 128, 8, 4>(p, s);

@@ -22,7 +22,7 @@ accurate arithmetic, not the reference's.
 ``NVFP4Execution(activations="unquantized")`` is the weight-only form: BF16 or
 F16 activations enter the GEMM as they are (FP32 ones as BF16), the weight's
 E2M1 values and block scales multiply exactly, and ``alpha * sum + bias`` is
-rounded to bf16 once.  It reads a weight's half byte per value whatever the
+rounded to bf16 once, for F16 activations too.  It reads a weight's half byte per value whatever the
 rows, so single tokens and small batches run at the weight's bytes;
 ``input_scale`` is not used.
 """
