@@ -461,6 +461,7 @@ int vflash_nvfp4_w16_linear(const void* x, int x_is_f16, int64_t ldx, const void
  *        rows outside every sequence, are zeros.  Scores, softmax and sums are binary32;
  *        probabilities are rounded to the operands' type for their product with v.  Every finite v
  *        has its place in the sums; bf16 values below 2^-118 times `keys` may lose bits.
+ *        Scores times log2(e) scale have to stay inside binary32.
  * Offsets and lengths are read on the device and clamped to the operands: values that decrease or
  * overlap give unspecified results, but nothing outside the operands is read or written, and every
  * row of out is.  A masked key has no effect through k; its v may enter with weight 0 if it lies in
