@@ -16,7 +16,7 @@
 // of 40 heads of 128, unmasked, 19.8 ms (1.11 PFLOP/s, MFMAs busy 0.60 of the cycles at 1.65 GHz, VALU
 // 0.50); 8191 causal tokens of 16 heads of 64 0.165 ms (0.83 PFLOP/s; VALU 0.54, MFMAs 0.38: a wave's
 // products and softmax follow each other, and the others' fill its gaps in part); 24 causal prompts of
-// up to 1023 tokens, 28 heads over 4, 0.126 ms (VALU 0.43, MFMAs 0.30).  Boxes differ by 5 %.  Blocks of
+// up to 1023 tokens, 28 heads over 4, 0.126 ms (VALU 0.43, MFMAs 0.30).  Cards differ by 5 %.  Blocks of
 // 32 keys above dimension 64 let three workgroups share a CU, 64 below four.
 #include "attention.h"
 #include "attention_plan.h"
