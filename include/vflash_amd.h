@@ -480,6 +480,95 @@ int vflash_packed_attention(const void* q, int64_t q_ts, int64_t q_hs, const voi
                             float scale, void* out, int64_t o_ts, int64_t o_hs, void* workspace,
                             int64_t workspace_bytes, void* stream);
 
+/*
+ * Rotary positions.  No reference counterpart in this form: the reference rotates split halves by a table of
+ * cosines (src/vflash/native/h3_fused_ops.py:428-507).
+ *   q      bf16 (f16 when f16) [tokens, heads, dim], element (t, h, d) at t * q_ts + h * q_hs + d
+ *   k      the same with key_heads, or NULL (then k_out is not used)
+ *   phases uint64 [pairs]: pair i turns by phases[i] 2^-64 of a turn a position (modulo one turn)
+ *   axis   int64 [pairs]: which of the token's positions pair i follows, or NULL (the first); outside [0, axes): none
+ *   positions int64 [tokens, axes], any value
+ *   pair i is the elements 2 i and 2 i + 1 (interleaved) or i and i + pairs; elements past 2 pairs are copied
+ *   (a, b) -> magnitude (a cos - b sin, a sin + b cos), in binary32 with one rounding
+ *   q_out, k_out  contiguous, apart from the inputs
+ *   Requires dim % 8 == 0, 8 <= dim <= 256, 2 pairs <= dim, axes <= 64, heads and key_heads <= 65536, tokens < 2^30, a
+ *   finite magnitude, strides multiples of 8 and not negative, 16-byte aligned pointers.
+ */
+int vflash_rotate(const void* q, int64_t q_ts, int64_t q_hs, const void* k, int64_t k_ts, int64_t k_hs, int f16,
+                  int64_t tokens, int64_t heads, int64_t key_heads, int64_t dim, const uint64_t* phases,
+                  const int64_t* axis, int64_t pairs, int interleaved, float magnitude, const int64_t* positions,
+                  int64_t axes, void* q_out, void* k_out, void* stream);
+
+/*
+ * The keys and values of new tokens into a paged cache, and the rotary positions of q and k on the way.  No
+ * reference counterpart.
+ *   q, k, v   bf16 (f16 when f16) [tokens, heads | key_heads | key_heads, dim] as vflash_rotate takes them; q: or NULL
+ *   q_offsets int64 [batch + 1]: sequence b's new tokens, or NULL: one a sequence (tokens == batch)
+ *   lengths   int64 [batch]: the sequence's tokens, the new ones among them: token i of nq is its
+ *             token lengths[b] - nq + i, whose place is slot i % page of page table[b * width + i / page]
+ *   values    [pages, 2, key_heads, page, dim]: keys, then values, in q's type; with scales fp32 [pages, 2, key_heads,
+ *             page] E4M3 codes: scale = amax > 0 ? max(amax / 448, FLT_MIN) : 1 over the dim values of a row, from the
+ *             unrounded rotated ones, and code = e4m3_rne(clamp(x / scale, -448, 448))
+ *   phases    as vflash_rotate, or NULL: no rotation (then q is NULL); positions NULL: the tokens' own in their sequences
+ *   q_out     [tokens, heads, dim] contiguous: q rotated
+ * A token without a place (outside the offsets, before its sequence's start, past the table, or on a page outside
+ * [0, pages)) is not stored, and its rows of q_out are zeros.  Slots that no token has are left as they are.  Two
+ * tokens with one place leave either.
+ *   Requires page a power of two from 16 to 4096, dim % 8 == 0 (16 with scales), 8 <= dim <= 128, key_heads <= 4096,
+ *   width * page, pages, tokens and batch < 2^30, and what vflash_rotate does.
+ */
+int vflash_paged_append(const void* q, int64_t q_ts, int64_t q_hs, const void* k, int64_t k_ts, int64_t k_hs,
+                        const void* v, int64_t v_ts, int64_t v_hs, int f16, int64_t tokens, int64_t heads,
+                        int64_t key_heads, int64_t dim, const int64_t* q_offsets, const uint64_t* phases,
+                        const int64_t* axis, int64_t pairs, int interleaved, float magnitude, const int64_t* positions,
+                        int64_t axes, void* values, float* scales, int64_t pages, int64_t page, const int64_t* table,
+                        int64_t width, const int64_t* lengths, int64_t batch, void* q_out, void* stream);
+
+/*
+ * Attention of new tokens, one or a few a sequence, over a paged cache that holds them already: vflash_packed_attention,
+ * causal, with the keys and values of vflash_paged_append.  No reference counterpart.
+ *   q_offsets, values, scales, table, lengths, batch as there; out as vflash_packed_attention
+ *   With scales, a key's factor multiplies its score and a value's its weight before that is rounded to bf16.
+ * Lengths are clamped to the table.  Keys on a page outside [0, pages) count as keys and values of zeros.  Nothing
+ * else outside a sequence's pages is read.  Masked keys, rows that see none, and scores as vflash_packed_attention.
+ *   workspace  vflash_paged_attention_workspace(...) bytes (0: may be NULL), 16-byte aligned, without contents to
+ *              keep; one call at a time
+ *   Requires what vflash_paged_append does, and heads % key_heads == 0.
+ */
+int64_t vflash_paged_attention_workspace(int64_t tokens, int64_t batch, int64_t heads, int64_t key_heads, int64_t dim,
+                                         int64_t page, int64_t width);
+int vflash_paged_attention(const void* q, int64_t q_ts, int64_t q_hs, int f16, int64_t tokens, int64_t heads,
+                           int64_t key_heads, int64_t dim, const int64_t* q_offsets, const void* values,
+                           const float* scales, int64_t pages, int64_t page, const int64_t* table, int64_t width,
+                           const int64_t* lengths, int64_t batch, float scale, void* out, int64_t o_ts, int64_t o_hs,
+                           void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * The low-rank adapters of many requests beside a shared projection.  No reference counterpart (its hook,
+ * src/vflash/adapters/h3_reference_lora.py:75-92, serves one adapter at a time).
+ *   base, out bf16 (f16 when f16) [rows, n], row strides ldb, ldo; out may be base
+ *   x         the same type, [rows, k], row stride ldx
+ *   widths    branches (1..3) column counts on the host, n their sum: the projections that are merged
+ *   down      [adapters, branches * width, k], up [adapters, n, width], contiguous; ranks at and past an adapter's own
+ *             are zeros in both
+ *   scaling   fp32 [adapters, branches];  ranks int32 [adapters]
+ *   index     int64 [rows]: the row's adapter; outside [0, adapters): none
+ *   out[m, n] = base[m, n] + scaling[i, b] sum_r (sum_k x[m, k] down[i, b * width + r, k]) up[i, n, r], i = index[m],
+ *   b the branch of column n.  Sums are binary32; t = scaling (x down^T) enters the second product as two 16-bit parts,
+ *   and the result is rounded once.  Rows without an adapter are copied.
+ *   workspace vflash_request_adapters_workspace(...) bytes, 16-byte aligned, without contents to keep; one call at a
+ *             time
+ *   Requires width % 16 == 0, 16 <= width <= 128, adapters < 8192, k % 8 == 0, every widths[b] % 8 == 0 and < 2^21, rows <
+ *   2^24, row strides multiples of 8 (equal where out is base), 16-byte aligned matrices.
+ */
+int64_t vflash_request_adapters_workspace(int64_t rows, int64_t k, const int64_t* widths, int64_t branches,
+                                          int64_t adapters, int64_t width);
+int vflash_request_adapters(const void* base, int64_t ldb, const void* x, int64_t ldx, int f16, int64_t rows, int64_t k,
+                            const int64_t* widths, int64_t branches, const void* down, const void* up,
+                            const float* scaling, const int32_t* ranks, int64_t adapters, int64_t width,
+                            const int64_t* index, void* out, int64_t ldo, void* workspace, int64_t workspace_bytes,
+                            void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -109,6 +109,27 @@ SIGNATURES: dict[str, tuple[list, object]] = {
          _I64, _I32, _F32, _P, _I64, _I64, _P, _I64, _P],
         _I32,
     ),
+    "vflash_rotate": (
+        [_P, _I64, _I64, _P, _I64, _I64, _I32, _I64, _I64, _I64, _I64, _P, _P, _I64, _I32, _F32, _P, _I64, _P, _P, _P],
+        _I32,
+    ),
+    "vflash_paged_append": (
+        [_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I32, _I64, _I64, _I64, _I64, _P, _P, _P, _I64, _I32, _F32, _P,
+         _I64, _P, _P, _I64, _I64, _P, _I64, _P, _I64, _P, _P],
+        _I32,
+    ),
+    "vflash_paged_attention_workspace": ([_I64] * 7, _I64),
+    "vflash_paged_attention": (
+        [_P, _I64, _I64, _I32, _I64, _I64, _I64, _I64, _P, _P, _P, _I64, _I64, _P, _I64, _P, _I64, _F32, _P, _I64, _I64,
+         _P, _I64, _P],
+        _I32,
+    ),
+    "vflash_request_adapters_workspace": ([_I64, _I64, ctypes.POINTER(_I64), _I64, _I64, _I64], _I64),
+    "vflash_request_adapters": (
+        [_P, _I64, _P, _I64, _I32, _I64, _I64, ctypes.POINTER(_I64), _I64, _P, _P, _P, _P, _I64, _I64, _P, _P, _I64, _P,
+         _I64, _P],
+        _I32,
+    ),
     "vflash_nvfp4_w4a4_linear": (
         [_P, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _P, _P, _I64, _P],
         _I32,
@@ -116,7 +137,8 @@ SIGNATURES: dict[str, tuple[list, object]] = {
 }
 
 # What the native host path (csrc/host.cpp) serves.
-HOST_CALLS = ("w8a8_linear", "w8a8_linear_lora", "nvfp4_w16_linear", "packed_attention")
+HOST_CALLS = ("w8a8_linear", "w8a8_linear_lora", "nvfp4_w16_linear", "packed_attention", "rotate", "paged_append",
+              "paged_attention", "request_adapters")
 
 
 class KernelError(RuntimeError):

@@ -129,6 +129,8 @@ struct AttentionSeq {
 // This lane's sequence, base + lane of 0 .. batch + 1 (0 and batch + 1: the rows outside the
 // offsets).  Sequences begin where the one before ends, at the running maximum of the offsets, so
 // that they cover every row once whatever these hold; `reached` carries it from base to base.
+// With PAGED, k0 is the sequence itself, 0 .. batch - 1.
+template <bool PAGED = false>
 __device__ __forceinline__ AttentionSeq attention_sequence(const AttentionParams& p, int64_t base, int& reached) {
   // Clamped to [0, hi] through the 32 bits that are left when the others say which side.
   auto clamp = [](int64_t v, int hi) { return v < 0 ? 0 : (uint64_t)v > (uint64_t)hi ? hi : (int)v; };
@@ -136,19 +138,32 @@ __device__ __forceinline__ AttentionSeq attention_sequence(const AttentionParams
   const bool real = s > 0 && s <= p.batch;
   // Every lane loads, from a place that exists, so that no load waits for another.
   const int64_t at = s < 1 ? 0 : s > p.batch ? p.batch : s, before = at > 0 ? at - 1 : 0;
-  const int64_t from = p.q_offsets[before], to = p.q_offsets[at];
+  int64_t from = before, to = at;  // a token a sequence
+  if (!PAGED || p.q_offsets) {
+    from = p.q_offsets[before];
+    to = p.q_offsets[at];
+  }
   int64_t k0 = 0, kn = 0;
   if (p.batch) {
-    k0 = p.k_offsets[before];
-    kn = (p.k_lengths ? p.k_lengths : p.k_offsets + 1)[before];
+    if constexpr (PAGED) {
+      kn = p.cache.lengths[before];
+    } else {
+      k0 = p.k_offsets[before];
+      kn = (p.k_lengths ? p.k_lengths : p.k_offsets + 1)[before];
+    }
   }
   // Sequence batch + 1 begins where the offsets end; later ones are empty.
   const int first = s == 0 ? 0 : clamp(s > p.batch ? to : from, p.tokens);
   AttentionSeq r;
   r.q0 = max(reached, wave_scan_max(first, (int)threadIdx.x & 63));
   r.nq = s > p.batch + 1 ? 0 : max(0, (s > p.batch ? p.tokens : clamp(to, p.tokens)) - r.q0);
-  r.k0 = clamp(k0, p.keys);
-  r.nk = !real ? 0 : p.k_lengths ? clamp(kn, p.keys - r.k0) : max(0, clamp(kn, p.keys) - r.k0);
+  if constexpr (PAGED) {
+    r.k0 = (int)before;
+    r.nk = real ? clamp(kn, p.keys) : 0;
+  } else {
+    r.k0 = clamp(k0, p.keys);
+    r.nk = !real ? 0 : p.k_lengths ? clamp(kn, p.keys - r.k0) : max(0, clamp(kn, p.keys) - r.k0);
+  }
   reached = __builtin_amdgcn_readlane(r.q0 + r.nq, 63);
   return r;
 }
@@ -361,13 +376,14 @@ __device__ __forceinline__ uint32_t attention_units_of(const AttentionLine& l, c
   return max(1u, ((uint32_t)s.nk + (1u << l.unit_shift) - 1) >> l.unit_shift);
 }
 
+template <bool PAGED = false>
 __device__ __forceinline__ AttentionLine attention_line(const AttentionParams& p, int grid) {
   const int lane = (int)threadIdx.x & 63;
   AttentionLine l{};
   l.unit_shift = p.unit_shift;
   int reached = 0;
   for (int64_t base = 0; base < p.batch + 2; base += 64) {
-    l.mine = attention_sequence(p, base, reached);
+    l.mine = attention_sequence<PAGED>(p, base, reached);
     int sum;
     wave_scan((int)(attention_tiles_of(p, l.mine) * attention_units_of(l, l.mine)), lane, sum);
     l.units += (uint32_t)sum;
@@ -381,6 +397,7 @@ __device__ __forceinline__ AttentionLine attention_line(const AttentionParams& p
 }
 
 // The rest of the tile at unit `pos` (< line.end) of workgroup b's line, up to unit `stop`.
+template <bool PAGED = false>
 __device__ __forceinline__ AttentionSegment attention_segment(const AttentionParams& p, const AttentionLine& line, int b,
                                                               uint32_t pos, uint32_t stop) {
   const int lane = (int)threadIdx.x & 63;
@@ -391,7 +408,7 @@ __device__ __forceinline__ AttentionSegment attention_segment(const AttentionPar
   uint32_t before = 0;
   int reached = 0;
   for (int64_t base = 0; base < n; base += 64) {
-    const AttentionSeq mine = n > 64 ? attention_sequence(p, base, reached) : line.mine;
+    const AttentionSeq mine = n > 64 ? attention_sequence<PAGED>(p, base, reached) : line.mine;
     const uint32_t u = attention_units_of(line, mine), own = attention_tiles_of(p, mine) * u;
     int sum;
     const uint32_t incl = (uint32_t)wave_scan((int)own, lane, sum);

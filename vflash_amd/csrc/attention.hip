@@ -244,7 +244,7 @@ __global__ void __launch_bounds__(256) attention_join(const AttentionParams p, i
 }
 
 // ---------------------------------------------------------------------------
-void launch_attention_step(const AttentionParams&, bool, int, bool, hipStream_t);
+void launch_attention_step(const AttentionParams&, bool, AttentionStore, int, bool, hipStream_t);
 
 namespace {
 
@@ -259,33 +259,58 @@ void launch_tiles(const AttentionParams& p, int64_t grid, hipStream_t s) {
 
 }  // namespace
 
+namespace {
+
+int64_t workspace_of(const AttentionParams& p, const AttentionPlan& plan) { return p.slots * plan.rows * (p.dim + 2) * 4; }
+
+bool plan_fits(const AttentionPlan& plan) {
+  return plan.grid < (int64_t(1) << 24) && plan.join < (int64_t(1) << 24) &&
+         plan.line < (int64_t(1) << 32) - (int64_t(1) << 24);
+}
+
+// The weights' range and the workspace's parts.  `above`: how far above 2^shift a weight may be, as a power of two.
+void attention_memory(AttentionParams& p, const AttentionPlan& plan, int above, void* workspace) {
+  int log = 0;  // at most 2^log keys
+  while ((int64_t(1) << log) < p.keys) ++log;
+  p.shift = -(float)(above + 1 + log);
+  p.bound = exp2f((float)above + p.shift);
+  p.part = static_cast<float*>(workspace);
+  p.part_ml = p.part + p.slots * plan.rows * p.dim;
+}
+
+}  // namespace
+
 // Bytes of workspace that the call may use: partial sums of the splits.
 int64_t attention_workspace(const AttentionParams& params) {
   AttentionParams p = params;
   const AttentionPlan plan = attention_plan(p);
-  return p.slots * plan.rows * (p.dim + 2) * 4;
+  return workspace_of(p, plan);
+}
+
+int64_t paged_attention_workspace(const AttentionParams& params) {
+  AttentionParams p = params;
+  const AttentionPlan plan = paged_attention_plan(p);
+  return workspace_of(p, plan);
 }
 
 // false: the grid would pass HIP's limit, or a line of attention_step 2^32 units (its workgroups'
 // parts end at most a grid past the line).
 bool attention_fits(const AttentionParams& params) {
   AttentionParams p = params;
-  const AttentionPlan plan = attention_plan(p);
-  return plan.grid < (int64_t(1) << 24) && plan.join < (int64_t(1) << 24) &&
-         plan.line < (int64_t(1) << 32) - (int64_t(1) << 24);
+  return plan_fits(attention_plan(p));
+}
+
+bool paged_attention_fits(const AttentionParams& params) {
+  AttentionParams p = params;
+  return plan_fits(paged_attention_plan(p));
 }
 
 hipError_t launch_attention(const AttentionParams& params, bool f16, void* workspace, hipStream_t s) {
   AttentionParams p = params;
   const AttentionPlan plan = attention_plan(p);
-  int log = 0;  // at most 2^log keys
-  while ((int64_t(1) << log) < p.keys) ++log;
-  p.shift = -(float)(21 + log);
-  p.bound = exp2f(20.0f + p.shift);
-  p.part = static_cast<float*>(workspace);
-  p.part_ml = p.part + p.slots * plan.rows * p.dim;
+  attention_memory(p, plan, 20, workspace);
   if (plan.step) {
-    launch_attention_step(p, f16, (int)plan.grid, plan.join != 0, s);
+    launch_attention_step(p, f16, kStoreRows, (int)plan.grid, plan.join != 0, s);
     return hipGetLastError();
   }
   if (f16) launch_tiles<true>(p, plan.grid, s);
@@ -295,6 +320,16 @@ hipError_t launch_attention(const AttentionParams& params, bool f16, void* works
     if (f16) attention_join<true><<<g, dim3(256), 0, s>>>(p, plan.rows);
     else attention_join<false><<<g, dim3(256), 0, s>>>(p, plan.rows);
   }
+  return hipGetLastError();
+}
+
+hipError_t launch_paged_attention(const AttentionParams& params, bool f16, void* workspace, hipStream_t s) {
+  AttentionParams p = params;
+  const AttentionPlan plan = paged_attention_plan(p);
+  // Tiles of 16 follow the maximum once it is 2^8 above: no shift for more, so that weights times the factors of small
+  // E4M3 values stay above bf16's subnormals.
+  attention_memory(p, plan, (int)kAttentionSlack, workspace);
+  launch_attention_step(p, f16, p.cache.scales ? kStoreE4M3 : kStorePages, (int)plan.grid, plan.join != 0, s);
   return hipGetLastError();
 }
 

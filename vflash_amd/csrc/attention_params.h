@@ -4,12 +4,29 @@
 
 namespace vfa {
 
+// Where keys and values lie: rows of two tensors, pages in the operands' type, pages of E4M3 codes.
+enum AttentionStore { kStoreRows, kStorePages, kStoreE4M3 };
+
+// A cache of pages: element (page, k or v, key head, slot, d), contiguous, in the operands' 16-bit type
+// or, with scales, E4M3 codes and a binary32 factor of each (page, k or v, key head, slot).
+struct PagedCacheParams {
+  uint8_t* values;
+  float* scales;  // or null
+  int64_t pages;
+  const int64_t* table;  // [batch][width], the page of keys slot * i .. slot * (i + 1) - 1
+  int64_t width;
+  const int64_t* lengths;  // [batch]
+  int page_shift;          // log2 of a page's keys, 4 at least
+  int key_heads;
+};
+
 struct AttentionParams {
   const uint16_t *q, *k, *v;  // element (row, head, d) at row * *_ts + head * *_hs + d
   uint16_t* out;
   int64_t q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, o_ts, o_hs;
   const int64_t *q_offsets, *k_offsets, *k_lengths;  // k_lengths: or null
-  int tokens, keys;  // rows
+  PagedCacheParams cache;  // pages: these instead of k, v, k_offsets and k_lengths; q_offsets may be null
+  int tokens, keys;  // rows; pages: the most that a sequence has
   int64_t batch;
   int heads, group, dim;  // group: query heads of a key head
   int causal;

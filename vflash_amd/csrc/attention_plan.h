@@ -15,6 +15,51 @@ struct AttentionPlan {
   int64_t line;        // step: units that a line may hold, counted in 32 bits
 };
 
+// The shape of the tiles.
+inline void attention_shape(AttentionParams& p, AttentionPlan& plan, bool step) {
+  plan.step = step;
+  plan.rows = step ? kStepRows : kTileRows;
+  p.heads_per_tile = p.group < plan.rows ? p.group : plan.rows;
+  p.parts = (p.group + p.heads_per_tile - 1) / p.heads_per_tile;
+  p.head_blocks = p.heads / p.group * p.parts;
+  p.tile_tokens = plan.rows / p.heads_per_tile;
+  // Divisions by these two as products: exact below 2^31 and 2^9.
+  p.tile_shift = 31;
+  while ((1 << (p.tile_shift - 31)) < p.tile_tokens) ++p.tile_shift;
+  p.tile_mul = (uint32_t)(((uint64_t(1) << p.tile_shift) + p.tile_tokens - 1) / p.tile_tokens);
+  p.row_mul = (65536 + p.heads_per_tile - 1) / p.heads_per_tile;
+}
+
+// At most a tile per token, or whole tiles and one partial tile per sequence.
+inline int64_t attention_tiles_at_most(const AttentionParams& p) {
+  const int64_t tiles = p.tokens / p.tile_tokens + p.batch + 2;
+  return tiles < p.tokens ? tiles : p.tokens;
+}
+
+// The rest of the plan of tiles of 16.
+inline void attention_step_plan(AttentionParams& p, AttentionPlan& plan, bool split) {
+  // A CU holds one workgroup of dimension 128, two of 64.
+  const int64_t tiles = attention_tiles_at_most(p);
+  p.unit_shift = split ? 7 : 31;
+  auto bound = [&] { return tiles * p.head_blocks * (((int64_t)p.keys >> p.unit_shift) + 1); };
+  while (bound() >= int64_t(1) << 30 && p.unit_shift < 31) ++p.unit_shift;  // the kernel counts in 32 bits
+  const int64_t units = bound();
+  plan.line = p.head_blocks % 8 ? units : units / 8;
+  plan.grid = (compute_units() + 7) / 8 * 8 * (p.dim <= 64 ? 2 : 1);
+  if (units < plan.grid) plan.grid = (units + 7) / 8 * 8;
+  plan.join = split;
+  p.slots = split ? 2 * plan.grid : 0;
+}
+
+// Over a paged cache every call runs in tiles of 16; the keys are split where a sequence has room for more than
+// 768.
+inline AttentionPlan paged_attention_plan(AttentionParams& p) {
+  AttentionPlan plan{};
+  attention_shape(p, plan, true);
+  attention_step_plan(p, plan, p.keys > 768);
+  return plan;
+}
+
 // The launch of a call, from its sizes alone: the lengths are on the device.  Measured as one side
 // and the other, us, head dimension 128, 32 heads over 8 key heads unless said otherwise:
 //   tiles of 16 rows up to 16 rows a sequence and, where two for each sequence and key head are fewer
@@ -37,40 +82,15 @@ struct AttentionPlan {
 inline AttentionPlan attention_plan(AttentionParams& p) {
   const int64_t cus = compute_units();
   AttentionPlan plan{};
-  auto shape = [&](bool step) {
-    plan.step = step;
-    plan.rows = step ? kStepRows : kTileRows;
-    p.heads_per_tile = p.group < plan.rows ? p.group : plan.rows;
-    p.parts = (p.group + p.heads_per_tile - 1) / p.heads_per_tile;
-    p.head_blocks = p.heads / p.group * p.parts;
-    p.tile_tokens = plan.rows / p.heads_per_tile;
-  };
+  auto shape = [&](bool step) { attention_shape(p, plan, step); };
   shape(false);
   const int64_t rows = (int64_t)p.tokens * (p.group < kStepRows ? p.group : kStepRows);
   if (rows <= kStepRows * p.batch || (rows <= 2 * kStepRows * p.batch && 2 * p.batch * p.head_blocks < cus)) shape(true);
-  // Divisions by these two as products: exact below 2^31 and 2^9.
-  p.tile_shift = 31;
-  while ((1 << (p.tile_shift - 31)) < p.tile_tokens) ++p.tile_shift;
-  p.tile_mul = (uint32_t)(((uint64_t(1) << p.tile_shift) + p.tile_tokens - 1) / p.tile_tokens);
-  p.row_mul = (65536 + p.heads_per_tile - 1) / p.heads_per_tile;
-  // At most a tile per token, or whole tiles and one partial tile per sequence.
-  const int64_t whole = p.tokens / p.tile_tokens;
-  int64_t tiles = whole + p.batch + 2;
-  if (tiles > p.tokens) tiles = p.tokens;
   if (plan.step) {
-    // A CU holds one workgroup of dimension 128, two of 64.
-    const bool split = p.keys > 768 && p.keys > 512 * p.batch;
-    p.unit_shift = split ? 7 : 31;
-    auto bound = [&] { return tiles * p.head_blocks * (((int64_t)p.keys >> p.unit_shift) + 1); };
-    while (bound() >= int64_t(1) << 30 && p.unit_shift < 31) ++p.unit_shift;  // the kernel counts in 32 bits
-    const int64_t units = bound();
-    plan.line = p.head_blocks % 8 ? units : units / 8;
-    plan.grid = (cus + 7) / 8 * 8 * (p.dim <= 64 ? 2 : 1);
-    if (units < plan.grid) plan.grid = (units + 7) / 8 * 8;
-    plan.join = split;
-    p.slots = split ? 2 * plan.grid : 0;
+    attention_step_plan(p, plan, p.keys > 768 && p.keys > 512 * p.batch);
     return plan;
   }
+  const int64_t tiles = attention_tiles_at_most(p), whole = p.tokens / p.tile_tokens;
   // About how many tiles there are: whole ones, or one a sequence.
   int64_t about = p.batch < p.tokens ? p.batch : p.tokens;
   if (about < whole) about = whole;

@@ -10,15 +10,22 @@
 // waves' sums are added up.  131071 keys of 8 heads of 128: 107 us, 5.0 TB/s, what a copy of 1 GiB
 // reaches; 16 sequences of up to 8191: 65 us, 4.2 TB/s; 77 keys: 7.5 us a call, a chain of loads, search
 // and sums in one wave after another.
+//
+// A paged cache differs in where a block's keys come from: each 16 lie in one page, whose number a scalar
+// load fetches one block ahead.  E4M3 codes go to LDS as they are, with their factors, and become 16 bits between
+// LDS and the matrix cores (exactly): a key's factor multiplies its score, a value's its weight before that is
+// rounded, to bf16 whatever q's type (a factor has binary32's range).
 #include "attention.h"
 
 namespace vfa {
 
-template <int DP>
+template <int DP, int STORE>
 struct AttentionSteps {
-  static constexpr int PITCH = DP <= 64 ? 128 : 256, CHUNKS = PITCH / 16, ROWS = 1024 / PITCH;
-  static constexpr int KEYS = 32, TILE = KEYS * PITCH, SLOT = 2 * TILE, NS = 2, WAVES = 4;
-  static constexpr int DMA = SLOT / 1024;  // instructions per stage
+  static constexpr bool E4M3 = STORE == kStoreE4M3;
+  static constexpr int PITCH = (DP <= 64 ? 64 : 128) * (E4M3 ? 1 : 2), CHUNKS = PITCH / 16, ROWS = 1024 / PITCH;
+  static constexpr int KEYS = 32, TILE = KEYS * PITCH, SLOT = 2 * TILE + (E4M3 ? 512 : 0), WAVES = 4;
+  static constexpr int NS = E4M3 ? 4 : 2;
+  static constexpr int DMA = 2 * TILE / 1024 + (E4M3 ? 2 : 0);  // instructions per stage
   static constexpr int ACC = DP * 4 + 16;  // bytes of a row's sums in LDS
 };
 template <int PITCH>
@@ -31,9 +38,48 @@ __device__ __forceinline__ int step_v_swizzle(int r) {
   return PITCH == 256 ? (r & 7) << 1 : (r >> 1 & 3) << 1;
 }
 
-template <bool F16, int DP>
+// Tiles of codes: the 16 rows of a score block, and the eight rows of a transposing read (four keys from each
+// half of the block), take different slots.
+template <int PITCH>
+__device__ __forceinline__ int step_k_code_swizzle(int r) {
+  return PITCH == 128 ? r >> 1 & 7 : r >> 2 & 3;
+}
+template <int PITCH>
+__device__ __forceinline__ int step_v_code_swizzle(int r) {
+  return PITCH == 128 ? (r >> 1 & 3) | (r >> 4 & 1) << 2 : (r >> 2 & 1) | (r >> 4 & 1) << 1;
+}
+
+// Eight E4M3 codes as 16-bit operands of a product; exact.
+template <bool F16>
+__device__ __forceinline__ v4i step_widen(v2i c) {
+  v4i w;
+  static_for<4>([&](auto i) {
+    if constexpr (F16)
+      w[(int)i] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c[i / 2], 1.0f, (i & 1) != 0));
+    else
+      w[(int)i] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[i / 2], 1.0f, (i & 1) != 0));
+  });
+  return w;
+}
+// Eight bytes per lane, transposed inside each group of 16 lanes: lanes 2 r and 2 r + 1 give the address of
+// elements 0 .. 7 and 8 .. 15 of row r, and lane i receives element i of the eight rows.
+__device__ __forceinline__ v2i lds_read_tr8(const uint8_t* p) {
+  typedef __attribute__((address_space(3))) v2i lds_v2i;
+  return __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i*)(uint32_t)lds_addr(p));
+}
+// lds_dma16 with four bytes a lane.
+__device__ __forceinline__ void lds_dma4(__amdgpu_buffer_rsrc_t r, uint32_t lds_dst, uint32_t voffset) {
+  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+               :
+               : "s"(lds_dst), "v"(voffset), "s"(r)
+               : "m0");
+}
+
+template <bool F16, int DP, int STORE>
 __global__ void __launch_bounds__(256, 1) attention_step(const AttentionParams p) {
-  using L = AttentionSteps<DP>;
+  using L = AttentionSteps<DP, STORE>;
+  constexpr bool PAGED = STORE != kStoreRows, E4M3 = L::E4M3;
+  constexpr bool W16 = F16 && !E4M3;  // the type of the weights
   constexpr int QS = (DP + 31) / 32, DB = DP / 16;
   __shared__ __attribute__((aligned(1024))) uint8_t lds[L::WAVES * L::NS * L::SLOT];
   __shared__ float stat[L::WAVES][16][2];
@@ -44,10 +90,10 @@ __global__ void __launch_bounds__(256, 1) attention_step(const AttentionParams p
   uint8_t* ring = lds + wave * (L::NS * L::SLOT);
   const uint32_t ring_lds = __builtin_amdgcn_readfirstlane(lds_addr(ring));
 
-  const AttentionLine line = attention_line(p, gridDim.x);
+  const AttentionLine line = attention_line<PAGED>(p, gridDim.x);
   const uint32_t begin = (blockIdx.x >> (line.xcds == 8 ? 3 : 0)) * line.quota, stop = min(begin + line.quota, line.end);
   for (uint32_t pos = begin; pos < stop;) {
-    const AttentionSegment seg = attention_segment(p, line, blockIdx.x, pos, stop);
+    const AttentionSegment seg = attention_segment<PAGED>(p, line, blockIdx.x, pos, stop);
     const AttentionItem& it = seg.it;
     if (!it.live) return;
     const AttentionRow row = attention_row(p, it, fr);
@@ -60,29 +106,73 @@ __global__ void __launch_bounds__(256, 1) attention_step(const AttentionParams p
     // Keys that every row sees.
     const int open = min(attention_limit(p, it.seq, min(it.tile * p.tile_tokens, it.seq.nq)), last);
 
-    const uint8_t* kb = reinterpret_cast<const uint8_t*>(p.k + (int64_t)it.seq.k0 * p.k_ts + (int64_t)key_head * p.k_hs);
-    const uint8_t* vb = reinterpret_cast<const uint8_t*>(p.v + (int64_t)it.seq.k0 * p.v_ts + (int64_t)key_head * p.v_hs);
-    const uint32_t kts = (uint32_t)p.k_ts * 2, vts = (uint32_t)p.v_ts * 2;
     const int drow = lane / L::CHUNKS, dslot = lane % L::CHUNKS;
+    int64_t pages[2] = {-1, -1};  // of the next block's halves
+    auto look = [&](int key0) {
+      if constexpr (PAGED) {
+        if (last <= 0) return;
+        typedef const __attribute__((address_space(4))) int64_t table_t;  // scalar loads, waited for where they are used
+        table_t* row = (table_t*)(uintptr_t)(p.cache.table + (int64_t)it.seq.k0 * p.cache.width);
+        static_for<2>([&](auto h) { pages[h] = row[min(key0 + 16 * h, last - 1) >> p.cache.page_shift]; });
+      }
+    };
     auto issue = [&](int buf, int key0) {
       const int left = last - key0;  // none: every lane reads zeros
-      const __amdgpu_buffer_rsrc_t rk = make_rsrc(kb + (int64_t)key0 * kts, 0x7fffffffu);
-      const __amdgpu_buffer_rsrc_t rv = make_rsrc(vb + (int64_t)key0 * vts, 0x7fffffffu);
       const uint32_t dst = ring_lds + buf * L::SLOT;
-      static_for<L::DMA / 2>([&](auto i) {
-        const int r = drow + i * L::ROWS;
-        const int c = dslot ^ step_k_swizzle<L::PITCH>(r);
-        lds_dma16(rk, dst + i * 1024, r < left && c * 8 < p.dim ? (uint32_t)r * kts + c * 16 : VFA_OOB);
-      });
-      static_for<L::DMA / 2>([&](auto i) {
-        const int r = drow + i * L::ROWS;
-        const int c = dslot ^ step_v_swizzle<L::PITCH>(r);
-        lds_dma16(rv, dst + L::TILE + i * 1024, r < left && c * 8 < p.dim ? (uint32_t)r * vts + c * 16 : VFA_OOB);
-      });
+      if constexpr (!PAGED) {
+        const uint8_t* kb = reinterpret_cast<const uint8_t*>(p.k + (int64_t)it.seq.k0 * p.k_ts + (int64_t)key_head * p.k_hs);
+        const uint8_t* vb = reinterpret_cast<const uint8_t*>(p.v + (int64_t)it.seq.k0 * p.v_ts + (int64_t)key_head * p.v_hs);
+        const uint32_t kts = (uint32_t)p.k_ts * 2, vts = (uint32_t)p.v_ts * 2;
+        const __amdgpu_buffer_rsrc_t rk = make_rsrc(kb + (int64_t)key0 * kts, 0x7fffffffu);
+        const __amdgpu_buffer_rsrc_t rv = make_rsrc(vb + (int64_t)key0 * vts, 0x7fffffffu);
+        static_for<L::TILE / 1024>([&](auto i) {
+          const int r = drow + i * L::ROWS;
+          const int c = dslot ^ step_k_swizzle<L::PITCH>(r);
+          lds_dma16(rk, dst + i * 1024, r < left && c * 8 < p.dim ? (uint32_t)r * kts + c * 16 : VFA_OOB);
+        });
+        static_for<L::TILE / 1024>([&](auto i) {
+          const int r = drow + i * L::ROWS;
+          const int c = dslot ^ step_v_swizzle<L::PITCH>(r);
+          lds_dma16(rv, dst + L::TILE + i * 1024, r < left && c * 8 < p.dim ? (uint32_t)r * vts + c * 16 : VFA_OOB);
+        });
+      } else {
+        constexpr int PER = L::TILE / 2048;  // instructions of 16 keys
+        const uint32_t row_bytes = (uint32_t)p.dim * (E4M3 ? 1 : 2);
+        const int64_t head_rows = (int64_t)p.cache.key_heads << p.cache.page_shift;  // from a page's keys to its values
+        static_for<2>([&](auto h) {
+          const bool none = (uint64_t)pages[h] >= (uint64_t)p.cache.pages;  // reads zeros
+          const uint32_t size = none ? 0 : 0x7fffffffu;
+          const int64_t row = none ? 0
+                                   : 2 * pages[h] * head_rows + ((int64_t)key_head << p.cache.page_shift) +
+                                         ((key0 + 16 * h) & ((1 << p.cache.page_shift) - 1));
+          const uint8_t* at = p.cache.values + row * row_bytes;
+          const __amdgpu_buffer_rsrc_t rk = make_rsrc(at, size), rv = make_rsrc(at + head_rows * row_bytes, size);
+          static_for<PER>([&](auto i) {
+            const int r = drow + (h * PER + i) * L::ROWS;
+            const int c = dslot ^ (E4M3 ? step_k_code_swizzle<L::PITCH>(r) : step_k_swizzle<L::PITCH>(r));
+            lds_dma16(rk, dst + (h * PER + i) * 1024,
+                      r < left && (uint32_t)c * 16 < row_bytes ? (uint32_t)(r - 16 * h) * row_bytes + c * 16 : VFA_OOB);
+          });
+          static_for<PER>([&](auto i) {
+            const int r = drow + (h * PER + i) * L::ROWS;
+            const int c = dslot ^ (E4M3 ? step_v_code_swizzle<L::PITCH>(r) : step_v_swizzle<L::PITCH>(r));
+            lds_dma16(rv, dst + L::TILE + (h * PER + i) * 1024,
+                      r < left && (uint32_t)c * 16 < row_bytes ? (uint32_t)(r - 16 * h) * row_bytes + c * 16 : VFA_OOB);
+          });
+          if constexpr (E4M3)  // 16 keys' factors, then 16 values'
+            lds_dma4(make_rsrc(p.cache.scales + row, size), dst + 2 * L::TILE + h * 256,
+                     lane < 32 && 16 * h + (lane & 15) < left
+                         ? 4 * ((uint32_t)(lane & 15) + (lane & 16 ? (uint32_t)head_rows : 0)) : VFA_OOB);
+        });
+      }
     };
     constexpr int STRIDE = L::WAVES * L::KEYS;
     const int start = first + wave * L::KEYS;
-    static_for<L::NS>([&](auto i) { issue(i, start + i * STRIDE); });
+    look(start);
+    static_for<L::NS>([&](auto i) {
+      issue(i, start + i * STRIDE);
+      look(start + (i + 1) * STRIDE);
+    });
 
     v4i q[QS];
     static_for<QS>([&](auto s) { q[s] = attention_query(p, it, row, s * 32 + fg * 8); });
@@ -90,12 +180,13 @@ __global__ void __launch_bounds__(256, 1) attention_step(const AttentionParams p
     static_for<DB>([&](auto i) { o[i] = v4f{}; });
     float m = VFA_LOWEST, l = 0;
     bool far = false;
-    const uint8_t* krow = ring + fr * L::PITCH;
-    const int ksw = step_k_swizzle<L::PITCH>(fr);
-    const int vr = 4 * fg + ((lane >> 2) & 3);
+    const uint8_t* krow = ring + fr * L::PITCH + (E4M3 ? (fg & 1) * 8 : 0);
+    const int ksw = E4M3 ? step_k_code_swizzle<L::PITCH>(fr) : step_k_swizzle<L::PITCH>(fr);
+    const int vr = E4M3 ? 4 * fg + (lane >> 1 & 3) + (lane & 8) * 2 : 4 * fg + ((lane >> 2) & 3);
     const int vc = (lane & 3) >> 1;
     const uint8_t* vrow = ring + L::TILE + vr * L::PITCH + (lane & 1) * 8;
-    const int vsw = step_v_swizzle<L::PITCH>(vr);
+    const int vsw = E4M3 ? step_v_code_swizzle<L::PITCH>(vr) : step_v_swizzle<L::PITCH>(vr);
+    const uint8_t* factors = ring + 2 * L::TILE + 16 * fg;
 
     int buf = 0;
     for (int key0 = start; key0 < last; key0 += STRIDE, buf = buf + 1 == L::NS ? 0 : buf + 1) {
@@ -105,10 +196,13 @@ __global__ void __launch_bounds__(256, 1) attention_step(const AttentionParams p
       static_for<2>([&](auto kbk) {
         s[kbk] = v4f{};
         static_for<QS>([&](auto st) {
-          const v4i a = *reinterpret_cast<const v4i*>(krow + buf * L::SLOT + kbk * 16 * L::PITCH +
-                                                      (((4 * st + fg) ^ ksw) << 4));
+          const uint8_t* src = krow + buf * L::SLOT + kbk * 16 * L::PITCH;
+          v4i a;
+          if constexpr (E4M3) a = step_widen<F16>(*reinterpret_cast<const v2i*>(src + (((2 * st + (fg >> 1)) ^ ksw) << 4)));
+          else a = *reinterpret_cast<const v4i*>(src + (((4 * st + fg) ^ ksw) << 4));
           s[kbk] = mfma16<F16>(a, q[st], s[kbk]);
         });
+        if constexpr (E4M3) s[kbk] *= *reinterpret_cast<const v4f*>(factors + buf * L::SLOT + kbk * 256);
       });
       if (key0 + L::KEYS > open) {
         const int lim = limit - key0 - 4 * fg;
@@ -126,26 +220,39 @@ __global__ void __launch_bounds__(256, 1) attention_step(const AttentionParams p
         m = next;
         far = __builtin_amdgcn_ballot_w64(fabsf(m * p.c) >= kAttentionFar && m > VFA_LOWEST) != 0;
       }
-      const float ref = attention_shift<F16>(p) - attention_top(m, p.c);
+      const float ref = attention_shift<W16>(p) - attention_top(m, p.c);
       v4i pk;
       auto weights = [&](auto far_rows) {
         static_for<4>([&](auto j) {
           constexpr int r = (j % 2) * 2;
-          pk[(int)j] = pack2<F16>(attention_weight<far_rows>(s[j / 2][r], p.c, m, ref, attention_shift<F16>(p)),
-                                  attention_weight<far_rows>(s[j / 2][r + 1], p.c, m, ref, attention_shift<F16>(p)));
-          l = attention_sum2<F16>(pk[(int)j], l);
+          const float w0 = attention_weight<far_rows>(s[j / 2][r], p.c, m, ref, attention_shift<W16>(p));
+          const float w1 = attention_weight<far_rows>(s[j / 2][r + 1], p.c, m, ref, attention_shift<W16>(p));
+          if constexpr (E4M3) {
+            const v2f f = *reinterpret_cast<const v2f*>(factors + buf * L::SLOT + (j / 2) * 256 + 64 + r * 4);
+            pk[(int)j] = pack2<W16>(w0 * f[0], w1 * f[1]);
+            l += w0 + w1;
+          } else {
+            pk[(int)j] = pack2<W16>(w0, w1);
+            l = attention_sum2<W16>(pk[(int)j], l);
+          }
         });
       };
       if (far) weights(std::true_type{});
       else weights(std::false_type{});
       static_for<DB>([&](auto db) {
-        const uint8_t* src = vrow + buf * L::SLOT + (((2 * db + vc) ^ vsw) << 4);
-        const v2i lo = lds_read_tr16(src), hi = lds_read_tr16(src + 16 * L::PITCH);
-        o[db] = mfma16<F16>(v4i{lo[0], lo[1], hi[0], hi[1]}, pk, o[db]);
+        if constexpr (E4M3) {
+          const v4i a = step_widen<false>(lds_read_tr8(vrow + buf * L::SLOT + ((db ^ vsw) << 4)));
+          o[db] = mfma16<W16>(a, pk, o[db]);
+        } else {
+          const uint8_t* src = vrow + buf * L::SLOT + (((2 * db + vc) ^ vsw) << 4);
+          const v2i lo = lds_read_tr16(src), hi = lds_read_tr16(src + 16 * L::PITCH);
+          o[db] = mfma16<W16>(v4i{lo[0], lo[1], hi[0], hi[1]}, pk, o[db]);
+        }
       });
       __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the slot is read
       asm volatile("" ::: "memory");
       issue(buf, key0 + L::NS * STRIDE);
+      look(key0 + (L::NS + 1) * STRIDE);
     }
     l = sum_across32(sum_across16(l));
     wait_vmcnt<0, true>();
@@ -191,13 +298,13 @@ __global__ void __launch_bounds__(256, 1) attention_step(const AttentionParams p
 // The sum over a tile's segments: out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s.  Workgroup b
 // takes the tile that workgroup b of attention_step began and did not end.  Thread t: d 4 (t % 16) and
 // 64 more, one row, every groups-th segment under a maximum of its own; the groups meet in LDS.
-template <bool F16>
+template <bool F16, bool PAGED>
 __global__ void __launch_bounds__(1024) attention_step_join(const AttentionParams p) {
-  const AttentionLine line = attention_line(p, gridDim.x);
+  const AttentionLine line = attention_line<PAGED>(p, gridDim.x);
   const int part = blockIdx.x >> (line.xcds == 8 ? 3 : 0);
   const uint32_t begin = part * line.quota, stop = min(begin + line.quota, line.end);
   if (begin >= stop) return;
-  const AttentionSegment seg = attention_segment(p, line, blockIdx.x, stop - 1, line.end);
+  const AttentionSegment seg = attention_segment<PAGED>(p, line, blockIdx.x, stop - 1, line.end);
   const uint32_t tile_begin = stop - 1 - seg.first, tile_end = tile_begin + seg.of;
   if (!seg.it.live || tile_begin < begin || tile_end <= stop) return;
   const int segments = (int)((tile_end - 1) / line.quota) - part + 1;
@@ -253,18 +360,22 @@ __global__ void __launch_bounds__(1024) attention_step_join(const AttentionParam
   });
 }
 
-void launch_attention_step(const AttentionParams& p, bool f16, int grid, bool join, hipStream_t s) {
+template <bool F16, int STORE>
+static void launch_step(const AttentionParams& p, int grid, bool join, hipStream_t s) {
   const dim3 g((unsigned)grid), b(256);
-  if (p.dim <= 64) {
-    if (f16) attention_step<true, 64><<<g, b, 0, s>>>(p);
-    else attention_step<false, 64><<<g, b, 0, s>>>(p);
-  } else {
-    if (f16) attention_step<true, 128><<<g, b, 0, s>>>(p);
-    else attention_step<false, 128><<<g, b, 0, s>>>(p);
-  }
-  if (!join) return;
-  if (f16) attention_step_join<true><<<g, dim3(1024), 0, s>>>(p);
-  else attention_step_join<false><<<g, dim3(1024), 0, s>>>(p);
+  if (p.dim <= 64) attention_step<F16, 64, STORE><<<g, b, 0, s>>>(p);
+  else attention_step<F16, 128, STORE><<<g, b, 0, s>>>(p);
+  if (join) attention_step_join<F16, STORE != kStoreRows><<<g, dim3(1024), 0, s>>>(p);
+}
+
+void launch_attention_step(const AttentionParams& p, bool f16, AttentionStore store, int grid, bool join, hipStream_t s) {
+  auto of = [&](auto stored) {
+    if (f16) launch_step<true, stored>(p, grid, join, s);
+    else launch_step<false, stored>(p, grid, join, s);
+  };
+  if (store == kStoreE4M3) of(std::integral_constant<int, kStoreE4M3>{});
+  else if (store == kStorePages) of(std::integral_constant<int, kStorePages>{});
+  else of(std::integral_constant<int, kStoreRows>{});
 }
 
 }  // namespace vfa

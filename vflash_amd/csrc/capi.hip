@@ -10,6 +10,8 @@
 #include "attention_params.h"
 #include "common.h"
 #include "gemm_params.h"
+#include "paged_params.h"
+#include "request_adapters.h"
 
 namespace vfa {
 hipError_t launch_quant_rows(const uint16_t*, int64_t, int64_t, int64_t, uint8_t*, float*,
@@ -40,6 +42,12 @@ hipError_t launch_nvfp4_w16(const GemmParams&, bool, hipStream_t);
 int64_t attention_workspace(const AttentionParams&);
 bool attention_fits(const AttentionParams&);
 hipError_t launch_attention(const AttentionParams&, bool, void*, hipStream_t);
+int64_t paged_attention_workspace(const AttentionParams&);
+bool paged_attention_fits(const AttentionParams&);
+hipError_t launch_paged_attention(const AttentionParams&, bool, void*, hipStream_t);
+hipError_t launch_rotate(const RotateParams&, hipStream_t);
+int64_t request_workspace(const RequestAdapterParams&);
+hipError_t launch_request_adapters(const RequestAdapterParams&, bool, void*, hipStream_t);
 }  // namespace vfa
 
 namespace {
@@ -158,6 +166,89 @@ bool attention_sizes(vfa::AttentionParams& p, int64_t tokens, int64_t keys, int6
   p.group = (int)(heads / key_heads);
   p.dim = (int)dim;
   return vfa::attention_fits(p);
+}
+
+constexpr int64_t ROWS_LIMIT = int64_t(1) << 30;
+
+// Sizes of a call over a paged cache.
+bool paged_sizes(vfa::PagedCacheParams& c, int64_t pages, int64_t page, int64_t width, int64_t batch, int64_t key_heads,
+                 int64_t dim, bool codes) {
+  if (pages < 0 || pages >= ROWS_LIMIT || width < 1 || width >= ROWS_LIMIT || batch < 0 || batch >= ROWS_LIMIT) return false;
+  if (page < 16 || page > 4096 || (page & (page - 1)) || width * page >= ROWS_LIMIT) return false;
+  if (key_heads < 1 || key_heads > 4096 || dim < 8 || dim > 128 || dim % (codes ? 16 : 8)) return false;
+  c.pages = pages;
+  c.width = width;
+  c.key_heads = (int)key_heads;
+  c.page_shift = 0;
+  while ((int64_t(1) << c.page_shift) < page) ++c.page_shift;
+  return true;
+}
+
+bool set_cache(vfa::PagedCacheParams& c, void* values, float* scales, const int64_t* table, const int64_t* lengths,
+               int64_t batch) {
+  if ((c.pages && !values) || !aligned(values, 16) || !aligned(scales, 4) || !aligned(table, 8) || !aligned(lengths, 8))
+    return false;
+  if (batch && (!table || !lengths)) return false;
+  c.values = static_cast<uint8_t*>(values);
+  c.scales = scales;
+  c.table = table;
+  c.lengths = lengths;
+  return true;
+}
+
+bool paged_attention_sizes(vfa::AttentionParams& p, int64_t tokens, int64_t batch, int64_t heads, int64_t key_heads,
+                           int64_t dim, int64_t pages, int64_t page, int64_t width, bool codes) {
+  if (tokens < 1 || tokens >= ROWS_LIMIT || !paged_sizes(p.cache, pages, page, width, batch, key_heads, dim, codes))
+    return false;
+  if (heads < key_heads || heads % key_heads || heads >= ROWS_LIMIT / 2) return false;
+  p.tokens = (int)tokens;
+  p.keys = (int)(width * page);
+  p.batch = batch;
+  p.heads = (int)heads;
+  p.group = (int)(heads / key_heads);
+  p.dim = (int)dim;
+  p.causal = 1;
+  return vfa::paged_attention_fits(p);
+}
+
+// Rows [tokens, heads, dim] that 16-byte vectors can be taken from.
+bool head_rows_ok(const void* x, int64_t ts, int64_t hs) {
+  return x && aligned(x, 16) && ts >= 0 && hs >= 0 && ts % 8 == 0 && hs % 8 == 0;
+}
+
+bool set_rotary(vfa::RotaryParams& r, const uint64_t* phases, const int64_t* axis, int64_t pairs, int interleaved,
+                float magnitude, const int64_t* positions, int64_t axes, int64_t dim) {
+  if (!phases || !aligned(phases, 8) || !aligned(axis, 8) || !aligned(positions, 8)) return false;
+  if (pairs < 1 || 2 * pairs > dim || axes < 1 || axes > 64 || (axes > 1 && !positions)) return false;
+  if (!(magnitude > -3.4e38f && magnitude < 3.4e38f)) return false;
+  r.phases = phases;
+  r.axis = axis;
+  r.positions = positions;
+  r.axes = (int)axes;
+  r.pairs = (int)pairs;
+  r.interleaved = interleaved != 0;
+  r.magnitude = magnitude;
+  return true;
+}
+
+bool request_sizes(vfa::RequestAdapterParams& p, int64_t rows, int64_t k, const int64_t* widths, int64_t branches,
+                   int64_t adapters, int64_t width) {
+  if (rows < 1 || rows >= (int64_t(1) << 24) || k < 8 || k % 8 || k >= ROWS_LIMIT || !widths) return false;
+  if (branches < 1 || branches > vfa::RA_BRANCHES || adapters < 1 || adapters >= 8192) return false;
+  if (width < 16 || width > 128 || width % 16) return false;
+  int64_t n = 0;
+  for (int64_t b = 0; b < branches; ++b) {
+    if (widths[b] < 8 || widths[b] % 8 || widths[b] >= (int64_t(1) << 21)) return false;
+    n += widths[b];
+    p.ends[b] = (int)n;
+  }
+  p.rows = rows;
+  p.k = k;
+  p.n = n;
+  p.adapters = (int)adapters;
+  p.branches = (int)branches;
+  p.width = (int)width;
+  return true;
 }
 
 }  // namespace
@@ -554,6 +645,135 @@ int vflash_packed_attention(const void* q, int64_t q_ts, int64_t q_hs, const voi
   p.k_lengths = k_lengths;
   p.causal = causal != 0;
   return status(vfa::launch_attention(p, f16 != 0, workspace, static_cast<hipStream_t>(stream)));
+}
+
+int vflash_rotate(const void* q, int64_t q_ts, int64_t q_hs, const void* k, int64_t k_ts, int64_t k_hs, int f16,
+                  int64_t tokens, int64_t heads, int64_t key_heads, int64_t dim, const uint64_t* phases,
+                  const int64_t* axis, int64_t pairs, int interleaved, float magnitude, const int64_t* positions,
+                  int64_t axes, void* q_out, void* k_out, void* stream) {
+  vfa::RotateParams p{};
+  if (tokens < 1 || tokens >= ROWS_LIMIT || heads < 1 || heads > 65536 || dim < 8 || dim > 256 || dim % 8) return VFLASH_EINVAL;
+  if (!head_rows_ok(q, q_ts, q_hs) || !q_out || !aligned(q_out, 16) || !positions) return VFLASH_EINVAL;
+  if (k && (key_heads < 1 || key_heads > 65536 || !head_rows_ok(k, k_ts, k_hs) || !k_out || !aligned(k_out, 16)))
+    return VFLASH_EINVAL;
+  if (!set_rotary(p.rotary, phases, axis, pairs, interleaved, magnitude, positions, axes, dim)) return VFLASH_EINVAL;
+  p.q = static_cast<const uint16_t*>(q);
+  p.k = static_cast<const uint16_t*>(k);
+  p.q_ts = q_ts;
+  p.q_hs = q_hs;
+  p.k_ts = k_ts;
+  p.k_hs = k_hs;
+  p.q_out = static_cast<uint16_t*>(q_out);
+  p.k_out = static_cast<uint16_t*>(k_out);
+  p.tokens = tokens;
+  p.heads = (int)heads;
+  p.key_heads = k ? (int)key_heads : 0;
+  p.dim = (int)dim;
+  p.f16 = f16 != 0;
+  return status(vfa::launch_rotate(p, static_cast<hipStream_t>(stream)));
+}
+
+int vflash_paged_append(const void* q, int64_t q_ts, int64_t q_hs, const void* k, int64_t k_ts, int64_t k_hs,
+                        const void* v, int64_t v_ts, int64_t v_hs, int f16, int64_t tokens, int64_t heads,
+                        int64_t key_heads, int64_t dim, const int64_t* q_offsets, const uint64_t* phases,
+                        const int64_t* axis, int64_t pairs, int interleaved, float magnitude, const int64_t* positions,
+                        int64_t axes, void* values, float* scales, int64_t pages, int64_t page, const int64_t* table,
+                        int64_t width, const int64_t* lengths, int64_t batch, void* q_out, void* stream) {
+  vfa::RotateParams p{};
+  if (tokens < 1 || tokens >= ROWS_LIMIT || !values) return VFLASH_EINVAL;
+  if (!paged_sizes(p.cache, pages, page, width, batch, key_heads, dim, scales != nullptr) ||
+      !set_cache(p.cache, values, scales, table, lengths, batch))
+    return VFLASH_EINVAL;
+  if (!head_rows_ok(k, k_ts, k_hs) || !head_rows_ok(v, v_ts, v_hs)) return VFLASH_EINVAL;
+  if (q && (heads < 1 || heads > 65536 || !head_rows_ok(q, q_ts, q_hs) || !q_out || !aligned(q_out, 16))) return VFLASH_EINVAL;
+  if ((q && !phases) || !aligned(q_offsets, 8) || (!q_offsets && tokens != batch)) return VFLASH_EINVAL;
+  if (phases && !set_rotary(p.rotary, phases, axis, pairs, interleaved, magnitude, positions, axes, dim)) return VFLASH_EINVAL;
+  p.q = static_cast<const uint16_t*>(q);
+  p.k = static_cast<const uint16_t*>(k);
+  p.v = static_cast<const uint16_t*>(v);
+  p.q_ts = q_ts;
+  p.q_hs = q_hs;
+  p.k_ts = k_ts;
+  p.k_hs = k_hs;
+  p.v_ts = v_ts;
+  p.v_hs = v_hs;
+  p.q_out = q ? static_cast<uint16_t*>(q_out) : nullptr;
+  p.tokens = tokens;
+  p.batch = batch;
+  p.heads = q ? (int)heads : 0;
+  p.key_heads = (int)key_heads;
+  p.dim = (int)dim;
+  p.f16 = f16 != 0;
+  p.q_offsets = q_offsets;
+  return status(vfa::launch_rotate(p, static_cast<hipStream_t>(stream)));
+}
+
+int64_t vflash_paged_attention_workspace(int64_t tokens, int64_t batch, int64_t heads, int64_t key_heads, int64_t dim,
+                                         int64_t page, int64_t width) {
+  vfa::AttentionParams p{};
+  if (!paged_attention_sizes(p, tokens, batch, heads, key_heads, dim, 0, page, width, false)) return VFLASH_EINVAL;
+  return vfa::paged_attention_workspace(p);
+}
+
+int vflash_paged_attention(const void* q, int64_t q_ts, int64_t q_hs, int f16, int64_t tokens, int64_t heads,
+                           int64_t key_heads, int64_t dim, const int64_t* q_offsets, const void* values,
+                           const float* scales, int64_t pages, int64_t page, const int64_t* table, int64_t width,
+                           const int64_t* lengths, int64_t batch, float scale, void* out, int64_t o_ts, int64_t o_hs,
+                           void* workspace, int64_t workspace_bytes, void* stream) {
+  vfa::AttentionParams p{};
+  if (!paged_attention_sizes(p, tokens, batch, heads, key_heads, dim, pages, page, width, scales != nullptr))
+    return VFLASH_EINVAL;
+  if (!set_cache(p.cache, const_cast<void*>(values), const_cast<float*>(scales), table, lengths, batch)) return VFLASH_EINVAL;
+  if (!head_rows_ok(q, q_ts, q_hs) || !head_rows_ok(out, o_ts, o_hs)) return VFLASH_EINVAL;
+  if (!aligned(q_offsets, 8) || (!q_offsets && tokens != batch)) return VFLASH_EINVAL;
+  if (!(o_hs >= dim && o_ts >= (heads - 1) * o_hs + dim) && !(o_ts >= dim && o_hs >= (tokens - 1) * o_ts + dim))
+    return VFLASH_EINVAL;
+  p.c = scale * 1.4426950408889634f;
+  if (!(p.c > 0.0f) || p.c > 3.4028234663852886e38f) return VFLASH_EINVAL;  // rejects NaN and infinity too
+  const int64_t need = vfa::paged_attention_workspace(p);
+  if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16))) return VFLASH_EINVAL;
+  p.q = static_cast<const uint16_t*>(q);
+  p.out = static_cast<uint16_t*>(out);
+  p.q_ts = q_ts;
+  p.q_hs = q_hs;
+  p.o_ts = o_ts;
+  p.o_hs = o_hs;
+  p.q_offsets = q_offsets;
+  return status(vfa::launch_paged_attention(p, f16 != 0, workspace, static_cast<hipStream_t>(stream)));
+}
+
+int64_t vflash_request_adapters_workspace(int64_t rows, int64_t k, const int64_t* widths, int64_t branches,
+                                          int64_t adapters, int64_t width) {
+  vfa::RequestAdapterParams p{};
+  if (!request_sizes(p, rows, k, widths, branches, adapters, width)) return VFLASH_EINVAL;
+  return vfa::request_workspace(p);
+}
+
+int vflash_request_adapters(const void* base, int64_t ldb, const void* x, int64_t ldx, int f16, int64_t rows, int64_t k,
+                            const int64_t* widths, int64_t branches, const void* down, const void* up,
+                            const float* scaling, const int32_t* ranks, int64_t adapters, int64_t width,
+                            const int64_t* index, void* out, int64_t ldo, void* workspace, int64_t workspace_bytes,
+                            void* stream) {
+  vfa::RequestAdapterParams p{};
+  if (!request_sizes(p, rows, k, widths, branches, adapters, width)) return VFLASH_EINVAL;
+  if (!base || !x || !down || !up || !scaling || !ranks || !index || !out || !workspace) return VFLASH_EINVAL;
+  if (ldb < p.n || ldx < k || ldo < p.n || ldb % 8 || ldx % 8 || ldo % 8 || (out == base && ldo != ldb)) return VFLASH_EINVAL;
+  for (const void* q : {base, x, down, up, static_cast<const void*>(out), static_cast<const void*>(workspace)})
+    if (!aligned(q, 16)) return VFLASH_EINVAL;
+  if (!aligned(scaling, 4) || !aligned(ranks, 4) || !aligned(index, 8)) return VFLASH_EINVAL;
+  if (workspace_bytes < vfa::request_workspace(p)) return VFLASH_EINVAL;
+  p.x = static_cast<const uint16_t*>(x);
+  p.base = static_cast<const uint16_t*>(base);
+  p.down = static_cast<const uint16_t*>(down);
+  p.up = static_cast<const uint16_t*>(up);
+  p.out = static_cast<uint16_t*>(out);
+  p.ldx = ldx;
+  p.ldb = ldb;
+  p.ldo = ldo;
+  p.scaling = scaling;
+  p.ranks = ranks;
+  p.index = index;
+  return status(vfa::launch_request_adapters(p, f16 != 0, workspace, static_cast<hipStream_t>(stream)));
 }
 
 }  // extern "C"

@@ -727,3 +727,110 @@ def packed_attention(q, k, v, q_offsets, k_offsets, k_lengths, causal, scale):
          ptr(q_offsets), ptr(k_offsets), ptr(k_lengths), batch, int(causal), scale, ptr(out), out.stride(0),
          out.stride(1), ptr(workspace), size, stream_of(device))
     return out
+
+
+def _rotary_arguments(rotary, positions):
+    if rotary is None:
+        return None, None, 0, 0, 1.0, None, 1
+    return (ptr(rotary.phases), ptr(rotary.axis), rotary.pairs, int(rotary.interleaved), rotary.magnitude, ptr(positions),
+            rotary.axes)
+
+
+def rotate(q, k, positions, rotary):
+    """Rotary positions of q and k (operands as ``rotary.rotate`` checks them)."""
+    device = require_device(q, k, positions, rotary.phases, rotary.axis)
+    q = _attention_rows(q)
+    k = None if k is None else _attention_rows(k)
+    positions = positions.resolve_neg().contiguous()
+    tokens, heads, dim = q.shape
+    q_out = torch.empty((tokens, heads, dim), device=device, dtype=q.dtype)
+    k_out = None if k is None else torch.empty(k.shape, device=device, dtype=q.dtype)
+    if tokens:
+        call("vflash_rotate", ptr(q), q.stride(0), q.stride(1), ptr(k), k.stride(0) if k is not None else 0,
+             k.stride(1) if k is not None else 0, int(q.dtype == torch.float16), tokens, heads,
+             k.shape[1] if k is not None else 0, dim, *_rotary_arguments(rotary, positions), ptr(q_out), ptr(k_out),
+             stream_of(device))
+    return q_out, k_out
+
+
+def paged_append(cache, q, k, v, table, lengths, q_offsets, rotary, positions):
+    """New keys and values into a paged cache (operands as ``paged.paged_append`` checks them)."""
+    axes = (rotary.phases, rotary.axis) if rotary is not None else ()
+    device = require_device(k, v, q, cache.values, table, lengths, q_offsets, positions, *axes)
+    k, v = _attention_rows(k), _attention_rows(v)
+    q = None if q is None else _attention_rows(q)
+    positions = None if positions is None else positions.resolve_neg().contiguous()
+    tokens, key_heads, dim = k.shape
+    q_out = None if q is None else torch.empty(q.shape, device=device, dtype=q.dtype)
+    values = cache.values
+    if tokens and values.shape[0]:
+        call("vflash_paged_append", ptr(q), q.stride(0) if q is not None else 0, q.stride(1) if q is not None else 0,
+             ptr(k), k.stride(0), k.stride(1), ptr(v), v.stride(0), v.stride(1), int(k.dtype == torch.float16), tokens,
+             q.shape[1] if q is not None else 0, key_heads, dim, ptr(q_offsets), *_rotary_arguments(rotary, positions),
+             ptr(values), ptr(cache.scales), values.shape[0], values.shape[3], ptr(table), table.shape[1], ptr(lengths),
+             table.shape[0], ptr(q_out), stream_of(device))
+    elif q_out is not None:
+        q_out.zero_()  # a cache without pages has no place
+    return q_out
+
+
+def paged_attention(q, cache, table, lengths, q_offsets, scale):
+    """softmax(scale q k^T) v over a paged cache (operands as ``paged.paged_attention`` checks them)."""
+    device = require_device(q, cache.values, table, lengths, q_offsets)
+    q = _attention_rows(q)
+    tokens, heads, dim = q.shape
+    out = torch.empty((tokens, heads, dim), device=device, dtype=q.dtype)
+    if not tokens:
+        return out
+    pages, _, key_heads, page, _ = cache.values.shape
+    batch, width = table.shape
+    size = _lib.library().vflash_paged_attention_workspace(tokens, batch, heads, key_heads, dim, page, width)
+    if size < 0:
+        raise ValueError("paged attention: more rows than a call takes")
+    workspace = torch.empty(size, device=device, dtype=torch.uint8) if size else None
+    call("vflash_paged_attention", ptr(q), q.stride(0), q.stride(1), int(q.dtype == torch.float16), tokens, heads,
+         key_heads, dim, ptr(q_offsets), ptr(cache.values), ptr(cache.scales), pages, page, ptr(table), width,
+         ptr(lengths), batch, scale, ptr(out), out.stride(0), out.stride(1), ptr(workspace), size, stream_of(device))
+    return out
+
+
+def request_adapters(base, x, adapters, index, inplace):
+    """base plus each row's adapter (operands as ``adapters.add_request_adapters`` checks them)."""
+    device = require_device(base, x, adapters.down, index)
+    k, n = adapters.down.shape[2], adapters.up.shape[1]
+    rows = base.shape[:-1].numel()
+    matrix, index = x.resolve_neg().reshape(rows, k), index.resolve_neg()
+    if matrix.stride(1) != 1 or matrix.stride(0) % 8 or matrix.data_ptr() % 16 or matrix.stride(0) < k:
+        matrix = matrix.clone(memory_format=torch.contiguous_format)
+
+    def taken(t):
+        return t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0 and t.stride(0) >= n
+
+    if inplace:
+        try:
+            source = base.view(rows, n)
+        except RuntimeError:
+            source = None
+        if base.is_neg() or source is None or (rows and not taken(source)):
+            raise ValueError("adding in place takes rows that are 16-byte runs apart from each other")
+        out = base
+        rows_out = source
+    else:
+        source = base.resolve_neg().reshape(rows, n)
+        if rows and not taken(source):
+            source = source.clone(memory_format=torch.contiguous_format)
+        out = torch.empty(base.shape, device=device, dtype=base.dtype)
+        rows_out = out.view(rows, n)
+    if not rows:
+        return out
+    widths, branches = adapters.c_widths, len(adapters.widths)
+    count, _, width = adapters.up.shape
+    size = _lib.library().vflash_request_adapters_workspace(rows, k, widths, branches, count, width)
+    if size < 0:
+        raise ValueError("request adapters: more rows than a call takes")
+    workspace = torch.empty(size, device=device, dtype=torch.uint8)
+    call("vflash_request_adapters", ptr(source), source.stride(0), ptr(matrix), matrix.stride(0),
+         int(x.dtype == torch.float16), rows, k, widths, branches, ptr(adapters.down), ptr(adapters.up),
+         ptr(adapters.scaling), ptr(adapters.ranks), count, width, ptr(index), ptr(rows_out), rows_out.stride(0),
+         ptr(workspace), size, stream_of(device))
+    return out
