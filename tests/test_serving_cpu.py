@@ -319,7 +319,7 @@ def test_workspaces():
     assert lib.vflash_paged_attention_workspace(4, 4, 32, 8, 128, 17, 49) == _lib.VFLASH_EINVAL
     widths = (ctypes.c_int64 * 1)(64)
     small = lib.vflash_request_adapters_workspace(64, 64, widths, 1, 5, 16)
-    assert small == 64 * 16 * 4  # one part of t
+    assert small == 64 * 16 * 4 + 10 * (4 + 16) * 4  # one part of t, and at most ten items
     assert lib.vflash_request_adapters_workspace(65, 64, widths, 1, 5, 16) > 65 * 16 * 4
     assert lib.vflash_request_adapters_workspace(65, 60, widths, 1, 5, 16) == _lib.VFLASH_EINVAL
 

@@ -18,11 +18,12 @@ struct RequestAdapterParams {
   int64_t rows, k, n;
   int adapters, branches, width;
   int ends[RA_BRANCHES];   // columns at which the branches end
-  int tiles[RA_BRANCHES];  // of 64 columns, up to and with each branch
+  int groups[RA_BRANCHES];  // of columns, a workgroup's each, up to and with each branch
   int splits, steps;       // of K; 32-wide steps of a split
   int items, item_rows;    // at most; rows of one
   float* t;                // [splits][rows][branches * width]
-  int32_t *order, *list;   // rows by adapter; [items][3]: adapter, first place in order, count
+  int32_t *order, *list;   // [items][item_rows] rows; [items][4]: adapter, count, rank
+  int32_t* before;         // [rows] rows of the same adapter before
 };
 
 }  // namespace vfa

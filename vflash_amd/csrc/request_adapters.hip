@@ -6,9 +6,11 @@
 // adapter in use is read about once.  Two products on the matrix cores, v_mfma_f32_16x16x32 with the
 // adapter's rows as operand A and the items' rows as operand B:
 //   request_down  t = x A^T, binary32.  K is split over the waves of a workgroup and, where there are few items, over
-//                 workgroups, whose sums are added in their order by the reader: no atomics.
-//   request_up    t times scaling, as two 16-bit numbers (high and low part: 16 bits of t or more enter the product),
-//                 times B; base is added and the sum rounded once.
+//                 workgroups.
+//   request_up    adds the splits up in their order, keeps t of its item in LDS as two bf16, a high and a low part (16
+//                 bits of it or more, in binary32's range), and multiplies by B.  Binary16 factors of B are two bf16
+//                 as well, exactly.  scaling, base and one rounding follow.
+// Nothing is added by atomics: a row's result does not depend on its company.
 // Bound by launches for a few rows, by the adapters' bytes for a decoding batch, and by base and out for prompts.
 #include "request_adapters.h"
 
@@ -26,54 +28,49 @@ constexpr int RD_WAVES = 8;  // of request_down: parts of K
 constexpr int RU_WAVES = 4;  // of request_up: column tiles
 
 struct RequestItem {
-  int adapter, count;  // adapter -1: none; count 0: no such item
-  int row;             // this lane's row (by lane % 16, of the first block)
+  int adapter, count, rank;  // adapter -1: none; count 0: no such item
 };
+
+__device__ __forceinline__ int rank_of(const RequestAdapterParams& p, int adapter) {
+  return max(0, min(p.ranks[adapter], p.width));
+}
 
 // Item `index` of at most 64 rows, found by the wave: the adapters by their first row, their rows in order.
 __device__ __forceinline__ RequestItem request_find(const RequestAdapterParams& p, int index, int* rows) {
   const int lane = (int)threadIdx.x & 63;
-  int mine = -2;  // no row
+  int mine = -2, rank = 0;  // no row
   if (lane < p.rows) {
     const int64_t i = p.index[lane];
     mine = (uint64_t)i < (uint64_t)p.adapters ? (int)i : -1;
+    if (mine >= 0) rank = rank_of(p, mine);
   }
   uint64_t left = __builtin_amdgcn_ballot_w64(mine != -2);
-  RequestItem it{-1, 0, 0};
   while (left) {
-    const int a = __builtin_amdgcn_readlane(mine, __builtin_ctzll(left));
+    const int first = __builtin_ctzll(left), a = __builtin_amdgcn_readlane(mine, first);
     const uint64_t same = __builtin_amdgcn_ballot_w64(mine == a);
     const int count = __popcll(same), items = (count + p.item_rows - 1) / p.item_rows;
     if (index < items) {
       // Lane l of the adapter's rows goes to its place among them.
       const int place = __popcll(same & ((uint64_t(1) << lane) - 1)) - index * p.item_rows;
       if (mine == a && place >= 0 && place < p.item_rows) rows[place] = lane;
-      it.adapter = a;
-      it.count = min(p.item_rows, count - index * p.item_rows);
-      return it;
+      return RequestItem{a, min(p.item_rows, count - index * p.item_rows), __builtin_amdgcn_readlane(rank, first)};
     }
     index -= items;
     left &= ~same;
   }
-  return it;
+  return RequestItem{-1, 0, 0};
 }
 
-// Item `index`, its rows in `rows` (LDS of this workgroup).
-__device__ __forceinline__ RequestItem request_item(const RequestAdapterParams& p, int index, int* rows) {
-  RequestItem it;
-  if (!p.order) {
-    // Every wave finds the same and writes the same.
-    it = request_find(p, index, rows);
-  } else {
-    it.adapter = p.list[3 * index];
-    const int first = p.list[3 * index + 1];
-    it.count = p.list[3 * index + 2];
-    if ((int)threadIdx.x < it.count) rows[threadIdx.x] = p.order[first + threadIdx.x];
-  }
-  it.adapter = __builtin_amdgcn_readfirstlane(it.adapter);
-  it.count = __builtin_amdgcn_readfirstlane(it.count);
-  __syncthreads();
-  return it;
+// Item `index` as request_groups or request_down left it, its rows in `rows` (LDS of this workgroup).
+__device__ __forceinline__ RequestItem request_listed(const RequestAdapterParams& p, int index, int* rows) {
+  const v4i item = *reinterpret_cast<const v4i*>(p.list + 4 * index);
+  if ((int)threadIdx.x < p.item_rows) rows[threadIdx.x] = p.order[(int64_t)index * p.item_rows + threadIdx.x];
+  return RequestItem{item[0], item[1], item[2]};
+}
+
+__device__ __forceinline__ RequestItem uniform(const RequestItem& it) {
+  return RequestItem{__builtin_amdgcn_readfirstlane(it.adapter), __builtin_amdgcn_readfirstlane(it.count),
+                     __builtin_amdgcn_readfirstlane(it.rank)};
 }
 
 template <bool F16>
@@ -86,209 +83,285 @@ __device__ __forceinline__ int pack(float a, float b) {
   if constexpr (F16) return __builtin_bit_cast(int, v2hf{(_Float16)a, (_Float16)b});
   else return __builtin_bit_cast(int, v2bf{(__bf16)a, (__bf16)b});
 }
+// Two values as bf16 and what that leaves of them, as bf16.  An infinity leaves nothing.
+__device__ __forceinline__ void parts(float a, float b, int& high, int& low) {
+  high = pack<false>(a, b);
+  const float x = bf16_lo((uint32_t)high), y = bf16_hi((uint32_t)high);
+  low = pack<false>(fabsf(x) < __builtin_inff() ? a - x : 0.0f, fabsf(y) < __builtin_inff() ? b - y : 0.0f);
+}
+
+// Eight bf16, zeros in the place of those that are not finite.
+__device__ __forceinline__ v4i finite(v4i w) {
+  static_for<4>([&](auto i) {
+    const uint32_t u = (uint32_t)w[(int)i];
+    w[(int)i] = (int)(((u & 0x7f80u) == 0x7f80u ? 0 : u & 0xffffu) | ((u & 0x7f800000u) == 0x7f800000u ? 0 : u & 0xffff0000u));
+  });
+  return w;
+}
+
+__device__ __forceinline__ int wave_sum_before(int v, int lane) {  // inclusive
+  for (int o = 1; o < 64; o <<= 1) {
+    const int u = __shfl_up(v, o, 64);
+    if (lane >= o) v += u;
+  }
+  return v;
+}
 
 }  // namespace
 
-// Rows by adapter, those with none last, and the items.  One workgroup: a histogram, its prefix sums, and the rows
-// to their places (within an adapter in any order: no row's result depends on it).
+// The items of more than 64 rows, by adapter, those without one last.  One workgroup: a histogram, its prefix sums,
+// and the rows to their places (within an adapter in any order: no row's result depends on it).
 __global__ void __launch_bounds__(1024) request_groups(const RequestAdapterParams p) {
-  extern __shared__ int counts[];  // [adapters + 1] rows, then places; [1024] sums
-  __shared__ int row_sums[1024], item_sums[1024];
-  const int bins = p.adapters + 1, t = (int)threadIdx.x;
+  extern __shared__ int counts[];  // [adapters + 1]: rows, then the first place in p.order
+  __shared__ int sums[17];
+  const int bins = p.adapters + 1, t = (int)threadIdx.x, lane = t & 63, wave = t >> 6;
   for (int b = t; b < bins; b += 1024) counts[b] = 0;
   __syncthreads();
   auto bin_of = [&](int64_t m) {
+    if (m >= p.rows) return -1;
     const int64_t i = p.index[m];
     return (uint64_t)i < (uint64_t)p.adapters ? (int)i : p.adapters;
   };
-  for (int64_t m = t; m < p.rows; m += 1024) atomicAdd(&counts[bin_of(m)], 1);
+  // Adds one to a bin for each lane, and gives each the count before it.  Lanes of one bin (runs) go together, for the first
+  // few bins of a wave: the same word is added to once at a time.
+  auto add = [&](int bin) {
+    int before = 0;
+    uint64_t left = __builtin_amdgcn_ballot_w64(bin >= 0);
+    for (int i = 0; i < 6 && left; ++i) {
+      const int first = __builtin_ctzll(left), b = __builtin_amdgcn_readlane(bin, first);
+      const uint64_t same = __builtin_amdgcn_ballot_w64(bin == b);
+      int old = 0;
+      if (lane == first) old = atomicAdd(&counts[b], __popcll(same));
+      old = __builtin_amdgcn_readlane(old, first);
+      if (bin == b) before = old + __popcll(same & ((uint64_t(1) << lane) - 1));
+      left &= ~same;
+    }
+    if (left >> lane & 1) before = atomicAdd(&counts[bin], 1);
+    return before;
+  };
+  // The first rows of each thread stay in registers.
+  constexpr int KEPT = 8;
+  int bins_of[KEPT], before_of[KEPT];
+  static_for<KEPT>([&](auto i) { bins_of[i] = bin_of(t + 1024 * i); });
+  static_for<KEPT>([&](auto i) {
+    if (1024 * i < p.rows) before_of[i] = add(bins_of[i]);
+  });
+  const int64_t end = (p.rows + 1023) / 1024 * 1024;
+  for (int64_t m = t + 1024 * KEPT; m < end; m += 1024) {
+    const int before = add(bin_of(m));
+    if (m < p.rows) p.before[m] = before;
+  }
   __syncthreads();
   // Thread t's bins are next to each other.
   const int per = (bins + 1023) / 1024, b0 = min(t * per, bins), b1 = min(b0 + per, bins);
   auto items_of = [&](int c) { return (c + p.item_rows - 1) / p.item_rows; };
-  int rows = 0, items = 0;
-  for (int b = b0; b < b1; ++b) {
-    rows += counts[b];
-    items += items_of(counts[b]);
-  }
-  row_sums[t] = rows;
-  item_sums[t] = items;
+  int items = 0;
+  for (int b = b0; b < b1; ++b) items += items_of(counts[b]);
+  int item = wave_sum_before(items, lane);
+  if (lane == 63) sums[wave] = item;
   __syncthreads();
-  for (int o = 1; o < 1024; o <<= 1) {
-    const int r = t >= o ? row_sums[t - o] : 0, i = t >= o ? item_sums[t - o] : 0;
-    __syncthreads();
-    row_sums[t] += r;
-    item_sums[t] += i;
-    __syncthreads();
+  int all = 0;
+  for (int w = 0; w < 16; ++w) {
+    if (w < wave) item += sums[w];
+    all += sums[w];
   }
-  int row = row_sums[t] - rows, item = item_sums[t] - items;
+  item -= items;
   for (int b = b0; b < b1; ++b) {
-    const int c = counts[b];
-    for (int first = 0; first < c; first += p.item_rows, ++item) {
-      p.list[3 * item] = b < p.adapters ? b : -1;
-      p.list[3 * item + 1] = row + first;
-      p.list[3 * item + 2] = min(p.item_rows, c - first);
-    }
-    counts[b] = row;
-    row += c;
+    const int c = counts[b], rank = b < p.adapters && c ? rank_of(p, b) : 0;
+    counts[b] = item * p.item_rows;
+    for (int first = 0; first < c; first += p.item_rows, ++item)
+      *reinterpret_cast<v4i*>(p.list + 4 * item) = v4i{b < p.adapters ? b : -1, min(p.item_rows, c - first), rank, 0};
   }
-  for (int i = item_sums[1023] + t; i < p.items; i += 1024) p.list[3 * i + 2] = 0;
+  for (int i = all + t; i < p.items; i += 1024) *reinterpret_cast<v4i*>(p.list + 4 * i) = v4i{};
   __syncthreads();
-  for (int64_t m = t; m < p.rows; m += 1024) p.order[atomicAdd(&counts[bin_of(m)], 1)] = (int)m;
+  static_for<KEPT>([&](auto i) {
+    if (bins_of[i] >= 0) p.order[counts[bins_of[i]] + before_of[i]] = t + 1024 * i;
+  });
+  for (int64_t m = t + 1024 * KEPT; m < p.rows; m += 1024) p.order[counts[bin_of(m)] + p.before[m]] = (int)m;
 }
 
-// t of one item for RK blocks of 16 adapter rows and one split of K.
-template <bool F16, int RB, int RK>
+// t of 16 rows of an item for RK blocks of 16 adapter rows and one split of K.
+template <bool F16, int RK>
 __global__ void __launch_bounds__(64 * RD_WAVES) request_down(const RequestAdapterParams p) {
-  __shared__ int rows[RB * 16];
-  __shared__ v4f part[RD_WAVES][RB * RK][64];
-  const RequestItem it = request_item(p, (int)blockIdx.x, rows);
-  if (it.count == 0 || it.adapter < 0) return;
+  __shared__ int rows[64];
+  __shared__ v4f part[RD_WAVES][RK][64];
+  const bool grouped = p.rows > RA_WAVE_ROWS;
+  const int per_item = p.item_rows / 16, item = (int)blockIdx.x / per_item, first = ((int)blockIdx.x - item * per_item) * 16;
+  // Ungrouped, every wave finds the same and writes the same.
+  const RequestItem it = uniform(grouped ? request_listed(p, item, rows) : request_find(p, item, rows));
+  __syncthreads();
+  if (!grouped && blockIdx.y == 0 && blockIdx.z == 0) {  // for request_up
+    if (threadIdx.x == 0) *reinterpret_cast<v4i*>(p.list + 4 * item) = v4i{it.adapter, it.count, it.rank, 0};
+    if ((int)threadIdx.x < it.count) p.order[item * p.item_rows + threadIdx.x] = rows[threadIdx.x];
+  }
+  if (first >= it.count || it.adapter < 0) return;
   const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int fr = lane & 15, fg = lane >> 4;
   const int all = p.branches * p.width, r0 = (int)blockIdx.z * RK * 16;
-  const int rank = p.ranks[it.adapter];
 
   // Blocks of adapter rows that hold some of the rank.
   bool used[RK], any = false;
-  const uint16_t *xr[RB], *ar[RK];
+  const uint16_t* ar[RK];
   static_for<RK>([&](auto j) {
     const int r = r0 + j * 16;
-    used[j] = r < all && r % p.width < rank;
+    used[j] = r < all && r % p.width < it.rank;
     any = any || used[j];
     ar[j] = p.down + ((int64_t)it.adapter * all + min(r + fr, all - 1)) * p.k;
   });
   if (!any) return;
-  static_for<RB>([&](auto i) { xr[i] = p.x + (int64_t)rows[min((int)i * 16 + fr, it.count - 1)] * p.ldx; });
+  const int row = rows[min(first + fr, it.count - 1)];
+  const uint16_t* xr = p.x + (int64_t)row * p.ldx;
   const int steps = (int)((p.k + 31) / 32);
   const int from = (int)blockIdx.y * p.steps, to = min(from + p.steps, steps);
   const int s0 = from + max(0, to - from) * wave / RD_WAVES, s1 = from + max(0, to - from) * (wave + 1) / RD_WAVES;
 
-  constexpr int AHEAD = RB * RK >= 4 ? 2 : 4;
-  v4f acc[RB][RK];
-  static_for<RB>([&](auto i) { static_for<RK>([&](auto j) { acc[i][j] = v4f{}; }); });
+  constexpr int AHEAD = 8;  // steps whose loads are in flight together
+  v4f acc[RK];
+  static_for<RK>([&](auto j) { acc[j] = v4f{}; });
   for (int s = s0; s < s1; s += AHEAD) {
-    v4i xv[AHEAD][RB], av[AHEAD][RK];
+    v4i xv[AHEAD], av[AHEAD][RK];
     static_for<AHEAD>([&](auto a) {
       const int64_t at = (int64_t)(s + a) * 32 + fg * 8;
       const bool ok = s + a < s1 && at < p.k;
-      static_for<RB>([&](auto i) { xv[a][i] = ok ? *reinterpret_cast<const v4i*>(xr[i] + at) : v4i{}; });
+      xv[a] = ok ? *reinterpret_cast<const v4i*>(xr + at) : v4i{};
       static_for<RK>([&](auto j) { av[a][j] = ok && used[j] ? *reinterpret_cast<const v4i*>(ar[j] + at) : v4i{}; });
     });
     static_for<AHEAD>([&](auto a) {
-      static_for<RB>([&](auto i) {
-        static_for<RK>([&](auto j) { acc[i][j] = mfma16<F16>(av[a][j], xv[a][i], acc[i][j]); });
-      });
+      static_for<RK>([&](auto j) { acc[j] = mfma16<F16>(av[a][j], xv[a], acc[j]); });
     });
   }
-  static_for<RB>([&](auto i) { static_for<RK>([&](auto j) { part[wave][i * RK + j][lane] = acc[i][j]; }); });
+  static_for<RK>([&](auto j) { part[wave][j][lane] = acc[j]; });
   __syncthreads();
-  // Lane (fr, fg) of block (i, j): t of row i * 16 + fr, ranks r0 + j * 16 + 4 fg + 0 .. 3.
-  for (int b = wave; b < RB * RK; b += RD_WAVES) {
-    const int i = b / RK, j = b % RK, r = r0 + j * 16;
-    if (r >= all || i * 16 + fr >= it.count) continue;
-    v4f sum = part[0][b][lane];
-    static_for<RD_WAVES - 1>([&](auto w) { sum += part[w + 1][b][lane]; });
-    *reinterpret_cast<v4f*>(p.t + ((int64_t)blockIdx.y * p.rows + rows[i * 16 + fr]) * all + r + 4 * fg) = sum;
+  // Lane (fr, fg) of block j: t of row fr, ranks r0 + j * 16 + 4 fg + 0 .. 3.
+  for (int j = wave; j < RK; j += RD_WAVES) {
+    const int r = r0 + j * 16;
+    if (r >= all || first + fr >= it.count) continue;
+    v4f sum = part[0][j][lane];
+    static_for<RD_WAVES - 1>([&](auto w) { sum += part[w + 1][j][lane]; });
+    *reinterpret_cast<v4f*>(p.t + ((int64_t)blockIdx.y * p.rows + row) * all + r + 4 * fg) = sum;
   }
 }
 
-// Tiles of 64 columns of one item.  MFMA block j of a tile holds the columns 16 g + 4 j + e in its rows 4 g + e, so that a
-// lane ends with 16 columns of one row next to each other.
-template <bool F16, int RB>
+// Tiles of 64 columns of one branch and item, ranks in NC runs of 32.  MFMA block j of a tile holds the columns
+// 32 (j / 2) + 8 g + 4 (j % 2) + e in its rows 4 g + e, so that a lane ends with two runs of eight columns of one row, and
+// the four lanes of a row store 64 bytes at once.
+template <bool F16, int NC>
 __global__ void __launch_bounds__(64 * RU_WAVES) request_up(const RequestAdapterParams p, int tiles_per_wave) {
-  __shared__ int rows[RB * 16];
-  const RequestItem it = request_item(p, (int)blockIdx.x, rows);
+  constexpr int PITCH = 64 * NC + 8;  // of a row in LDS: high parts, low parts, and eight against bank conflicts
+  __shared__ int rows[64];
+  __shared__ __attribute__((aligned(16))) uint16_t low_rank[64 * PITCH];
+  const RequestItem it = uniform(request_listed(p, (int)blockIdx.x, rows));
+  __syncthreads();
   if (it.count == 0) return;
   const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int fr = lane & 15, fg = lane >> 4;
-  const int total = p.tiles[p.branches - 1], all = p.branches * p.width;
-  const int rank = it.adapter < 0 ? 0 : p.ranks[it.adapter];
-  const int begin = ((int)blockIdx.y * RU_WAVES + wave) * tiles_per_wave, end = min(begin + tiles_per_wave, total);
-  for (int tile = begin; tile < end; ++tile) {
-    int branch = 0;
-    while (branch + 1 < p.branches && tile >= p.tiles[branch]) ++branch;
-    const int n0 = (branch ? p.ends[branch - 1] : 0) + (tile - (branch ? p.tiles[branch - 1] : 0)) * 64;
-    const int stop = p.ends[branch], n = n0 + 16 * fg;  // this lane's columns: n .. n + 15, up to stop
-    v4f acc[RB][4];
-    static_for<RB>([&](auto i) { static_for<4>([&](auto j) { acc[i][j] = v4f{}; }); });
-    // Ranks r .. r + 7 of row block i, scaled; zeros past the rank.
-    const float scaling = it.adapter < 0 ? 0.0f : p.scaling[it.adapter * p.branches + branch];
-    auto low = [&](int i, int r, float (&v)[8]) {
-      const float* src = p.t + (int64_t)rows[min(i * 16 + fr, it.count - 1)] * all + branch * p.width + min(r, p.width - 8);
+  int branch = 0, group = (int)blockIdx.y;
+  while (branch + 1 < p.branches && group >= p.groups[branch]) ++branch;
+  if (branch) group -= p.groups[branch - 1];
+  const int first_col = branch ? p.ends[branch - 1] : 0, stop = p.ends[branch];
+  const float scaling = it.adapter < 0 ? 0.0f : p.scaling[it.adapter * p.branches + branch];
+
+  // t, eight ranks a thread; zeros past the rank.
+  if (it.rank > 0) {
+    const int all = p.branches * p.width;
+    for (int e = (int)threadIdx.x; e < it.count * 4 * NC; e += 64 * RU_WAVES) {
+      const int row = e / (4 * NC), r = e % (4 * NC) * 8;
       v4f x[2] = {v4f{}, v4f{}};
-      for (int s = 0; s < p.splits; ++s) {
-        x[0] += *reinterpret_cast<const v4f*>(src);
-        x[1] += *reinterpret_cast<const v4f*>(src + 4);
-        src += p.rows * all;
+      if (r < it.rank) {
+        const float* src = p.t + (int64_t)rows[row] * all + branch * p.width + r;
+#pragma unroll 4
+        for (int s = 0; s < p.splits; ++s, src += p.rows * all) {
+          x[0] += *reinterpret_cast<const v4f*>(src);
+          x[1] += *reinterpret_cast<const v4f*>(src + 4);
+        }
       }
-      static_for<8>([&](auto e) { v[e] = r + e < rank ? x[e / 4][(int)(e % 4)] * scaling : 0.0f; });
-    };
-    // binary16 has not t's range: a row enters with its largest value in [1, 2).
-    int shift[RB];
-    static_for<RB>([&](auto i) {
-      shift[i] = 0;
-      if (!F16 || i * 16 >= it.count) return;
-      float top = 0;
-      for (int c0 = 0; c0 < rank; c0 += 32) {
-        float v[8];
-        low(i, c0 + 8 * fg, v);
-        static_for<8>([&](auto e) { top = nan_max(top, fabsf(v[e])); });
-      }
-      top = nan_max(top, __shfl_xor(top, 16, 64));
-      top = nan_max(top, __shfl_xor(top, 32, 64));
-      const int exponent = (int)(__float_as_uint(top) >> 23);
-      if (exponent < 255) shift[i] = exponent - 127;
-    });
-    for (int c0 = 0; c0 < rank; c0 += 32) {
-      const int r = c0 + 8 * fg;
-      v4i b[4];
-      static_for<4>([&](auto j) {
-        const int col = n0 + 16 * (fr >> 2) + 4 * j + (fr & 3);
-        b[j] = r < p.width && col < stop
-                   ? *reinterpret_cast<const v4i*>(p.up + ((int64_t)it.adapter * p.n + col) * p.width + r) : v4i{};
+      v4i high, low;
+      static_for<4>([&](auto i) {
+        int h, l;
+        parts(r + 2 * i < it.rank ? x[i / 2][2 * (i % 2)] : 0.0f, r + 2 * i + 1 < it.rank ? x[i / 2][2 * (i % 2) + 1] : 0.0f, h, l);
+        high[(int)i] = h;
+        low[(int)i] = l;
       });
-      static_for<RB>([&](auto i) {
-        if (i * 16 >= it.count) return;
-        float v[8];
-        low(i, r, v);
-        v4i hi, lo;
-        static_for<4>([&](auto e) {
-          if constexpr (F16) static_for<2>([&](auto h) { v[2 * e + h] = __builtin_ldexpf(v[2 * e + h], -shift[i]); });
-          hi[(int)e] = pack<F16>(v[2 * e], v[2 * e + 1]);
-          float d[2];
-          static_for<2>([&](auto h) {
-            const float w = widen<F16>((uint32_t)hi[(int)e], h);
-            d[h] = fabsf(w) < __builtin_inff() ? v[2 * e + h] - w : 0.0f;
-          });
-          lo[(int)e] = pack<F16>(d[0], d[1]);
-        });
-        static_for<4>([&](auto j) {
-          acc[i][j] = mfma16<F16>(b[j], hi, acc[i][j]);
-          acc[i][j] = mfma16<F16>(b[j], lo, acc[i][j]);
-        });
-      });
+      *reinterpret_cast<v4i*>(low_rank + row * PITCH + r) = high;
+      *reinterpret_cast<v4i*>(low_rank + row * PITCH + 32 * NC + r) = low;
     }
-    if constexpr (F16)
-      static_for<RB>([&](auto i) {
-        static_for<4>([&](auto j) { static_for<4>([&](auto e) { acc[i][j][(int)e] = __builtin_ldexpf(acc[i][j][(int)e], shift[i]); }); });
+  }
+  __syncthreads();
+
+  // The waves' tiles lie side by side.
+  for (int k = 0; k < tiles_per_wave; ++k) {
+    const int n0 = first_col + ((group * tiles_per_wave + k) * RU_WAVES + wave) * 64;
+    if (n0 >= stop) return;
+    const int n = n0 + 8 * fg;  // this lane's columns: n .. n + 7 and 32 further, up to stop
+    v4i b[NC][4], rest[NC][4];
+    static_for<NC>([&](auto c) {
+      const int r = c * 32 + 8 * fg;
+      static_for<4>([&](auto j) {
+        const int col = n0 + 32 * (j / 2) + 8 * (fr >> 2) + 4 * (j % 2) + (fr & 3);
+        b[c][j] = r < it.rank && col < stop
+                      ? *reinterpret_cast<const v4i*>(p.up + ((int64_t)it.adapter * p.n + col) * p.width + r) : v4i{};
       });
-    static_for<RB>([&](auto i) {
-      if (i * 16 + fr >= it.count) return;
-      const int64_t row = rows[i * 16 + fr];
+    });
+    int64_t row[4];
+    v4i base[4][2];
+    static_for<4>([&](auto i) {
+      if (16 * i >= it.count) return;
+      row[i] = rows[min(16 * (int)i + fr, it.count - 1)];
       static_for<2>([&](auto h) {
-        if (n + 8 * h >= stop) return;
-        const v4i base = *reinterpret_cast<const v4i*>(p.base + row * p.ldb + n + 8 * h);
+        base[i][h] = n + 32 * h < stop ? *reinterpret_cast<const v4i*>(p.base + row[i] * p.ldb + n + 32 * h) : v4i{};
+      });
+    });
+    if constexpr (F16)
+      static_for<NC>([&](auto c) {
+        static_for<4>([&](auto j) {
+          static_for<4>([&](auto e) {
+            const uint32_t w = (uint32_t)b[c][j][(int)e];
+            int high, low;
+            parts(widen<true>(w, 0), widen<true>(w, 1), high, low);
+            b[c][j][(int)e] = high;
+            rest[c][j][(int)e] = low;
+          });
+        });
+      });
+    static_for<4>([&](auto i) {
+      if (16 * i >= it.count) return;
+      v4f acc[4];
+      static_for<4>([&](auto j) { acc[j] = v4f{}; });
+      const uint16_t* src = low_rank + min(16 * (int)i + fr, it.count - 1) * PITCH + 8 * fg;
+      static_for<NC>([&](auto c) {
+        if (c * 32 >= it.rank) return;
+        const v4i high = *reinterpret_cast<const v4i*>(src + c * 32), low = *reinterpret_cast<const v4i*>(src + 32 * NC + c * 32);
+        static_for<4>([&](auto j) {
+          acc[j] = mfma16<false>(b[c][j], high, acc[j]);
+          acc[j] = mfma16<false>(b[c][j], low, acc[j]);
+        });
+        if constexpr (F16) {
+          const v4i near = finite(high);  // an infinity is in the first product
+          static_for<4>([&](auto j) { acc[j] = mfma16<false>(rest[c][j], near, acc[j]); });
+        }
+      });
+      if (16 * i + fr >= it.count) return;
+      static_for<2>([&](auto h) {
+        if (n + 32 * h >= stop) return;
         v4i o;
         static_for<4>([&](auto e) {
           constexpr int at = 8 * h + 2 * e;
-          const uint32_t w = (uint32_t)base[(int)e];
-          o[(int)e] = pack<F16>(widen<F16>(w, 0) + acc[i][at / 4][at % 4], widen<F16>(w, 1) + acc[i][at / 4][at % 4 + 1]);
+          const uint32_t w = (uint32_t)base[i][h][(int)e];
+          o[(int)e] = pack<F16>(__builtin_fmaf(acc[at / 4][at % 4], scaling, widen<F16>(w, 0)),
+                                __builtin_fmaf(acc[at / 4][at % 4 + 1], scaling, widen<F16>(w, 1)));
         });
-        *reinterpret_cast<v4i*>(p.out + row * p.ldo + n + 8 * h) = rank > 0 ? o : base;
+        *reinterpret_cast<v4i*>(p.out + row[i] * p.ldo + n + 32 * h) = it.rank > 0 ? o : base[i][h];
       });
     });
   }
+}
+
+namespace {
+
+// Adapter rows that a workgroup of request_down takes.
+int request_ranks(const RequestAdapterParams& p) {
+  const int all = p.branches * p.width;
+  return all >= 64 ? 64 : all >= 32 ? 32 : 16;
 }
 
 // The launch of a call, from its sizes alone.
@@ -298,49 +371,51 @@ void request_plan(RequestAdapterParams& p) {
   const int64_t groups = p.rows < p.adapters + 1 ? p.rows : p.adapters + 1;
   p.items = (int)(p.rows / p.item_rows + groups);
   if (p.items > p.rows) p.items = (int)p.rows;
-  const int64_t steps = (p.k + 31) / 32, blocks = (p.branches * p.width + 63) / 64;
+  const int64_t steps = (p.k + 31) / 32, blocks = (p.branches * p.width + request_ranks(p) - 1) / request_ranks(p);
   // About one workgroup a CU, of at least two steps a wave.
-  int64_t splits = cus / (p.items * blocks);
+  int64_t splits = cus / (p.items * (p.item_rows / 16) * blocks);
   if (splits > steps / (2 * RD_WAVES)) splits = steps / (2 * RD_WAVES);
   if (splits < 1) splits = 1;
   p.steps = (int)((steps + splits - 1) / splits);
   p.splits = (int)((steps + p.steps - 1) / p.steps);
 }
 
+// Values of t.
+int64_t request_low_ranks(const RequestAdapterParams& p) { return (int64_t)p.splits * p.rows * p.branches * p.width; }
+
+}  // namespace
+
 int64_t request_workspace(const RequestAdapterParams& params) {
   RequestAdapterParams p = params;
   request_plan(p);
-  const int64_t grouped = p.rows > RA_WAVE_ROWS ? 4 * (p.rows + 3 * (int64_t)p.items) : 0;
-  return 4 * p.splits * p.rows * p.branches * p.width + grouped;
+  return 4 * (request_low_ranks(p) + (int64_t)p.items * (4 + p.item_rows) + (p.rows > RA_WAVE_ROWS ? p.rows : 0));
 }
 
 hipError_t launch_request_adapters(const RequestAdapterParams& params, bool f16, void* workspace, hipStream_t s) {
   RequestAdapterParams p = params;
   request_plan(p);
   p.t = static_cast<float*>(workspace);
-  p.order = p.list = nullptr;
-  if (p.rows > RA_WAVE_ROWS) {
-    p.order = reinterpret_cast<int32_t*>(p.t + p.splits * p.rows * p.branches * p.width);
-    p.list = p.order + p.rows;
-    request_groups<<<1, 1024, 4 * (p.adapters + 1), s>>>(p);
-  }
-  int tiles = 0;
+  p.list = reinterpret_cast<int32_t*>(p.t + request_low_ranks(p));
+  p.order = p.list + 4 * (int64_t)p.items;
+  p.before = p.order + (int64_t)p.items * p.item_rows;
+  if (p.rows > RA_WAVE_ROWS) request_groups<<<1, 1024, 4 * (p.adapters + 1), s>>>(p);
+  const int per = p.item_rows > 16 ? 4 : 1, ranks = request_ranks(p);
+  int groups = 0;
   for (int b = 0; b < p.branches; ++b) {
-    tiles += (p.ends[b] - (b ? p.ends[b - 1] : 0) + 63) / 64;
-    p.tiles[b] = tiles;
+    groups += (p.ends[b] - (b ? p.ends[b - 1] : 0) + 64 * RU_WAVES * per - 1) / (64 * RU_WAVES * per);
+    p.groups[b] = groups;
   }
-  const int per = p.item_rows > 16 ? 4 : 1;
-  const dim3 down((unsigned)p.items, (unsigned)p.splits, (unsigned)((p.branches * p.width + 63) / 64));
-  const dim3 up((unsigned)p.items, (unsigned)((tiles + RU_WAVES * per - 1) / (RU_WAVES * per)));
-  auto run = [&](auto type, auto blocks) {
-    constexpr bool F16 = type;
-    constexpr int RB = blocks;
-    request_down<F16, RB, 4><<<down, 64 * RD_WAVES, 0, s>>>(p);
-    request_up<F16, RB><<<up, 64 * RU_WAVES, 0, s>>>(p, per);
-  };
+  const dim3 down((unsigned)(p.items * (p.item_rows / 16)), (unsigned)p.splits,
+                  (unsigned)((p.branches * p.width + ranks - 1) / ranks));
+  const dim3 up((unsigned)p.items, (unsigned)groups);
   auto typed = [&](auto type) {
-    if (p.item_rows > 16) run(type, std::integral_constant<int, 4>{});
-    else run(type, std::integral_constant<int, 1>{});
+    constexpr bool F16 = type;
+    if (ranks == 64) request_down<F16, 4><<<down, 64 * RD_WAVES, 0, s>>>(p);
+    else if (ranks == 32) request_down<F16, 2><<<down, 64 * RD_WAVES, 0, s>>>(p);
+    else request_down<F16, 1><<<down, 64 * RD_WAVES, 0, s>>>(p);
+    if (p.width <= 32) request_up<F16, 1><<<up, 64 * RU_WAVES, 0, s>>>(p, per);
+    else if (p.width <= 64) request_up<F16, 2><<<up, 64 * RU_WAVES, 0, s>>>(p, per);
+    else request_up<F16, 4><<<up, 64 * RU_WAVES, 0, s>>>(p, per);
   };
   if (f16) typed(std::true_type{});
   else typed(std::false_type{});
