@@ -531,12 +531,12 @@ int vflash_paged_append(const void* q, int64_t q_ts, int64_t q_hs, const void* k
  *   With scales, a key's factor multiplies its score and a value's its weight before that is rounded to bf16.
  * Lengths are clamped to the table.  Keys on a page outside [0, pages) count as keys and values of zeros.  Nothing
  * else outside a sequence's pages is read.  Masked keys, rows that see none, and scores as vflash_packed_attention.
- *   workspace  vflash_paged_attention_workspace(...) bytes (0: may be NULL), 16-byte aligned, without contents to
- *              keep; one call at a time
+ *   workspace  vflash_paged_attention_workspace(...) bytes (e4m3: with scales; 0: may be NULL), 16-byte aligned,
+ *              without contents to keep; one call at a time
  *   Requires what vflash_paged_append does, and heads % key_heads == 0.
  */
 int64_t vflash_paged_attention_workspace(int64_t tokens, int64_t batch, int64_t heads, int64_t key_heads, int64_t dim,
-                                         int64_t page, int64_t width);
+                                         int64_t page, int64_t width, int e4m3);
 int vflash_paged_attention(const void* q, int64_t q_ts, int64_t q_hs, int f16, int64_t tokens, int64_t heads,
                            int64_t key_heads, int64_t dim, const int64_t* q_offsets, const void* values,
                            const float* scales, int64_t pages, int64_t page, const int64_t* table, int64_t width,

@@ -143,7 +143,7 @@ int main() {
     p.tokens = tokens, p.keys = keys, p.batch = batch, p.heads = heads, p.group = group, p.dim = dim, p.causal = 1;
     if (given) p.q_offsets = vector(batch + 1, at_end);
     p.cache.lengths = vector(batch, at_end);
-    plan = paged_attention_plan(p);
+    plan = paged_attention_plan(p, at_end);
     printf("plan %d %d %d %d %d %lld %lld %d\n", plan.step, p.tile_tokens, p.heads_per_tile, p.parts, p.head_blocks,
            (long long)p.slots, (long long)plan.grid, plan.join != 0);
     blocks = (unsigned)plan.grid;

@@ -314,9 +314,9 @@ def test_adapter_entry_refuses():
 
 def test_workspaces():
     lib = _lib.library()
-    assert lib.vflash_paged_attention_workspace(4, 4, 32, 8, 128, 16, 48) == 0  # room for 768 keys: no split
-    assert lib.vflash_paged_attention_workspace(4, 4, 32, 8, 128, 16, 49) > 0
-    assert lib.vflash_paged_attention_workspace(4, 4, 32, 8, 128, 17, 49) == _lib.VFLASH_EINVAL
+    assert lib.vflash_paged_attention_workspace(4, 4, 32, 8, 128, 16, 48, 0) == 0  # room for 768 keys: no split
+    assert lib.vflash_paged_attention_workspace(4, 4, 32, 8, 128, 16, 49, 0) > 0
+    assert lib.vflash_paged_attention_workspace(4, 4, 32, 8, 128, 17, 49, 0) == _lib.VFLASH_EINVAL
     widths = (ctypes.c_int64 * 1)(64)
     small = lib.vflash_request_adapters_workspace(64, 64, widths, 1, 5, 16)
     assert small == 64 * 16 * 4 + 10 * (4 + 16) * 4  # one part of t, and at most ten items

@@ -118,7 +118,7 @@ SIGNATURES: dict[str, tuple[list, object]] = {
          _I64, _P, _P, _I64, _I64, _P, _I64, _P, _I64, _P, _P],
         _I32,
     ),
-    "vflash_paged_attention_workspace": ([_I64] * 7, _I64),
+    "vflash_paged_attention_workspace": ([_I64] * 7 + [_I32], _I64),
     "vflash_paged_attention": (
         [_P, _I64, _I64, _I32, _I64, _I64, _I64, _I64, _P, _P, _P, _I64, _I64, _P, _I64, _P, _I64, _F32, _P, _I64, _I64,
          _P, _I64, _P],

@@ -287,9 +287,9 @@ int64_t attention_workspace(const AttentionParams& params) {
   return workspace_of(p, plan);
 }
 
-int64_t paged_attention_workspace(const AttentionParams& params) {
+int64_t paged_attention_workspace(const AttentionParams& params, bool e4m3) {
   AttentionParams p = params;
-  const AttentionPlan plan = paged_attention_plan(p);
+  const AttentionPlan plan = paged_attention_plan(p, e4m3);
   return workspace_of(p, plan);
 }
 
@@ -300,9 +300,9 @@ bool attention_fits(const AttentionParams& params) {
   return plan_fits(attention_plan(p));
 }
 
-bool paged_attention_fits(const AttentionParams& params) {
+bool paged_attention_fits(const AttentionParams& params, bool e4m3) {
   AttentionParams p = params;
-  return plan_fits(paged_attention_plan(p));
+  return plan_fits(paged_attention_plan(p, e4m3));
 }
 
 hipError_t launch_attention(const AttentionParams& params, bool f16, void* workspace, hipStream_t s) {
@@ -325,7 +325,7 @@ hipError_t launch_attention(const AttentionParams& params, bool f16, void* works
 
 hipError_t launch_paged_attention(const AttentionParams& params, bool f16, void* workspace, hipStream_t s) {
   AttentionParams p = params;
-  const AttentionPlan plan = paged_attention_plan(p);
+  const AttentionPlan plan = paged_attention_plan(p, p.cache.scales != nullptr);
   // Tiles of 16 follow the maximum once it is 2^8 above: no shift for more, so that weights times the factors of small
   // E4M3 values stay above bf16's subnormals.
   attention_memory(p, plan, (int)kAttentionSlack, workspace);

@@ -36,16 +36,15 @@ inline int64_t attention_tiles_at_most(const AttentionParams& p) {
   return tiles < p.tokens ? tiles : p.tokens;
 }
 
-// The rest of the plan of tiles of 16.
-inline void attention_step_plan(AttentionParams& p, AttentionPlan& plan, bool split) {
-  // A CU holds one workgroup of dimension 128, two of 64.
+// The rest of the plan of tiles of 16; `per_cu`: workgroups that a CU holds.
+inline void attention_step_plan(AttentionParams& p, AttentionPlan& plan, bool split, int per_cu) {
   const int64_t tiles = attention_tiles_at_most(p);
   p.unit_shift = split ? 7 : 31;
   auto bound = [&] { return tiles * p.head_blocks * (((int64_t)p.keys >> p.unit_shift) + 1); };
   while (bound() >= int64_t(1) << 30 && p.unit_shift < 31) ++p.unit_shift;  // the kernel counts in 32 bits
   const int64_t units = bound();
   plan.line = p.head_blocks % 8 ? units : units / 8;
-  plan.grid = (compute_units() + 7) / 8 * 8 * (p.dim <= 64 ? 2 : 1);
+  plan.grid = (compute_units() + 7) / 8 * 8 * per_cu;
   if (units < plan.grid) plan.grid = (units + 7) / 8 * 8;
   plan.join = split;
   p.slots = split ? 2 * plan.grid : 0;
@@ -53,10 +52,10 @@ inline void attention_step_plan(AttentionParams& p, AttentionPlan& plan, bool sp
 
 // Over a paged cache every call runs in tiles of 16; the keys are split where a sequence has room for more than
 // 768.
-inline AttentionPlan paged_attention_plan(AttentionParams& p) {
+inline AttentionPlan paged_attention_plan(AttentionParams& p, bool e4m3) {
   AttentionPlan plan{};
   attention_shape(p, plan, true);
-  attention_step_plan(p, plan, p.keys > 768);
+  attention_step_plan(p, plan, p.keys > 768, (p.dim <= 64 ? 2 : 1) * (e4m3 ? 2 : 1));
   return plan;
 }
 
@@ -87,7 +86,7 @@ inline AttentionPlan attention_plan(AttentionParams& p) {
   const int64_t rows = (int64_t)p.tokens * (p.group < kStepRows ? p.group : kStepRows);
   if (rows <= kStepRows * p.batch || (rows <= 2 * kStepRows * p.batch && 2 * p.batch * p.head_blocks < cus)) shape(true);
   if (plan.step) {
-    attention_step_plan(p, plan, p.keys > 768 && p.keys > 512 * p.batch);
+    attention_step_plan(p, plan, p.keys > 768 && p.keys > 512 * p.batch, p.dim <= 64 ? 2 : 1);
     return plan;
   }
   const int64_t tiles = attention_tiles_at_most(p), whole = p.tokens / p.tile_tokens;

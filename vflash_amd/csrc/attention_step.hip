@@ -24,7 +24,7 @@ struct AttentionSteps {
   static constexpr bool E4M3 = STORE == kStoreE4M3;
   static constexpr int PITCH = (DP <= 64 ? 64 : 128) * (E4M3 ? 1 : 2), CHUNKS = PITCH / 16, ROWS = 1024 / PITCH;
   static constexpr int KEYS = 32, TILE = KEYS * PITCH, SLOT = 2 * TILE + (E4M3 ? 512 : 0), WAVES = 4;
-  static constexpr int NS = E4M3 ? 4 : 2;
+  static constexpr int NS = 2;
   static constexpr int DMA = 2 * TILE / 1024 + (E4M3 ? 2 : 0);  // instructions per stage
   static constexpr int ACC = DP * 4 + 16;  // bytes of a row's sums in LDS
 };

@@ -42,8 +42,8 @@ hipError_t launch_nvfp4_w16(const GemmParams&, bool, hipStream_t);
 int64_t attention_workspace(const AttentionParams&);
 bool attention_fits(const AttentionParams&);
 hipError_t launch_attention(const AttentionParams&, bool, void*, hipStream_t);
-int64_t paged_attention_workspace(const AttentionParams&);
-bool paged_attention_fits(const AttentionParams&);
+int64_t paged_attention_workspace(const AttentionParams&, bool);
+bool paged_attention_fits(const AttentionParams&, bool);
 hipError_t launch_paged_attention(const AttentionParams&, bool, void*, hipStream_t);
 hipError_t launch_rotate(const RotateParams&, hipStream_t);
 int64_t request_workspace(const RequestAdapterParams&);
@@ -208,7 +208,7 @@ bool paged_attention_sizes(vfa::AttentionParams& p, int64_t tokens, int64_t batc
   p.group = (int)(heads / key_heads);
   p.dim = (int)dim;
   p.causal = 1;
-  return vfa::paged_attention_fits(p);
+  return vfa::paged_attention_fits(p, codes);
 }
 
 // Rows [tokens, heads, dim] that 16-byte vectors can be taken from.
@@ -709,10 +709,10 @@ int vflash_paged_append(const void* q, int64_t q_ts, int64_t q_hs, const void* k
 }
 
 int64_t vflash_paged_attention_workspace(int64_t tokens, int64_t batch, int64_t heads, int64_t key_heads, int64_t dim,
-                                         int64_t page, int64_t width) {
+                                         int64_t page, int64_t width, int e4m3) {
   vfa::AttentionParams p{};
-  if (!paged_attention_sizes(p, tokens, batch, heads, key_heads, dim, 0, page, width, false)) return VFLASH_EINVAL;
-  return vfa::paged_attention_workspace(p);
+  if (!paged_attention_sizes(p, tokens, batch, heads, key_heads, dim, 0, page, width, e4m3 != 0)) return VFLASH_EINVAL;
+  return vfa::paged_attention_workspace(p, e4m3 != 0);
 }
 
 int vflash_paged_attention(const void* q, int64_t q_ts, int64_t q_hs, int f16, int64_t tokens, int64_t heads,
@@ -730,7 +730,7 @@ int vflash_paged_attention(const void* q, int64_t q_ts, int64_t q_hs, int f16, i
     return VFLASH_EINVAL;
   p.c = scale * 1.4426950408889634f;
   if (!(p.c > 0.0f) || p.c > 3.4028234663852886e38f) return VFLASH_EINVAL;  // rejects NaN and infinity too
-  const int64_t need = vfa::paged_attention_workspace(p);
+  const int64_t need = vfa::paged_attention_workspace(p, scales != nullptr);
   if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16))) return VFLASH_EINVAL;
   p.q = static_cast<const uint16_t*>(q);
   p.out = static_cast<uint16_t*>(out);

@@ -393,7 +393,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   const int64_t tokens = q->size(0), heads = q->size(1), dim = q->size(2);
   if (tokens == 0 || !pages_ok(a[1], a[2], a[3], a[4], a[5], *q, c)) Py_RETURN_NONE;
   const int64_t key_heads = c.values->size(2), page = c.values->size(3);
-  const int64_t bytes = vflash_paged_attention_workspace(tokens, c.batch, heads, key_heads, dim, page, c.width);
+  const int64_t bytes = vflash_paged_attention_workspace(tokens, c.batch, heads, key_heads, dim, page, c.width, c.scales != nullptr);
   if (bytes < 0) Py_RETURN_NONE;
   const double scale = a[6] == Py_None ? 1.0 / std::sqrt((double)dim) : PyFloat_AS_DOUBLE(a[6]);
   at::Tensor out;

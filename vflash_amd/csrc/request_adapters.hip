@@ -116,6 +116,9 @@ __global__ void __launch_bounds__(1024) request_groups(const RequestAdapterParam
   __shared__ int sums[17];
   const int bins = p.adapters + 1, t = (int)threadIdx.x, lane = t & 63, wave = t >> 6;
   for (int b = t; b < bins; b += 1024) counts[b] = 0;
+  // Thread t's bins are next to each other; their ranks are on the way meanwhile.
+  const int per = (bins + 1023) / 1024, b0 = min(t * per, bins), b1 = min(b0 + per, bins);
+  const int rank0 = b0 < p.adapters ? rank_of(p, b0) : 0;
   __syncthreads();
   auto bin_of = [&](int64_t m) {
     if (m >= p.rows) return -1;
@@ -123,11 +126,11 @@ __global__ void __launch_bounds__(1024) request_groups(const RequestAdapterParam
     return (uint64_t)i < (uint64_t)p.adapters ? (int)i : p.adapters;
   };
   // Adds one to a bin for each lane, and gives each the count before it.  Lanes of one bin (runs) go together, for the first
-  // few bins of a wave: the same word is added to once at a time.
+  // two bins of a wave: the same word is added to once at a time.
   auto add = [&](int bin) {
     int before = 0;
     uint64_t left = __builtin_amdgcn_ballot_w64(bin >= 0);
-    for (int i = 0; i < 6 && left; ++i) {
+    for (int i = 0; i < 2 && left; ++i) {
       const int first = __builtin_ctzll(left), b = __builtin_amdgcn_readlane(bin, first);
       const uint64_t same = __builtin_amdgcn_ballot_w64(bin == b);
       int old = 0;
@@ -152,8 +155,6 @@ __global__ void __launch_bounds__(1024) request_groups(const RequestAdapterParam
     if (m < p.rows) p.before[m] = before;
   }
   __syncthreads();
-  // Thread t's bins are next to each other.
-  const int per = (bins + 1023) / 1024, b0 = min(t * per, bins), b1 = min(b0 + per, bins);
   auto items_of = [&](int c) { return (c + p.item_rows - 1) / p.item_rows; };
   int items = 0;
   for (int b = b0; b < b1; ++b) items += items_of(counts[b]);
@@ -167,7 +168,7 @@ __global__ void __launch_bounds__(1024) request_groups(const RequestAdapterParam
   }
   item -= items;
   for (int b = b0; b < b1; ++b) {
-    const int c = counts[b], rank = b < p.adapters && c ? rank_of(p, b) : 0;
+    const int c = counts[b], rank = b == b0 ? rank0 : b < p.adapters && c ? rank_of(p, b) : 0;
     counts[b] = item * p.item_rows;
     for (int first = 0; first < c; first += p.item_rows, ++item)
       *reinterpret_cast<v4i*>(p.list + 4 * item) = v4i{b < p.adapters ? b : -1, min(p.item_rows, c - first), rank, 0};
@@ -180,13 +181,16 @@ __global__ void __launch_bounds__(1024) request_groups(const RequestAdapterParam
   for (int64_t m = t + 1024 * KEPT; m < p.rows; m += 1024) p.order[counts[bin_of(m)] + p.before[m]] = (int)m;
 }
 
-// t of 16 rows of an item for RK blocks of 16 adapter rows and one split of K.
-template <bool F16, int RK>
+// t of an item's RB blocks of 16 rows for RK blocks of 16 adapter rows and one split of K.  Items of 64 rows read A
+// once for all four blocks: a workgroup for each 16 took 51 us for 1000 rows of 24 adapters (rank 64, K 5120, three
+// branches), bound by what L2 delivers.
+template <bool F16, int RB, int RK>
 __global__ void __launch_bounds__(64 * RD_WAVES) request_down(const RequestAdapterParams p) {
-  __shared__ int rows[64];
-  __shared__ v4f part[RD_WAVES][RK][64];
+  constexpr int PASS = RB > 2 ? 2 : RB;  // row blocks whose sums are in LDS together
+  __shared__ int rows[RB * 16];
+  __shared__ v4f part[RD_WAVES][PASS * RK][64];
+  const int item = (int)blockIdx.x;
   const bool grouped = p.rows > RA_WAVE_ROWS;
-  const int per_item = p.item_rows / 16, item = (int)blockIdx.x / per_item, first = ((int)blockIdx.x - item * per_item) * 16;
   // Ungrouped, every wave finds the same and writes the same.
   const RequestItem it = uniform(grouped ? request_listed(p, item, rows) : request_find(p, item, rows));
   __syncthreads();
@@ -194,14 +198,14 @@ __global__ void __launch_bounds__(64 * RD_WAVES) request_down(const RequestAdapt
     if (threadIdx.x == 0) *reinterpret_cast<v4i*>(p.list + 4 * item) = v4i{it.adapter, it.count, it.rank, 0};
     if ((int)threadIdx.x < it.count) p.order[item * p.item_rows + threadIdx.x] = rows[threadIdx.x];
   }
-  if (first >= it.count || it.adapter < 0) return;
+  if (it.count == 0 || it.adapter < 0) return;
   const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int fr = lane & 15, fg = lane >> 4;
   const int all = p.branches * p.width, r0 = (int)blockIdx.z * RK * 16;
 
   // Blocks of adapter rows that hold some of the rank.
   bool used[RK], any = false;
-  const uint16_t* ar[RK];
+  const uint16_t *xr[RB], *ar[RK];
   static_for<RK>([&](auto j) {
     const int r = r0 + j * 16;
     used[j] = r < all && r % p.width < it.rank;
@@ -209,44 +213,48 @@ __global__ void __launch_bounds__(64 * RD_WAVES) request_down(const RequestAdapt
     ar[j] = p.down + ((int64_t)it.adapter * all + min(r + fr, all - 1)) * p.k;
   });
   if (!any) return;
-  const int row = rows[min(first + fr, it.count - 1)];
-  const uint16_t* xr = p.x + (int64_t)row * p.ldx;
+  static_for<RB>([&](auto i) { xr[i] = p.x + (int64_t)rows[min((int)i * 16 + fr, it.count - 1)] * p.ldx; });
   const int steps = (int)((p.k + 31) / 32);
   const int from = (int)blockIdx.y * p.steps, to = min(from + p.steps, steps);
   const int s0 = from + max(0, to - from) * wave / RD_WAVES, s1 = from + max(0, to - from) * (wave + 1) / RD_WAVES;
 
-  constexpr int AHEAD = 8;  // steps whose loads are in flight together
-  v4f acc[RK];
-  static_for<RK>([&](auto j) { acc[j] = v4f{}; });
+  constexpr int AHEAD = RB == 1 || RK <= 2 ? 8 : 4;  // steps whose loads are in flight together
+  v4f acc[RB][RK];
+  static_for<RB>([&](auto i) { static_for<RK>([&](auto j) { acc[i][j] = v4f{}; }); });
   for (int s = s0; s < s1; s += AHEAD) {
-    v4i xv[AHEAD], av[AHEAD][RK];
+    v4i xv[AHEAD][RB], av[AHEAD][RK];
     static_for<AHEAD>([&](auto a) {
       const int64_t at = (int64_t)(s + a) * 32 + fg * 8;
       const bool ok = s + a < s1 && at < p.k;
-      xv[a] = ok ? *reinterpret_cast<const v4i*>(xr + at) : v4i{};
+      static_for<RB>([&](auto i) { xv[a][i] = ok && i * 16 < it.count ? *reinterpret_cast<const v4i*>(xr[i] + at) : v4i{}; });
       static_for<RK>([&](auto j) { av[a][j] = ok && used[j] ? *reinterpret_cast<const v4i*>(ar[j] + at) : v4i{}; });
     });
     static_for<AHEAD>([&](auto a) {
-      static_for<RK>([&](auto j) { acc[j] = mfma16<F16>(av[a][j], xv[a], acc[j]); });
+      static_for<RB>([&](auto i) {
+        static_for<RK>([&](auto j) { acc[i][j] = mfma16<F16>(av[a][j], xv[a][i], acc[i][j]); });
+      });
     });
   }
-  static_for<RK>([&](auto j) { part[wave][j][lane] = acc[j]; });
-  __syncthreads();
-  // Lane (fr, fg) of block j: t of row fr, ranks r0 + j * 16 + 4 fg + 0 .. 3.
-  for (int j = wave; j < RK; j += RD_WAVES) {
-    const int r = r0 + j * 16;
-    if (r >= all || first + fr >= it.count) continue;
-    v4f sum = part[0][j][lane];
-    static_for<RD_WAVES - 1>([&](auto w) { sum += part[w + 1][j][lane]; });
-    *reinterpret_cast<v4f*>(p.t + ((int64_t)blockIdx.y * p.rows + row) * all + r + 4 * fg) = sum;
-  }
+  static_for<RB / PASS>([&](auto pass) {
+    if (pass) __syncthreads();
+    static_for<PASS>([&](auto i) { static_for<RK>([&](auto j) { part[wave][i * RK + j][lane] = acc[pass * PASS + i][j]; }); });
+    __syncthreads();
+    // Lane (fr, fg) of block (i, j): t of row i * 16 + fr, ranks r0 + j * 16 + 4 fg + 0 .. 3.
+    for (int b = wave; b < PASS * RK; b += RD_WAVES) {
+      const int i = pass * PASS + b / RK, r = r0 + b % RK * 16;
+      if (r >= all || i * 16 + fr >= it.count) continue;
+      v4f sum = part[0][b][lane];
+      static_for<RD_WAVES - 1>([&](auto w) { sum += part[w + 1][b][lane]; });
+      *reinterpret_cast<v4f*>(p.t + ((int64_t)blockIdx.y * p.rows + rows[i * 16 + fr]) * all + r + 4 * fg) = sum;
+    }
+  });
 }
 
 // Tiles of 64 columns of one branch and item, ranks in NC runs of 32.  MFMA block j of a tile holds the columns
 // 32 (j / 2) + 8 g + 4 (j % 2) + e in its rows 4 g + e, so that a lane ends with two runs of eight columns of one row, and
 // the four lanes of a row store 64 bytes at once.
 template <bool F16, int NC>
-__global__ void __launch_bounds__(64 * RU_WAVES) request_up(const RequestAdapterParams p, int tiles_per_wave) {
+__global__ void __launch_bounds__(64 * RU_WAVES) request_up(const RequestAdapterParams p) {
   constexpr int PITCH = 64 * NC + 8;  // of a row in LDS: high parts, low parts, and eight against bank conflicts
   __shared__ int rows[64];
   __shared__ __attribute__((aligned(16))) uint16_t low_rank[64 * PITCH];
@@ -288,72 +296,69 @@ __global__ void __launch_bounds__(64 * RU_WAVES) request_up(const RequestAdapter
   }
   __syncthreads();
 
-  // The waves' tiles lie side by side.
-  for (int k = 0; k < tiles_per_wave; ++k) {
-    const int n0 = first_col + ((group * tiles_per_wave + k) * RU_WAVES + wave) * 64;
-    if (n0 >= stop) return;
-    const int n = n0 + 8 * fg;  // this lane's columns: n .. n + 7 and 32 further, up to stop
-    v4i b[NC][4], rest[NC][4];
+  const int n0 = first_col + (group * RU_WAVES + wave) * 64;
+  if (n0 >= stop) return;
+  const int n = n0 + 8 * fg;  // this lane's columns: n .. n + 7 and 32 further, up to stop
+  v4i b[NC][4], rest[NC][4];
+  static_for<NC>([&](auto c) {
+    const int r = c * 32 + 8 * fg;
+    static_for<4>([&](auto j) {
+      const int col = n0 + 32 * (j / 2) + 8 * (fr >> 2) + 4 * (j % 2) + (fr & 3);
+      b[c][j] = r < it.rank && col < stop
+                    ? *reinterpret_cast<const v4i*>(p.up + ((int64_t)it.adapter * p.n + col) * p.width + r) : v4i{};
+    });
+  });
+  int64_t row[4];
+  v4i base[4][2];
+  static_for<4>([&](auto i) {
+    if (16 * i >= it.count) return;
+    row[i] = rows[min(16 * (int)i + fr, it.count - 1)];
+    static_for<2>([&](auto h) {
+      base[i][h] = n + 32 * h < stop ? *reinterpret_cast<const v4i*>(p.base + row[i] * p.ldb + n + 32 * h) : v4i{};
+    });
+  });
+  if constexpr (F16)
     static_for<NC>([&](auto c) {
-      const int r = c * 32 + 8 * fg;
       static_for<4>([&](auto j) {
-        const int col = n0 + 32 * (j / 2) + 8 * (fr >> 2) + 4 * (j % 2) + (fr & 3);
-        b[c][j] = r < it.rank && col < stop
-                      ? *reinterpret_cast<const v4i*>(p.up + ((int64_t)it.adapter * p.n + col) * p.width + r) : v4i{};
-      });
-    });
-    int64_t row[4];
-    v4i base[4][2];
-    static_for<4>([&](auto i) {
-      if (16 * i >= it.count) return;
-      row[i] = rows[min(16 * (int)i + fr, it.count - 1)];
-      static_for<2>([&](auto h) {
-        base[i][h] = n + 32 * h < stop ? *reinterpret_cast<const v4i*>(p.base + row[i] * p.ldb + n + 32 * h) : v4i{};
-      });
-    });
-    if constexpr (F16)
-      static_for<NC>([&](auto c) {
-        static_for<4>([&](auto j) {
-          static_for<4>([&](auto e) {
-            const uint32_t w = (uint32_t)b[c][j][(int)e];
-            int high, low;
-            parts(widen<true>(w, 0), widen<true>(w, 1), high, low);
-            b[c][j][(int)e] = high;
-            rest[c][j][(int)e] = low;
-          });
-        });
-      });
-    static_for<4>([&](auto i) {
-      if (16 * i >= it.count) return;
-      v4f acc[4];
-      static_for<4>([&](auto j) { acc[j] = v4f{}; });
-      const uint16_t* src = low_rank + min(16 * (int)i + fr, it.count - 1) * PITCH + 8 * fg;
-      static_for<NC>([&](auto c) {
-        if (c * 32 >= it.rank) return;
-        const v4i high = *reinterpret_cast<const v4i*>(src + c * 32), low = *reinterpret_cast<const v4i*>(src + 32 * NC + c * 32);
-        static_for<4>([&](auto j) {
-          acc[j] = mfma16<false>(b[c][j], high, acc[j]);
-          acc[j] = mfma16<false>(b[c][j], low, acc[j]);
-        });
-        if constexpr (F16) {
-          const v4i near = finite(high);  // an infinity is in the first product
-          static_for<4>([&](auto j) { acc[j] = mfma16<false>(rest[c][j], near, acc[j]); });
-        }
-      });
-      if (16 * i + fr >= it.count) return;
-      static_for<2>([&](auto h) {
-        if (n + 32 * h >= stop) return;
-        v4i o;
         static_for<4>([&](auto e) {
-          constexpr int at = 8 * h + 2 * e;
-          const uint32_t w = (uint32_t)base[i][h][(int)e];
-          o[(int)e] = pack<F16>(__builtin_fmaf(acc[at / 4][at % 4], scaling, widen<F16>(w, 0)),
-                                __builtin_fmaf(acc[at / 4][at % 4 + 1], scaling, widen<F16>(w, 1)));
+          const uint32_t w = (uint32_t)b[c][j][(int)e];
+          int high, low;
+          parts(widen<true>(w, 0), widen<true>(w, 1), high, low);
+          b[c][j][(int)e] = high;
+          rest[c][j][(int)e] = low;
         });
-        *reinterpret_cast<v4i*>(p.out + row[i] * p.ldo + n + 32 * h) = it.rank > 0 ? o : base[i][h];
       });
     });
-  }
+  static_for<4>([&](auto i) {
+    if (16 * i >= it.count) return;
+    v4f acc[4];
+    static_for<4>([&](auto j) { acc[j] = v4f{}; });
+    const uint16_t* src = low_rank + min(16 * (int)i + fr, it.count - 1) * PITCH + 8 * fg;
+    static_for<NC>([&](auto c) {
+      if (c * 32 >= it.rank) return;
+      const v4i high = *reinterpret_cast<const v4i*>(src + c * 32), low = *reinterpret_cast<const v4i*>(src + 32 * NC + c * 32);
+      static_for<4>([&](auto j) {
+        acc[j] = mfma16<false>(b[c][j], high, acc[j]);
+        acc[j] = mfma16<false>(b[c][j], low, acc[j]);
+      });
+      if constexpr (F16) {
+        const v4i near = finite(high);  // an infinity is in the first product
+        static_for<4>([&](auto j) { acc[j] = mfma16<false>(rest[c][j], near, acc[j]); });
+      }
+    });
+    if (16 * i + fr >= it.count) return;
+    static_for<2>([&](auto h) {
+      if (n + 32 * h >= stop) return;
+      v4i o;
+      static_for<4>([&](auto e) {
+        constexpr int at = 8 * h + 2 * e;
+        const uint32_t w = (uint32_t)base[i][h][(int)e];
+        o[(int)e] = pack<F16>(__builtin_fmaf(acc[at / 4][at % 4], scaling, widen<F16>(w, 0)),
+                              __builtin_fmaf(acc[at / 4][at % 4 + 1], scaling, widen<F16>(w, 1)));
+      });
+      *reinterpret_cast<v4i*>(p.out + row[i] * p.ldo + n + 32 * h) = it.rank > 0 ? o : base[i][h];
+    });
+  });
 }
 
 namespace {
@@ -373,7 +378,7 @@ void request_plan(RequestAdapterParams& p) {
   if (p.items > p.rows) p.items = (int)p.rows;
   const int64_t steps = (p.k + 31) / 32, blocks = (p.branches * p.width + request_ranks(p) - 1) / request_ranks(p);
   // About one workgroup a CU, of at least two steps a wave.
-  int64_t splits = cus / (p.items * (p.item_rows / 16) * blocks);
+  int64_t splits = cus / (p.items * blocks);
   if (splits > steps / (2 * RD_WAVES)) splits = steps / (2 * RD_WAVES);
   if (splits < 1) splits = 1;
   p.steps = (int)((steps + splits - 1) / splits);
@@ -399,23 +404,28 @@ hipError_t launch_request_adapters(const RequestAdapterParams& params, bool f16,
   p.order = p.list + 4 * (int64_t)p.items;
   p.before = p.order + (int64_t)p.items * p.item_rows;
   if (p.rows > RA_WAVE_ROWS) request_groups<<<1, 1024, 4 * (p.adapters + 1), s>>>(p);
-  const int per = p.item_rows > 16 ? 4 : 1, ranks = request_ranks(p);
+  const int ranks = request_ranks(p);
   int groups = 0;
   for (int b = 0; b < p.branches; ++b) {
-    groups += (p.ends[b] - (b ? p.ends[b - 1] : 0) + 64 * RU_WAVES * per - 1) / (64 * RU_WAVES * per);
+    groups += (p.ends[b] - (b ? p.ends[b - 1] : 0) + 64 * RU_WAVES - 1) / (64 * RU_WAVES);
     p.groups[b] = groups;
   }
-  const dim3 down((unsigned)(p.items * (p.item_rows / 16)), (unsigned)p.splits,
-                  (unsigned)((p.branches * p.width + ranks - 1) / ranks));
+  const dim3 down((unsigned)p.items, (unsigned)p.splits, (unsigned)((p.branches * p.width + ranks - 1) / ranks));
   const dim3 up((unsigned)p.items, (unsigned)groups);
+  auto run_down = [&](auto type, auto blocks) {
+    constexpr bool F16 = type;
+    constexpr int RB = blocks;
+    if (ranks == 64) request_down<F16, RB, 4><<<down, 64 * RD_WAVES, 0, s>>>(p);
+    else if (ranks == 32) request_down<F16, RB, 2><<<down, 64 * RD_WAVES, 0, s>>>(p);
+    else request_down<F16, RB, 1><<<down, 64 * RD_WAVES, 0, s>>>(p);
+  };
   auto typed = [&](auto type) {
     constexpr bool F16 = type;
-    if (ranks == 64) request_down<F16, 4><<<down, 64 * RD_WAVES, 0, s>>>(p);
-    else if (ranks == 32) request_down<F16, 2><<<down, 64 * RD_WAVES, 0, s>>>(p);
-    else request_down<F16, 1><<<down, 64 * RD_WAVES, 0, s>>>(p);
-    if (p.width <= 32) request_up<F16, 1><<<up, 64 * RU_WAVES, 0, s>>>(p, per);
-    else if (p.width <= 64) request_up<F16, 2><<<up, 64 * RU_WAVES, 0, s>>>(p, per);
-    else request_up<F16, 4><<<up, 64 * RU_WAVES, 0, s>>>(p, per);
+    if (p.item_rows > 16) run_down(type, std::integral_constant<int, 4>{});
+    else run_down(type, std::integral_constant<int, 1>{});
+    if (p.width <= 32) request_up<F16, 1><<<up, 64 * RU_WAVES, 0, s>>>(p);
+    else if (p.width <= 64) request_up<F16, 2><<<up, 64 * RU_WAVES, 0, s>>>(p);
+    else request_up<F16, 4><<<up, 64 * RU_WAVES, 0, s>>>(p);
   };
   if (f16) typed(std::true_type{});
   else typed(std::false_type{});

@@ -784,7 +784,8 @@ def paged_attention(q, cache, table, lengths, q_offsets, scale):
         return out
     pages, _, key_heads, page, _ = cache.values.shape
     batch, width = table.shape
-    size = _lib.library().vflash_paged_attention_workspace(tokens, batch, heads, key_heads, dim, page, width)
+    size = _lib.library().vflash_paged_attention_workspace(tokens, batch, heads, key_heads, dim, page, width,
+                                                           int(cache.scales is not None))
     if size < 0:
         raise ValueError("paged attention: more rows than a call takes")
     workspace = torch.empty(size, device=device, dtype=torch.uint8) if size else None
