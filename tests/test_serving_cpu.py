@@ -331,18 +331,21 @@ def test_launches(tmp_path):
     def arguments(defaults, **change):
         return [f"@{v}" if v == P and isinstance(v, int) else v for v in {**defaults, **change}.values()]
 
-    # A workgroup a token; more tokens than a grid's first dimension takes continue in the second.  Few tokens: 32 heads
-    # of 64 at a time each.
+    # A workgroup a token; more tokens than a grid's first dimension takes continue in the second.  Few tokens: eight heads
+    # of 64 each.
     calls = [("vflash_rotate", arguments(ROTATE)), ("vflash_rotate", arguments(ROTATE, heads=40, key_heads=40)),
              ("vflash_rotate", arguments(ROTATE, tokens=(1 << 22) + 1, f16=1)),
              ("vflash_paged_append", arguments(APPEND)), ("vflash_paged_append", arguments(APPEND, tokens=2, q_offsets=None)),
              ("vflash_paged_attention", arguments(ATTEND)), ("vflash_paged_attention", arguments(ATTEND, scales=P, f16=1)),
-             ("vflash_paged_attention", arguments(ATTEND, width=64, workspace=P, workspace_bytes=1 << 30))]
+             ("vflash_paged_attention", arguments(ATTEND, width=64, workspace=P, workspace_bytes=1 << 30)),
+             ("vflash_paged_attention", arguments(ATTEND, tokens=300, batch=300, q_offsets=None, width=128, workspace=P,
+                                                  workspace_bytes=1 << 30))]
     got = launches(tmp_path, calls)
     assert all(status == 0 for status, _ in got)
     kernels = [[(name, grid) for name, grid, _ in done] for _, done in got]
-    assert kernels[0] == [("rotate_heads<0>", (4, 1, 1))] and kernels[1] == [("rotate_heads<0>", (4, 1, 3))]
+    assert kernels[0] == [("rotate_heads<0>", (4, 1, 1))] and kernels[1] == [("rotate_heads<0>", (4, 1, 10))]
     assert kernels[2] == [("rotate_heads<1>", (1 << 22, 2, 1))]
     assert kernels[3] == [("rotate_heads<0>", (4, 1, 1))] and kernels[4] == [("rotate_heads<0>", (2, 1, 1))]
     assert [k for k, _ in kernels[5]] == ["attention_step<0,64,1>"] and [k for k, _ in kernels[6]] == ["attention_step<1,64,2>"]
-    assert [k for k, _ in kernels[7]] == ["attention_step<0,64,1>", "attention_step_join<0,1>"]
+    assert [k for k, _ in kernels[7]] == ["attention_step<0,64,1>", "attention_step_join<0,1,1024>"]
+    assert [k for k, _ in kernels[8]] == ["attention_step<0,64,1>", "attention_step_join<0,1,256>"]

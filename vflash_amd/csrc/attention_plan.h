@@ -11,7 +11,7 @@ constexpr int kTileWaves = 4, kTileRows = 32 * kTileWaves, kStepRows = 16;
 struct AttentionPlan {
   bool step;
   int rows;            // of a tile
-  int64_t grid, join;  // workgroups; 0: no split
+  int64_t grid, join;  // workgroups; 0: no split (step: 1, and 2 for small workgroups of the join)
   int64_t line;        // step: units that a line may hold, counted in 32 bits
 };
 
@@ -50,12 +50,29 @@ inline void attention_step_plan(AttentionParams& p, AttentionPlan& plan, bool sp
   p.slots = split ? 2 * plan.grid : 0;
 }
 
-// Over a paged cache every call runs in tiles of 16; the keys are split where a sequence has room for more than
-// 768.
+// Over a paged cache every call runs in tiles of 16.  A sequence's room stands for its length, which varies: the keys are
+// split from 768 where the tiles leave half of the workgroups idle, and else from 1536.  Equal lengths, us
+// whole and split, 32 heads over 8 of dimension 128 in bf16 and E4M3, and of 64 in bf16: one of 500 keys 11.4 12.0, 10.2 11.4,
+// 8.1 10.4; of 1000 16.3 12.3, 14.5 11.8, 10.7 10.9; of 2000 25.9 13.5, 22.7 12.9, 16.2 11.9; 16 of 1000 18.6 21.5,
+// 15.6 18.2, 11.9 15.6; 16 of 2000 33.0 34.7, 24.4 22.0, 17.8 19.7; 32 of 2000 51.9 54.5, 29.9 34.5, 27.0 31.5.
+// E4M3 tiles take half the LDS, and two workgroups where bf16 has one: 61 sequences of 1 to 8191 keys 117 us, 129 with one.
 inline AttentionPlan paged_attention_plan(AttentionParams& p, bool e4m3) {
   AttentionPlan plan{};
   attention_shape(p, plan, true);
-  attention_step_plan(p, plan, p.keys > 768, (p.dim <= 64 ? 2 : 1) * (e4m3 ? 2 : 1));
+  // About how many tiles there are: whole ones, or one a sequence.
+  int64_t tiles = p.batch < p.tokens ? p.batch : p.tokens;
+  if (tiles < p.tokens / p.tile_tokens) tiles = p.tokens / p.tile_tokens;
+  tiles *= p.head_blocks;
+  const int per_cu = (p.dim <= 64 ? 2 : 1) * (e4m3 ? 2 : 1);
+  attention_step_plan(p, plan, p.keys > (2 * tiles < compute_units() * per_cu ? 768 : 1536), per_cu);
+  if (plan.join) {
+    // A join of 256 threads takes 16 / rows segments of a tile at a time, one of 1024 four times as many, but its
+    // grid takes longer to start: 128 sequences of 1000 keys in E4M3 58 and 62 us, 15 of four tokens 25.8 and 23.1.
+    const int64_t each = (p.tokens + p.batch) / (p.batch + 1);
+    int64_t rows = 1;
+    while (rows < 16 && rows < each * p.heads_per_tile) rows *= 2;
+    if (plan.grid * rows <= 64 * tiles) plan.join = 2;
+  }
   return plan;
 }
 

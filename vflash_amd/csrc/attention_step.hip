@@ -298,8 +298,8 @@ __global__ void __launch_bounds__(256, 1) attention_step(const AttentionParams p
 // The sum over a tile's segments: out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s.  Workgroup b
 // takes the tile that workgroup b of attention_step began and did not end.  Thread t: d 4 (t % 16) and
 // 64 more, one row, every groups-th segment under a maximum of its own; the groups meet in LDS.
-template <bool F16, bool PAGED>
-__global__ void __launch_bounds__(1024) attention_step_join(const AttentionParams p) {
+template <bool F16, bool PAGED, int THREADS>
+__global__ void __launch_bounds__(THREADS) attention_step_join(const AttentionParams p) {
   const AttentionLine line = attention_line<PAGED>(p, gridDim.x);
   const int part = blockIdx.x >> (line.xcds == 8 ? 3 : 0);
   const uint32_t begin = part * line.quota, stop = min(begin + line.quota, line.end);
@@ -313,9 +313,9 @@ __global__ void __launch_bounds__(1024) attention_step_join(const AttentionParam
   const int tokens = min(p.tile_tokens, seg.it.seq.nq - seg.it.tile * p.tile_tokens);
   const int rows = min(16, tokens * p.heads_per_tile);
   const int pow = rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 4 ? 4 : rows <= 8 ? 8 : 16;
-  const int groups = min(16, 64 / pow);
+  const int groups = min(16, THREADS / 16 / pow);
   const int e = (int)threadIdx.x & 15, r = (int)threadIdx.x / 16 % pow, sg = (int)threadIdx.x / 16 / pow;
-  __shared__ float sums[64][132];
+  __shared__ float sums[THREADS / 16][132];
   float top = VFA_LOWEST, l = 0;
   v4f x[2] = {v4f{}, v4f{}};
 #pragma unroll 4
@@ -361,14 +361,16 @@ __global__ void __launch_bounds__(1024) attention_step_join(const AttentionParam
 }
 
 template <bool F16, int STORE>
-static void launch_step(const AttentionParams& p, int grid, bool join, hipStream_t s) {
+static void launch_step(const AttentionParams& p, int grid, int join, hipStream_t s) {
   const dim3 g((unsigned)grid), b(256);
   if (p.dim <= 64) attention_step<F16, 64, STORE><<<g, b, 0, s>>>(p);
   else attention_step<F16, 128, STORE><<<g, b, 0, s>>>(p);
-  if (join) attention_step_join<F16, STORE != kStoreRows><<<g, dim3(1024), 0, s>>>(p);
+  if (join == 1) attention_step_join<F16, STORE != kStoreRows, 1024><<<g, dim3(1024), 0, s>>>(p);
+  if constexpr (STORE != kStoreRows)
+    if (join == 2) attention_step_join<F16, true, 256><<<g, dim3(256), 0, s>>>(p);
 }
 
-void launch_attention_step(const AttentionParams& p, bool f16, AttentionStore store, int grid, bool join, hipStream_t s) {
+void launch_attention_step(const AttentionParams& p, bool f16, AttentionStore store, int grid, int join, hipStream_t s) {
   auto of = [&](auto stored) {
     if (f16) launch_step<true, stored>(p, grid, join, s);
     else launch_step<false, stored>(p, grid, join, s);

@@ -9,8 +9,11 @@
 // a 64-bit integer product, right for every 64-bit position, and its upper 32 bits are the phase (2^-33 of a turn
 // off at most, 7e-10 rad).  No table of cosines is read.
 //
-// Bound by the copy: each value is read and written once.  A workgroup takes one token, forms the sines and
-// cosines of its pairs once in LDS for all heads, and its first loads are in flight meanwhile.
+// Bound by the copy: each value is read and written once.  A workgroup is one wave and takes one token, whose sines and
+// cosines it forms once in LDS, a lane a pair, for all heads.  What counts is how many tokens are on their way: 32
+// workgroups a CU, by at most 64 registers.  32760 tokens of 80 heads of 128: 265 us, 5.1 TB/s; appending 9200 tokens of 36
+// heads, us in waves of 64 registers: one 43, two a workgroup 45, four 51 (and 60 with 67 registers, of which a CU
+// holds 28); with four heads a lane loaded ahead (91 registers) 70.
 #include "quant_ops.h"
 #include "rotary.h"
 
@@ -20,8 +23,15 @@ namespace vfa {
 
 namespace {
 
-constexpr int RT_THREADS = 256;
+constexpr int RT_THREADS = 64;
 constexpr int RT_PAIRS = 128;  // at most
+
+// row_divisor for heads that share a wave: fast where all of them are.
+__device__ __forceinline__ RowDivisor heads_divisor(float s, float amax) {
+  RowDivisor d{s, 1.0f / s, false};
+  d.fast = __builtin_amdgcn_ballot_w64(!(amax <= 3.40282347e38f && s >= 0x1p-72f && s <= 3.40282347e38f)) == 0;
+  return d;
+}
 
 template <bool F16>
 __device__ __forceinline__ void widen8(v4i w, float (&x)[8]) {
@@ -55,7 +65,7 @@ __device__ __forceinline__ v4i narrow8(const float (&x)[8]) {
 // One token, the heads of blockIdx.z: 2^lanes_shift lanes a head, eight d a lane.  Heads [0, heads) are q's,
 // [heads, heads + key_heads) k's and, with a cache, as many of v's.
 template <bool F16>
-__global__ void __launch_bounds__(RT_THREADS) rotate_heads(const RotateParams p, int lanes_shift, int heads_per_group) {
+__global__ void __launch_bounds__(RT_THREADS, 8) rotate_heads(const RotateParams p, int lanes_shift, int heads_per_group) {
   __shared__ float cosines[RT_PAIRS], sines[RT_PAIRS];
   const int64_t token = grid_row();
   if (token >= p.tokens) return;
@@ -133,18 +143,25 @@ __global__ void __launch_bounds__(RT_THREADS) rotate_heads(const RotateParams p,
       if (live && position >= 0) *reinterpret_cast<v4i*>(p.cache.values + 2 * (slot * p.dim + d)) = narrow8<F16>(x);
       continue;
     }
-    // E4M3: the scale of the row quantizer, from the unrounded values.
+    // E4M3: the scale and the quotients of the row quantizer, from the unrounded values.
     float top = 0;
-    static_for<8>([&](auto i) { top = nan_max(top, fabsf(x[i])); });
+    static_for<8>([&](auto j) { top = nan_max(top, fabsf(x[j])); });
     for (int o = 1; o < lanes; o <<= 1) top = nan_max(top, __shfl_xor(top, o, 64));
-    const float scale = row_scale(top);
-    uint32_t c[8];
-    static_for<8>([&](auto i) { c[i] = quant1(x[i], scale); });
+    const RowDivisor by = heads_divisor(row_scale(top), top);
+    uint2 codes;
+    if (by.fast) {
+      float q[8];
+      static_for<8>([&](auto j) { q[j] = clamped_row_quotient<true>(x[j], by); });
+      codes.x = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false), true);
+      codes.y = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[6], q[7], __builtin_amdgcn_cvt_pk_fp8_f32(q[4], q[5], 0, false), true);
+    } else {
+      uint32_t code[8];
+      static_for<8>([&](auto j) { code[j] = quant1(x[j], by.s); });
+      codes = make_uint2(code[0] | code[1] << 8 | code[2] << 16 | code[3] << 24, code[4] | code[5] << 8 | code[6] << 16 | code[7] << 24);
+    }
     if (position < 0) continue;
-    if (live)
-      *reinterpret_cast<uint2*>(p.cache.values + slot * p.dim + d) =
-          make_uint2(c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24, c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24);
-    if (d == 0) p.cache.scales[slot] = scale;
+    if (live) *reinterpret_cast<uint2*>(p.cache.values + slot * p.dim + d) = codes;
+    if (d == 0) p.cache.scales[slot] = by.s;
   }
 }
 
@@ -154,9 +171,12 @@ hipError_t launch_rotate(const RotateParams& p, hipStream_t s) {
   int lanes_shift = 0;
   while ((8 << lanes_shift) < p.dim) ++lanes_shift;
   const int all = (p.q_out ? p.heads : 0) + (p.cache.values ? 2 : 1) * p.key_heads;
-  const int rows = RT_THREADS >> lanes_shift;  // heads at a time
-  int per = all;
-  if (p.tokens < 4 * compute_units()) per = rows;
+  // Few tokens are spread over more workgroups, up to twice what the GPU holds.
+  const int rows = RT_THREADS >> lanes_shift, times = (all + rows - 1) / rows;  // heads at a time
+  int64_t parts = 64 * (int64_t)compute_units() / p.tokens;
+  if (parts > 1024) parts = 1024;
+  parts = parts < 1 ? 1 : parts > times ? times : parts;
+  const int per = (times + (int)parts - 1) / (int)parts * rows;
   dim3 grid = row_grid(p.tokens);
   grid.z = (unsigned)((all + per - 1) / per);
   if (p.f16) rotate_heads<true><<<grid, RT_THREADS, 0, s>>>(p, lanes_shift, per);
