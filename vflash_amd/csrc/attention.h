@@ -376,13 +376,18 @@ __device__ __forceinline__ uint32_t attention_units_of(const AttentionLine& l, c
   return max(1u, ((uint32_t)s.nk + (1u << l.unit_shift) - 1) >> l.unit_shift);
 }
 
+// Over a paged cache, one token a sequence and whole sequences: unit i of a head block is sequence i.
+__device__ __forceinline__ bool attention_direct(const AttentionParams& p) { return !p.q_offsets && p.unit_shift == 31; }
+
 template <bool PAGED = false>
 __device__ __forceinline__ AttentionLine attention_line(const AttentionParams& p, int grid) {
   const int lane = (int)threadIdx.x & 63;
   AttentionLine l{};
   l.unit_shift = p.unit_shift;
   int reached = 0;
-  for (int64_t base = 0; base < p.batch + 2; base += 64) {
+  const bool direct = PAGED && attention_direct(p);
+  if (direct) l.units = (uint32_t)p.batch;
+  for (int64_t base = 0; base < p.batch + 2 && !direct; base += 64) {
     l.mine = attention_sequence<PAGED>(p, base, reached);
     int sum;
     wave_scan((int)(attention_tiles_of(p, l.mine) * attention_units_of(l, l.mine)), lane, sum);
@@ -405,6 +410,13 @@ __device__ __forceinline__ AttentionSegment attention_segment(const AttentionPar
   AttentionSegment g{};
   const uint32_t local = attention_quotient(pos, line.units), x = pos - local * line.units;
   g.it.head_block = line.xcds == 8 ? (b & 7) + 8 * (int)local : (int)local;
+  if (PAGED && attention_direct(p)) {
+    const int64_t keys = p.cache.lengths[x];
+    g.it.seq = AttentionSeq{(int)x, (int)x, 1, keys < 0 ? 0 : keys < p.keys ? (int)keys : p.keys};
+    g.of = g.count = 1;
+    g.it.live = true;
+    return g;
+  }
   uint32_t before = 0;
   int reached = 0;
   for (int64_t base = 0; base < n; base += 64) {

@@ -107,16 +107,22 @@ __global__ void __launch_bounds__(256, 1) attention_step(const AttentionParams p
     const int open = min(attention_limit(p, it.seq, min(it.tile * p.tile_tokens, it.seq.nq)), last);
 
     const int drow = lane / L::CHUNKS, dslot = lane % L::CHUNKS;
-    int64_t pages[2] = {-1, -1};  // of the next block's halves
-    auto look = [&](int key0) {
-      if constexpr (PAGED) {
-        if (last <= 0) return;
-        typedef const __attribute__((address_space(4))) int64_t table_t;  // scalar loads, waited for where they are used
-        table_t* row = (table_t*)(uintptr_t)(p.cache.table + (int64_t)it.seq.k0 * p.cache.width);
-        static_for<2>([&](auto h) { pages[h] = row[min(key0 + 16 * h, last - 1) >> p.cache.page_shift]; });
-      }
+    struct Halves {
+      int64_t page[2];
     };
-    auto issue = [&](int buf, int key0) {
+    // The pages of a block's halves, by scalar loads that are waited for where they are used.
+    auto look = [&](int key0) {
+      Halves h{{-1, -1}};
+      if constexpr (PAGED) {
+        if (last > 0) {
+          typedef const __attribute__((address_space(4))) int64_t table_t;
+          table_t* row = (table_t*)(uintptr_t)(p.cache.table + (int64_t)it.seq.k0 * p.cache.width);
+          static_for<2>([&](auto i) { h.page[i] = row[min(key0 + 16 * i, last - 1) >> p.cache.page_shift]; });
+        }
+      }
+      return h;
+    };
+    auto issue = [&](int buf, int key0, const Halves& halves) {
       const int left = last - key0;  // none: every lane reads zeros
       const uint32_t dst = ring_lds + buf * L::SLOT;
       if constexpr (!PAGED) {
@@ -140,10 +146,11 @@ __global__ void __launch_bounds__(256, 1) attention_step(const AttentionParams p
         const uint32_t row_bytes = (uint32_t)p.dim * (E4M3 ? 1 : 2);
         const int64_t head_rows = (int64_t)p.cache.key_heads << p.cache.page_shift;  // from a page's keys to its values
         static_for<2>([&](auto h) {
-          const bool none = (uint64_t)pages[h] >= (uint64_t)p.cache.pages;  // reads zeros
+          const int64_t page = halves.page[h];
+          const bool none = (uint64_t)page >= (uint64_t)p.cache.pages;  // reads zeros
           const uint32_t size = none ? 0 : 0x7fffffffu;
           const int64_t row = none ? 0
-                                   : 2 * pages[h] * head_rows + ((int64_t)key_head << p.cache.page_shift) +
+                                   : 2 * page * head_rows + ((int64_t)key_head << p.cache.page_shift) +
                                          ((key0 + 16 * h) & ((1 << p.cache.page_shift) - 1));
           const uint8_t* at = p.cache.values + row * row_bytes;
           const __amdgpu_buffer_rsrc_t rk = make_rsrc(at, size), rv = make_rsrc(at + head_rows * row_bytes, size);
@@ -168,11 +175,13 @@ __global__ void __launch_bounds__(256, 1) attention_step(const AttentionParams p
     };
     constexpr int STRIDE = L::WAVES * L::KEYS;
     const int start = first + wave * L::KEYS;
-    look(start);
-    static_for<L::NS>([&](auto i) {
-      issue(i, start + i * STRIDE);
-      look(start + (i + 1) * STRIDE);
-    });
+    Halves next;
+    {
+      Halves begun[L::NS];
+      static_for<L::NS>([&](auto i) { begun[i] = look(start + i * STRIDE); });
+      static_for<L::NS>([&](auto i) { issue(i, start + i * STRIDE, begun[i]); });
+      next = look(start + L::NS * STRIDE);
+    }
 
     v4i q[QS];
     static_for<QS>([&](auto s) { q[s] = attention_query(p, it, row, s * 32 + fg * 8); });
@@ -251,8 +260,8 @@ __global__ void __launch_bounds__(256, 1) attention_step(const AttentionParams p
       });
       __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the slot is read
       asm volatile("" ::: "memory");
-      issue(buf, key0 + L::NS * STRIDE);
-      look(key0 + (L::NS + 1) * STRIDE);
+      issue(buf, key0 + L::NS * STRIDE, next);
+      next = look(key0 + (L::NS + 1) * STRIDE);
     }
     l = sum_across32(sum_across16(l));
     wait_vmcnt<0, true>();
