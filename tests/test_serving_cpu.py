@@ -339,13 +339,15 @@ def test_launches(tmp_path):
              ("vflash_paged_attention", arguments(ATTEND)), ("vflash_paged_attention", arguments(ATTEND, scales=P, f16=1)),
              ("vflash_paged_attention", arguments(ATTEND, width=64, workspace=P, workspace_bytes=1 << 30)),
              ("vflash_paged_attention", arguments(ATTEND, tokens=300, batch=300, q_offsets=None, width=128, workspace=P,
-                                                  workspace_bytes=1 << 30))]
+                                                  workspace_bytes=1 << 30)),
+             ("vflash_paged_attention", arguments(ATTEND, tokens=300, batch=300, q_offsets=None))]
     got = launches(tmp_path, calls)
     assert all(status == 0 for status, _ in got)
     kernels = [[(name, grid) for name, grid, _ in done] for _, done in got]
     assert kernels[0] == [("rotate_heads<0>", (4, 1, 1))] and kernels[1] == [("rotate_heads<0>", (4, 1, 10))]
     assert kernels[2] == [("rotate_heads<1>", (1 << 22, 2, 1))]
     assert kernels[3] == [("rotate_heads<0>", (4, 1, 1))] and kernels[4] == [("rotate_heads<0>", (2, 1, 1))]
-    assert [k for k, _ in kernels[5]] == ["attention_step<0,64,1>"] and [k for k, _ in kernels[6]] == ["attention_step<1,64,2>"]
-    assert [k for k, _ in kernels[7]] == ["attention_step<0,64,1>", "attention_step_join<0,1,1024>"]
-    assert [k for k, _ in kernels[8]] == ["attention_step<0,64,1>", "attention_step_join<0,1,256>"]
+    assert [k for k, _ in kernels[5]] == ["attention_step<0,64,1,4>"] and [k for k, _ in kernels[6]] == ["attention_step<1,64,2,4>"]
+    assert [k for k, _ in kernels[7]] == ["attention_step<0,64,1,4>", "attention_step_join<0,1,1024>"]
+    assert [k for k, _ in kernels[8]] == ["attention_step<0,64,1,4>", "attention_step_join<0,1,256>"]
+    assert kernels[9] == [("attention_step<0,64,1,2>", (600, 1, 1))]

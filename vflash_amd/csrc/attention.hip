@@ -244,7 +244,7 @@ __global__ void __launch_bounds__(256) attention_join(const AttentionParams p, i
 }
 
 // ---------------------------------------------------------------------------
-void launch_attention_step(const AttentionParams&, bool, AttentionStore, int, int, hipStream_t);
+void launch_attention_step(const AttentionParams&, bool, AttentionStore, int, int, int, hipStream_t);
 
 namespace {
 
@@ -310,7 +310,7 @@ hipError_t launch_attention(const AttentionParams& params, bool f16, void* works
   const AttentionPlan plan = attention_plan(p);
   attention_memory(p, plan, 20, workspace);
   if (plan.step) {
-    launch_attention_step(p, f16, kStoreRows, (int)plan.grid, (int)plan.join, s);
+    launch_attention_step(p, f16, kStoreRows, (int)plan.grid, 4, (int)plan.join, s);
     return hipGetLastError();
   }
   if (f16) launch_tiles<true>(p, plan.grid, s);
@@ -329,7 +329,8 @@ hipError_t launch_paged_attention(const AttentionParams& params, bool f16, void*
   // Tiles of 16 follow the maximum once it is 2^8 above: no shift for more, so that weights times the factors of small
   // E4M3 values stay above bf16's subnormals.
   attention_memory(p, plan, (int)kAttentionSlack, workspace);
-  launch_attention_step(p, f16, p.cache.scales ? kStoreE4M3 : kStorePages, (int)plan.grid, (int)plan.join, s);
+  launch_attention_step(p, f16, p.cache.scales ? kStoreE4M3 : kStorePages, (int)plan.grid, plan.waves, (int)plan.join,
+                        s);
   return hipGetLastError();
 }
 

@@ -19,11 +19,11 @@
 
 namespace vfa {
 
-template <int DP, int STORE>
+template <int DP, int STORE, int W>
 struct AttentionSteps {
   static constexpr bool E4M3 = STORE == kStoreE4M3;
   static constexpr int PITCH = (DP <= 64 ? 64 : 128) * (E4M3 ? 1 : 2), CHUNKS = PITCH / 16, ROWS = 1024 / PITCH;
-  static constexpr int KEYS = 32, TILE = KEYS * PITCH, SLOT = 2 * TILE + (E4M3 ? 512 : 0), WAVES = 4;
+  static constexpr int KEYS = 32, TILE = KEYS * PITCH, SLOT = 2 * TILE + (E4M3 ? 512 : 0), WAVES = W;
   static constexpr int NS = 2;
   static constexpr int DMA = 2 * TILE / 1024 + (E4M3 ? 2 : 0);  // instructions per stage
   static constexpr int ACC = DP * 4 + 16;  // bytes of a row's sums in LDS
@@ -75,9 +75,9 @@ __device__ __forceinline__ void lds_dma4(__amdgpu_buffer_rsrc_t r, uint32_t lds_
                : "m0");
 }
 
-template <bool F16, int DP, int STORE>
-__global__ void __launch_bounds__(256, 1) attention_step(const AttentionParams p) {
-  using L = AttentionSteps<DP, STORE>;
+template <bool F16, int DP, int STORE, int W>
+__global__ void __launch_bounds__(64 * W, 1) attention_step(const AttentionParams p) {
+  using L = AttentionSteps<DP, STORE, W>;
   constexpr bool PAGED = STORE != kStoreRows, E4M3 = L::E4M3;
   constexpr bool W16 = F16 && !E4M3;  // the type of the weights
   constexpr int QS = (DP + 31) / 32, DB = DP / 16;
@@ -275,10 +275,12 @@ __global__ void __launch_bounds__(256, 1) attention_step(const AttentionParams p
       stat[wave][fr][1] = l;
     }
     __syncthreads();
-    // Thread t: row t / 16, the d of t % 16 in runs of four.
-    const int r = (int)threadIdx.x >> 4, e = (int)threadIdx.x & 15;
-    const AttentionRow mine = attention_row(p, it, r);
-    if (mine.live) {
+    // Thread t: row t / 16 (and those 4 WAVES further), the d of t % 16 in runs of four.
+    const int e = (int)threadIdx.x & 15;
+    static_for<4 / L::WAVES>([&](auto turn) {
+      const int r = ((int)threadIdx.x >> 4) + turn * (4 * L::WAVES);
+      const AttentionRow mine = attention_row(p, it, r);
+      if (!mine.live) return;
       float top = stat[0][r][0], sum = 0, f[L::WAVES];
       static_for<L::WAVES - 1>([&](auto w) { top = fmaxf(top, stat[w + 1][r][0]); });
       static_for<L::WAVES>([&](auto w) {
@@ -298,7 +300,7 @@ __global__ void __launch_bounds__(256, 1) attention_step(const AttentionParams p
         if (whole) *reinterpret_cast<v2i*>(dst + d) = v2i{pack2<F16>(x[0], x[1]), pack2<F16>(x[2], x[3])};
         else *reinterpret_cast<v4f*>(p.part + at * p.dim + d) = x;
       }
-    }
+    });
     pos += seg.count;
     if (pos < stop) __syncthreads();  // the sums are read: the rings may be filled again
   }
@@ -369,24 +371,29 @@ __global__ void __launch_bounds__(THREADS) attention_step_join(const AttentionPa
   });
 }
 
-template <bool F16, int STORE>
+template <bool F16, int STORE, int W>
 static void launch_step(const AttentionParams& p, int grid, int join, hipStream_t s) {
-  const dim3 g((unsigned)grid), b(256);
-  if (p.dim <= 64) attention_step<F16, 64, STORE><<<g, b, 0, s>>>(p);
-  else attention_step<F16, 128, STORE><<<g, b, 0, s>>>(p);
+  const dim3 g((unsigned)grid), b(64 * W);
+  if (p.dim <= 64) attention_step<F16, 64, STORE, W><<<g, b, 0, s>>>(p);
+  else attention_step<F16, 128, STORE, W><<<g, b, 0, s>>>(p);
   if (join == 1) attention_step_join<F16, STORE != kStoreRows, 1024><<<g, dim3(1024), 0, s>>>(p);
   if constexpr (STORE != kStoreRows)
     if (join == 2) attention_step_join<F16, true, 256><<<g, dim3(256), 0, s>>>(p);
 }
 
-void launch_attention_step(const AttentionParams& p, bool f16, AttentionStore store, int grid, int join, hipStream_t s) {
-  auto of = [&](auto stored) {
-    if (f16) launch_step<true, stored>(p, grid, join, s);
-    else launch_step<false, stored>(p, grid, join, s);
+void launch_attention_step(const AttentionParams& p, bool f16, AttentionStore store, int grid, int waves, int join,
+                           hipStream_t s) {
+  auto of = [&](auto stored, auto w) {
+    if (f16) launch_step<true, stored, w>(p, grid, join, s);
+    else launch_step<false, stored, w>(p, grid, join, s);
   };
-  if (store == kStoreE4M3) of(std::integral_constant<int, kStoreE4M3>{});
-  else if (store == kStorePages) of(std::integral_constant<int, kStorePages>{});
-  else of(std::integral_constant<int, kStoreRows>{});
+  auto paged = [&](auto stored) {
+    if (waves == 2) of(stored, std::integral_constant<int, 2>{});
+    else of(stored, std::integral_constant<int, 4>{});
+  };
+  if (store == kStoreE4M3) paged(std::integral_constant<int, kStoreE4M3>{});
+  else if (store == kStorePages) paged(std::integral_constant<int, kStorePages>{});
+  else of(std::integral_constant<int, kStoreRows>{}, std::integral_constant<int, 4>{});
 }
 
 }  // namespace vfa

@@ -39,11 +39,15 @@ __device__ __forceinline__ int rank_of(const RequestAdapterParams& p, int adapte
 __device__ __forceinline__ RequestItem request_find(const RequestAdapterParams& p, int index, int* rows) {
   const int lane = (int)threadIdx.x & 63;
   int mine = -2, rank = 0;  // no row
+  // The ranks of up to 64 adapters come with the indices instead of after them.
+  const bool few = p.adapters <= 64;
+  const int ranks = few && lane < p.adapters ? rank_of(p, lane) : 0;
   if (lane < p.rows) {
     const int64_t i = p.index[lane];
     mine = (uint64_t)i < (uint64_t)p.adapters ? (int)i : -1;
-    if (mine >= 0) rank = rank_of(p, mine);
+    if (mine >= 0 && !few) rank = rank_of(p, mine);
   }
+  if (few) rank = __shfl(ranks, max(mine, 0), 64);
   uint64_t left = __builtin_amdgcn_ballot_w64(mine != -2);
   while (left) {
     const int first = __builtin_ctzll(left), a = __builtin_amdgcn_readlane(mine, first);
@@ -53,7 +57,7 @@ __device__ __forceinline__ RequestItem request_find(const RequestAdapterParams& 
       // Lane l of the adapter's rows goes to its place among them.
       const int place = __popcll(same & ((uint64_t(1) << lane) - 1)) - index * p.item_rows;
       if (mine == a && place >= 0 && place < p.item_rows) rows[place] = lane;
-      return RequestItem{a, min(p.item_rows, count - index * p.item_rows), __builtin_amdgcn_readlane(rank, first)};
+      return RequestItem{a, min(p.item_rows, count - index * p.item_rows), a < 0 ? 0 : __builtin_amdgcn_readlane(rank, first)};
     }
     index -= items;
     left &= ~same;
