@@ -525,8 +525,8 @@ int vflash_paged_append(const void* q, int64_t q_ts, int64_t q_hs, const void* k
                         int64_t width, const int64_t* lengths, int64_t batch, void* q_out, void* stream);
 
 /*
- * Attention of new tokens, one or a few a sequence, over a paged cache that holds them already: vflash_packed_attention,
- * causal, with the keys and values of vflash_paged_append.  No reference counterpart.
+ * Attention of new tokens over a paged cache that holds them already: vflash_packed_attention, causal, with the keys and
+ * values of vflash_paged_append.  No reference counterpart.
  *   q_offsets, values, scales, table, lengths, batch as there; out as vflash_packed_attention
  *   With scales, a key's factor multiplies its score and a value's its weight before that is rounded to bf16.
  * Lengths are clamped to the table.  Keys on a page outside [0, pages) count as keys and values of zeros.  Nothing

@@ -179,6 +179,8 @@ def test_positions_of_a_model_s_own(dev):
 
 
 # ---------------------------------------------------------------------------
+PROMPTS = [([200], [200]), ([129], [1000]), ([0, 150, 1, 300], [0, 400, 77, 300]), ([700], [900]), ([40, 500, 33], [40, 2000, 500]),
+           ([3] * 70 + [300], [9] * 70 + [1100])]
 ATTENDS = [([1], [1]), ([1], [77]), ([1, 1, 1], [31, 32, 33]), ([1] * 5, [0, 1, 127, 129, 2000]), ([1], [5000]), ([2, 3], [300, 3]),
            ([5, 1], [5, 900]), ([0, 4, 0, 1], [0, 4, 7, 129]), ([40], [17]), ([63], [130]), ([1] * 70, list(range(70)))]
 
@@ -187,7 +189,7 @@ ATTENDS = [([1], [1]), ([1], [77]), ([1, 1, 1], [31, 32, 33]), ([1] * 5, [0, 1, 
     (8, 2, 128, BF16, BF16, 16), (3, 3, 64, F16, F16, 64), (7, 1, 96, BF16, BF16, 32), (10, 2, 80, F16, F16, 16),
     (8, 2, 128, BF16, E4M3, 16), (32, 8, 128, F16, E4M3, 64), (4, 4, 64, BF16, E4M3, 16), (7, 1, 96, F16, E4M3, 128),
     (10, 2, 80, BF16, E4M3, 32)])
-@pytest.mark.parametrize("new,lengths", ATTENDS, ids=lambda v: "-".join(map(str, v[:6])))
+@pytest.mark.parametrize("new,lengths", ATTENDS + PROMPTS, ids=lambda v: "-".join(map(str, v[:6])))
 def test_attention(dev, new, lengths, heads, kv, dim, dtype, store, page):
     cache, table = pool(dev, lengths, page, kv, dim, store, seed=len(lengths))
     q = make(dev, sum(new), heads, dim, dtype=dtype, std=2.0)
@@ -200,9 +202,10 @@ def test_attention(dev, new, lengths, heads, kv, dim, dtype, store, page):
 def test_head_dimensions(dev, dim):
     for dtype, store in ((BF16, BF16), (F16, F16)) + (((BF16, E4M3), (F16, E4M3)) if dim % 16 == 0 else ()):
         cache, table = pool(dev, [45, 900], 16, 2, dim, store)
-        q = make(dev, 2, 4, dim, dtype=dtype, std=2.0)
-        got = paged_attention(q, cache, table, torch.tensor([45, 900], device=dev))
-        attended(cache, q, table, [45, 900], None, got)
+        n = torch.tensor([45, 900], device=dev)
+        for new in ([1, 1], [40, 130]):
+            q, qo = make(dev, sum(new), 4, dim, dtype=dtype, std=2.0), offsets(new, dev)
+            attended(cache, q, table, [45, 900], qo, paged_attention(q, cache, table, n, q_offsets=qo))
 
 
 @pytest.mark.parametrize("page", [16, 32, 64, 256, 1024, 4096])
@@ -210,22 +213,24 @@ def test_head_dimensions(dev, dim):
 def test_pages(dev, page, store):
     lengths = [1, page - 1, page, page + 1, 3 * page + 5, 700]
     cache, table = pool(dev, lengths, page, 2, 64, store, seed=page)
-    q = make(dev, 6, 4, 64, std=2.0)
-    got = paged_attention(q, cache, table, torch.tensor(lengths, device=dev))
-    attended(cache, q, table, lengths, None, got)
+    n = torch.tensor(lengths, device=dev)
+    for new in ([1] * 6, [1, 15, page, 100, 70, 300]):
+        q, qo = make(dev, sum(new), 4, 64, std=2.0), offsets(new, dev)
+        attended(cache, q, table, lengths, qo, paged_attention(q, cache, table, n, q_offsets=qo))
 
 
 @pytest.mark.parametrize("heads,kv", [(1, 1), (16, 1), (17, 1), (40, 1), (16, 16), (24, 8), (5, 5)])
 def test_groups(dev, heads, kv):
     for store in (BF16, E4M3):
         cache, table = pool(dev, [3, 400, 1290], 32, kv, 64, store)
-        q = make(dev, 3, heads, 64, std=2.0)
-        got = paged_attention(q, cache, table, torch.tensor([3, 400, 1290], device=dev))
-        attended(cache, q, table, [3, 400, 1290], None, got)
+        n = torch.tensor([3, 400, 1290], device=dev)
+        for new in ([1, 1, 1], [2, 90, 40]):
+            q, qo = make(dev, sum(new), heads, 64, std=2.0), offsets(new, dev)
+            attended(cache, q, table, [3, 400, 1290], qo, paged_attention(q, cache, table, n, q_offsets=qo))
 
 
 @pytest.mark.parametrize("store", [BF16, F16, E4M3])
-@pytest.mark.parametrize("nq,n", [(1, 33), (1, 640), (1, 5000), (3, 16000), (1, 16383)])
+@pytest.mark.parametrize("nq,n", [(1, 33), (1, 640), (1, 5000), (3, 16000), (1, 16383), (130, 1100), (300, 4000)])
 def test_every_key_counts_once(dev, nq, n, store):
     # Queries of zeros weigh all keys alike, and v marks key j by d = j % 128, a quarter of the keys for each
     # key head: an output is a count over n, of at most 32 keys, so that one key more or less is 1 / 32 of it.
@@ -265,9 +270,9 @@ def test_what_lies_past_a_sequence_is_not_read(dev):
     for store in (BF16, E4M3):
         lengths = [5, 70, 1001]
         cache, table = pool(dev, lengths, 32, 2, 64, store, width=40)
-        q = make(dev, 3, 4, 64, std=2.0)
         n = torch.tensor(lengths, device=dev)
-        want = paged_attention(q, cache, table, n)
+        calls = [(make(dev, sum(new), 4, 64, std=2.0), offsets(new, dev)) for new in ([1, 1, 1], [5, 70, 200])]
+        wants = [paged_attention(q, cache, table, n, q_offsets=qo) for q, qo in calls]
         own = torch.zeros(cache.values.shape[0], 32, dtype=torch.bool, device=dev)
         for row, m in zip(table.tolist(), lengths):
             for i in range(m):
@@ -276,14 +281,15 @@ def test_what_lies_past_a_sequence_is_not_read(dev):
         cache.values.view(torch.uint8).view(*foreign.shape, -1)[foreign] = 0xff  # NaN in each type
         if cache.scales is not None:
             cache.scales[foreign] = torch.nan
-        assert torch.equal(paged_attention(q, cache, table, n), want)
+        for (q, qo), want in zip(calls, wants):
+            assert torch.equal(paged_attention(q, cache, table, n, q_offsets=qo), want)
 
 
 def test_pages_that_do_not_exist_count_as_zeros(dev):
     for store in (BF16, E4M3):
         cache, table = pool(dev, [100, 1300], 16, 2, 64, store)
         n = torch.tensor([100, 1300], device=dev)
-        q = make(dev, 2, 4, 64, std=2.0)
+        calls = [(make(dev, sum(new), 4, 64, std=2.0), offsets(new, dev)) for new in ([1, 1], [80, 150])]
         clean = PagedCache(torch.cat((cache.values.view(torch.uint8), torch.zeros_like(cache.values[:1]).view(torch.uint8)))
                            .view(cache.values.dtype), None if cache.scales is None else
                            torch.cat((cache.scales, torch.zeros_like(cache.scales[:1]))))
@@ -291,16 +297,19 @@ def test_pages_that_do_not_exist_count_as_zeros(dev):
             table[0, 3] = table[1, 0] = table[1, 44] = bad
             zeros = table.clone()
             zeros[zeros == bad] = cache.values.shape[0]
-            assert torch.equal(paged_attention(q, cache, table, n), paged_attention(q, clean, zeros, n)), bad
+            for q, qo in calls:
+                got, want = (paged_attention(q, c, t, n, q_offsets=qo) for c, t in ((cache, table), (clean, zeros)))
+                assert torch.equal(got, want), bad
 
 
 def test_lengths_outside_the_table(dev):
     cache, table = pool(dev, [64, 1024], 16, 2, 64, BF16)
-    q = make(dev, 2, 4, 64)
-    full = paged_attention(q, cache, table, torch.tensor([0, 1024], device=dev))
-    for n in ([-1, 1025], [-(1 << 63), 1 << 40], [0, (1 << 63) - 1]):
-        assert torch.equal(paged_attention(q, cache, table, torch.tensor(n, device=dev)), full)
-    assert not full[0].any()
+    for new in ([1, 1], [40, 200]):
+        q, qo = make(dev, sum(new), 4, 64), offsets(new, dev)
+        full = paged_attention(q, cache, table, torch.tensor([0, 1024], device=dev), q_offsets=qo)
+        for n in ([-1, 1025], [-(1 << 63), 1 << 40], [0, (1 << 63) - 1]):
+            assert torch.equal(paged_attention(q, cache, table, torch.tensor(n, device=dev), q_offsets=qo), full)
+        assert not full[:new[0]].any()
 
 
 def test_offsets_that_decrease_or_lie_outside(dev):
@@ -308,7 +317,7 @@ def test_offsets_that_decrease_or_lie_outside(dev):
     rng = random.Random(4)
     rotary = Rotary(rotary_frequencies(64), device=dev)
     for i in range(24):
-        batch, tokens, page, width = rng.choice((1, 3, 70)), rng.randint(1, 60), 16, 60
+        batch, tokens, page, width = rng.choice((1, 3, 70)), rng.randint(1, 60) if i % 2 else rng.randint(200, 900), 16, 60
         whole = torch.full((40, 2, 2, page, 64), 7.0, device=dev, dtype=BF16)
         cache = PagedCache(whole[10:30])
         table = torch.randint(-3, 24, (batch, width), device=dev)
@@ -334,9 +343,10 @@ def test_scores_and_scales_far_from_one(dev, store):
             cache.scales[:, 1] *= size
         else:
             cache.values[:, 1] *= size
-        q = make(dev, 2, 4, 128, std=std)
-        for scale in (0.01, 0.3):
-            attended(cache, q, table, lengths, None, paged_attention(q, cache, table, n, scale=scale), scale)
+        for new in ([1, 1], [20, 150]):
+            q, qo = make(dev, sum(new), 4, 128, std=std), offsets(new, dev)
+            for scale in (0.01, 0.3):
+                attended(cache, q, table, lengths, qo, paged_attention(q, cache, table, n, q_offsets=qo, scale=scale), scale)
 
 
 def test_cache_past_32_bit_offsets(dev):
@@ -348,9 +358,9 @@ def test_cache_past_32_bit_offsets(dev):
     lengths, n = torch.tensor([3000], device=dev), 3000
     k, v = make(dev, n, kv, dim), make(dev, n, kv, dim, seed=1)
     paged_append(cache, k, v, table, lengths, q_offsets=offsets([n], dev))
-    q = make(dev, 1, 16, dim, std=2.0)
-    got = paged_attention(q, cache, table, lengths)
-    check(got, q, k, v, offsets([1], dev), offsets([n], dev), causal=True)
+    for new in (1, 60):
+        q, qo = make(dev, new, 16, dim, std=2.0), offsets([new], dev)
+        check(paged_attention(q, cache, table, lengths, q_offsets=qo), q, k, v, qo, offsets([n], dev), causal=True)
 
 
 def test_layouts_of_q(dev):
@@ -373,7 +383,7 @@ def test_prompts_then_single_tokens(dev, dtype, store):
     cache, table = pool(dev, total, page, kv, dim, store)
     tokens = [make(dev, n, heads + 2 * kv, dim, dtype=dtype, seed=i) for i, n in enumerate(total)]
     done, outs = [0, 0, 0], [[], [], []]
-    for step in ([60, 20, 1150], [1, 1, 1], [4, 0, 7], [1, 1, 1], [4, 11, 41]):
+    for step in ([60, 20, 500], [0, 0, 650], [1, 1, 1], [4, 0, 7], [1, 1, 1], [4, 11, 41]):
         parts = [t[a:a + m] for t, a, m in zip(tokens, done, step)]
         done = [a + m for a, m in zip(done, step)]
         q, k, v = torch.cat(parts).split((heads, kv, kv), 1)
@@ -425,20 +435,40 @@ def test_a_captured_step_replays_other_lengths_and_pages(dev):
             assert torch.equal(twin.values.view(torch.uint8), cache.values.view(torch.uint8))
 
 
+def test_a_captured_prompt_replays_other_lengths(dev):
+    for store in (BF16, E4M3):
+        cache, table = pool(dev, [1000] * 3, 16, 2, 64, store)
+        q, n, qo = make(dev, 300, 8, 64), torch.tensor([1000, 100, 30], device=dev), offsets([150, 100, 30], dev)
+        paged_attention(q, cache, table, n, q_offsets=qo)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = paged_attention(q, cache, table, n, q_offsets=qo)
+        for new, lengths in (([150, 100, 30], [1000, 100, 30]), ([300, 0, 0], [300, 9, 1000]), ([1, 298, 1], [700, 900, 1])):
+            n.copy_(torch.tensor(lengths, device=dev))
+            qo.copy_(offsets(new, dev))
+            q.normal_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, paged_attention(q, cache, table, n, q_offsets=qo))
+
+
 def test_repeated_calls_and_other_streams_agree(dev):
     for store in (BF16, E4M3):
         lengths = [5000, 20, 900]
         cache, table = pool(dev, lengths, 64, 2, 128, store)
-        q, n = make(dev, 3, 8, 128, std=2.0), torch.tensor(lengths, device=dev)
-        want = paged_attention(q, cache, table, n)
-        side = torch.cuda.Stream(dev)
-        side.wait_stream(torch.cuda.current_stream(dev))
-        with torch.cuda.stream(side):
-            got = paged_attention(q, cache, table, n)
-        torch.cuda.current_stream(dev).wait_stream(side)
-        assert torch.equal(got, want)
-        for _ in range(5):
-            assert torch.equal(paged_attention(q, cache, table, n), want)
+        n = torch.tensor(lengths, device=dev)
+        for new in ([1, 1, 1], [300, 4, 90]):
+            q, qo = make(dev, sum(new), 8, 128, std=2.0), offsets(new, dev)
+            want = paged_attention(q, cache, table, n, q_offsets=qo)
+            side = torch.cuda.Stream(dev)
+            side.wait_stream(torch.cuda.current_stream(dev))
+            with torch.cuda.stream(side):
+                got = paged_attention(q, cache, table, n, q_offsets=qo)
+            torch.cuda.current_stream(dev).wait_stream(side)
+            assert torch.equal(got, want)
+            for _ in range(5):
+                assert torch.equal(paged_attention(q, cache, table, n, q_offsets=qo), want)
 
 
 def test_native_host_path(dev):

@@ -125,8 +125,10 @@ def test_places(tmp_path, head):
 # tokens, room, sequences, heads, group, dim
 SIZES = {
     "one a sequence": (90, 4096, 90, 8, 4, 128), "XCDs": (70, 2048, 70, 32, 2, 128), "not split": (40, 512, 40, 6, 3, 64),
-    "many": (150, 131072, 150, 4, 4, 64), "several": (90, 4096, 20, 8, 4, 64), "wide group": (9, 4096, 3, 40, 40, 64),
-    "no sequence": (5, 4096, 0, 4, 2, 64),
+    "many": (150, 131072, 150, 4, 4, 64), "several": (90, 4096, 20, 8, 4, 64), "wide group": (3, 4096, 3, 40, 40, 64),
+    "tiles, wide group": (9, 4096, 3, 40, 40, 64),
+    "tiles, no sequence": (5, 4096, 0, 4, 2, 64), "tiles": (900, 4096, 2, 8, 8, 128), "tiles, several": (700, 8192, 5, 8, 1, 64),
+    "tiles, many": (3000, 2048, 100, 4, 2, 64), "tiles, not split": (6000, 512, 9, 7, 7, 64),
 }
 
 
@@ -134,6 +136,7 @@ SIZES = {
 def test_paged_schedule(tmp_path, head, size):
     tokens, room, batch, heads, group, dim = size
     text = head.replace("attention_line(p,", "attention_line<true>(p,").replace("attention_segment(p,", "attention_segment<true>(p,")
+    text = text.replace("attention_item<false>(p,", "attention_item<false, true>(p,").replace("attention_item<true>(p,", "attention_item<true, true>(p,")
     text += r"""
 int main() {
   int tokens, keys, heads, group, dim, given, at_end;
@@ -147,14 +150,18 @@ int main() {
     printf("plan %d %d %d %d %d %lld %lld %d\n", plan.step, p.tile_tokens, p.heads_per_tile, p.parts, p.head_blocks,
            (long long)p.slots, (long long)plan.grid, plan.join != 0);
     blocks = (unsigned)plan.grid;
-    wave(steps);
-    if (plan.join) wave(step_joins);
+    wave(plan.step ? steps : tiles);
+    if (plan.join) {
+      blocks = (unsigned)(plan.step ? plan.grid : plan.join);
+      wave(plan.step ? step_joins : joins);
+    }
     printf("end\n");
   }
 }
 """
     program = build(tmp_path, text)
     rng = random.Random(tokens)
+    name = next(k for k, v in SIZES.items() if v == size)
     calls, lines = [], []
     for i in range(6):
         given = tokens != batch or i % 2 == 1
@@ -176,6 +183,7 @@ int main() {
             results[-1][1 if kind == "rows" else 2].append(values)
     assert len(results) == len(calls)
     for (offsets, lengths), (plan, rows, joins) in zip(calls, results):
+        assert plan[0] == (not name.startswith("tiles"))
         # A sequence's number stands where packed attention has its first key; give it room after it.
         for row in rows:
             assert 0 <= row[8] < max(batch, 1) and 0 <= row[9] <= room

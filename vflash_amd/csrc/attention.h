@@ -213,13 +213,13 @@ __device__ __forceinline__ bool attention_place(const AttentionParams& p, uint32
 }
 
 // The unit `index` of the launch: an item, or with JOIN a tile (all its splits).
-template <bool JOIN>
+template <bool JOIN, bool PAGED = false>
 __device__ __forceinline__ AttentionItem attention_find(const AttentionParams& p, uint32_t index) {
   const int lane = (int)threadIdx.x & 63;
   const int64_t n = p.batch + 2;
   int reached = 0, x;
   AttentionItem it{};
-  AttentionSeq mine = attention_sequence(p, 0, reached);
+  AttentionSeq mine = attention_sequence<PAGED>(p, 0, reached);
   auto take = [&](int l) {
     auto pick = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
     it.seq = AttentionSeq{pick(mine.q0), pick(mine.k0), pick(mine.nq), pick(mine.nk)};
@@ -245,7 +245,7 @@ __device__ __forceinline__ AttentionItem attention_find(const AttentionParams& p
   auto each = [&](auto&& f) {  // f(tiles) for every 64 sequences, in `mine`, until it returns true
     reached = 0;
     for (int64_t base = 0; base < n; base += 64) {
-      if (n > 64) mine = attention_sequence(p, base, reached);
+      if (n > 64) mine = attention_sequence<PAGED>(p, base, reached);
       if (f((int)attention_tiles_of(p, mine))) return;
     }
   };
@@ -307,10 +307,10 @@ __device__ __forceinline__ AttentionItem attention_find(const AttentionParams& p
 }
 
 // The same in scalar registers, where the compiler does not see that the search is uniform.
-template <bool JOIN>
+template <bool JOIN, bool PAGED = false>
 __device__ __forceinline__ AttentionItem attention_item(const AttentionParams& p, uint32_t index) {
   auto u = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
-  const AttentionItem f = attention_find<JOIN>(p, index);
+  const AttentionItem f = attention_find<JOIN, PAGED>(p, index);
   AttentionItem it;
   it.seq = AttentionSeq{u(f.seq.q0), u(f.seq.k0), u(f.seq.nq), u(f.seq.nk)};
   it.tile = u(f.tile);

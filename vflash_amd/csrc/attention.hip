@@ -18,7 +18,11 @@
 // products and softmax follow each other, and the others' fill its gaps in part); 24 causal prompts of
 // up to 1023 tokens, 28 heads over 4, 0.126 ms (VALU 0.43, MFMAs 0.30).  Cards differ by 5 %.  Blocks of
 // 32 keys above dimension 64 let three workgroups share a CU, 64 below four.
-#include "attention.h"
+//
+// A paged cache differs in where a wave's part of a tile comes from: rows of one 16 keys, which lie in one page.
+// E4M3 codes go through registers, a tile ahead, and reach LDS as 16-bit numbers (exactly), converted once for
+// all waves; a key's factor multiplies its score, a value's its weight before that is rounded, to bf16.
+#include "attention_codes.h"
 #include "attention_plan.h"
 
 namespace vfa {
@@ -39,14 +43,17 @@ __device__ __forceinline__ int v_swizzle(int r) {
   return PITCH == 256 ? (r & 3) << 2 : (r >> 1 & 1) << 2;
 }
 
-template <bool F16, int DP, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES, DP <= 64 ? 4 : 3) attention_tiles(const AttentionParams p) {
+template <bool F16, int DP, int WAVES, int STORE>
+__global__ void __launch_bounds__(64 * WAVES, (DP <= 64 ? 4 : 3) - (STORE == kStoreE4M3)) attention_tiles(const AttentionParams p) {
   using L = AttentionTiles<DP>;
+  constexpr bool PAGED = STORE != kStoreRows, E4M3 = STORE == kStoreE4M3;
+  constexpr bool W16 = F16 && !E4M3;  // the type of the weights
   constexpr int QS = DP / 16, DB = DP / 32;            // contraction steps, blocks of 32 d
   constexpr int BLOCKS = L::TILE / 1024 / WAVES;       // DMA instructions per wave for K, and for V
   static_assert(L::TILE % (1024 * WAVES) == 0, "DMA blocks");
   __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * L::SLOT];
-  const AttentionItem it = attention_item<false>(p, blockIdx.x);
+  __shared__ float factors[E4M3 ? 2 : 1][2][E4M3 ? L::KEYS : 1];  // of keys and values
+  const AttentionItem it = attention_item<false, PAGED>(p, blockIdx.x);
   if (!it.live) return;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int lane = (int)threadIdx.x & 63;
@@ -68,32 +75,98 @@ __global__ void __launch_bounds__(64 * WAVES, DP <= 64 ? 4 : 3) attention_tiles(
   const int open = min(attention_limit(p, it.seq, wave_first_token), last);
   const int end = min(attention_limit(p, it.seq, wave_last_token), last);
 
-  const uint8_t* kb = reinterpret_cast<const uint8_t*>(p.k + (int64_t)it.seq.k0 * p.k_ts + (int64_t)part_head * p.k_hs);
-  const uint8_t* vb = reinterpret_cast<const uint8_t*>(p.v + (int64_t)it.seq.k0 * p.v_ts + (int64_t)part_head * p.v_hs);
-  const uint32_t kts = (uint32_t)p.k_ts * 2, vts = (uint32_t)p.v_ts * 2;
   // DMA: block i of this wave holds rows (wave * BLOCKS + i) * ROWS + lane / CHUNKS; lane l fills
   // slot l % CHUNKS.  Rows past the keys and chunks past the head read as zeros.
-  const int drow = wave * BLOCKS * L::ROWS + lane / L::CHUNKS, dslot = lane % L::CHUNKS;
-  auto issue = [&](int buf, int key0) {
+  constexpr int WAVE_ROWS = BLOCKS * L::ROWS;
+  static_assert(16 % WAVE_ROWS == 0, "a wave's rows lie in one page");
+  const int drow = wave * WAVE_ROWS + lane / L::CHUNKS, dslot = lane % L::CHUNKS;
+  // Pages: the 16 keys that this wave's rows are some of.
+  const int group = wave * WAVE_ROWS / 16 * 16;
+  const int64_t head_rows = (int64_t)p.cache.key_heads << p.cache.page_shift;  // from a page's keys to its values
+  auto look = [&](int key0) {  // a scalar load, waited for where it is used
+    if constexpr (PAGED) {
+      typedef const __attribute__((address_space(4))) int64_t table_t;
+      if (key0 + group < last)
+        return (int64_t)((table_t*)(uintptr_t)(p.cache.table + (int64_t)it.seq.k0 * p.cache.width))[(key0 + group) >> p.cache.page_shift];
+    }
+    return (int64_t)-1;
+  };
+  // The cache's row of key `key` on `page`, as keys count.
+  auto cache_row = [&](int64_t page, int key) {
+    return 2 * page * head_rows + ((int64_t)part_head << p.cache.page_shift) + (key & ((1 << p.cache.page_shift) - 1));
+  };
+  auto issue = [&](int buf, int key0, int64_t page) {
     const int left = last - key0;
-    const __amdgpu_buffer_rsrc_t rk = make_rsrc(kb + (int64_t)key0 * kts, 0x7fffffffu);
-    const __amdgpu_buffer_rsrc_t rv = make_rsrc(vb + (int64_t)key0 * vts, 0x7fffffffu);
     const uint32_t dst = base_lds + buf * L::SLOT + wave * BLOCKS * 1024;
+    uint32_t kts, vts, from;  // bytes of a row; the first row of the resources
+    __amdgpu_buffer_rsrc_t rk, rv;
+    if constexpr (PAGED) {
+      const bool none = (uint64_t)page >= (uint64_t)p.cache.pages;  // reads zeros
+      const uint8_t* at = p.cache.values + (none ? 0 : cache_row(page, key0 + group) * p.dim * 2);
+      rk = make_rsrc(at, none ? 0 : 0x7fffffffu);
+      rv = make_rsrc(at + head_rows * p.dim * 2, none ? 0 : 0x7fffffffu);
+      kts = vts = (uint32_t)p.dim * 2;
+      from = (uint32_t)group;
+    } else {
+      kts = (uint32_t)p.k_ts * 2;
+      vts = (uint32_t)p.v_ts * 2;
+      from = 0;
+      rk = make_rsrc(reinterpret_cast<const uint8_t*>(p.k + (int64_t)it.seq.k0 * p.k_ts + (int64_t)part_head * p.k_hs) +
+                         (int64_t)key0 * kts, 0x7fffffffu);
+      rv = make_rsrc(reinterpret_cast<const uint8_t*>(p.v + (int64_t)it.seq.k0 * p.v_ts + (int64_t)part_head * p.v_hs) +
+                         (int64_t)key0 * vts, 0x7fffffffu);
+    }
     static_for<BLOCKS>([&](auto i) {
       const int r = drow + i * L::ROWS;
       const int c = dslot ^ k_swizzle<L::PITCH>(r);
-      const uint32_t off = (uint32_t)r * kts + c * 16;
+      const uint32_t off = ((uint32_t)r - from) * kts + c * 16;
       lds_dma16(rk, dst + i * 1024, r < left && c * 8 < p.dim ? off : VFA_OOB);
     });
     static_for<BLOCKS>([&](auto i) {
       const int r = drow + i * L::ROWS;
       const int c = dslot ^ v_swizzle<L::PITCH>(r);
-      const uint32_t off = (uint32_t)r * vts + c * 16;
+      const uint32_t off = ((uint32_t)r - from) * vts + c * 16;
       lds_dma16(rv, dst + L::TILE + i * 1024, r < left && c * 8 < p.dim ? off : VFA_OOB);
     });
   };
+  // E4M3: thread t takes 16 codes of a key and of its value, one of the first threads also a factor.
+  constexpr int CODE_CHUNKS = L::CHUNKS / 2;
+  static_assert(!E4M3 || L::KEYS * CODE_CHUNKS == 64 * WAVES, "a chunk a thread");
+  const int crow = (int)threadIdx.x / CODE_CHUNKS, cchunk = (int)threadIdx.x % CODE_CHUNKS;
+  v4i key_codes, value_codes;
+  float factor;
+  auto fetch = [&](int key0, int64_t page) {
+    key_codes = value_codes = v4i{};
+    factor = 0;
+    if ((uint64_t)page < (uint64_t)p.cache.pages && key0 + crow < last && cchunk * 16 < p.dim) {
+      const uint8_t* at = p.cache.values + cache_row(page, key0 + crow) * p.dim + cchunk * 16;
+      key_codes = *reinterpret_cast<const v4i*>(at);
+      value_codes = *reinterpret_cast<const v4i*>(at + head_rows * p.dim);
+    }
+    const int t = (int)threadIdx.x, key = key0 + t % L::KEYS;
+    if (t < 2 * L::KEYS && key < last) {
+      const int64_t own = p.cache.table[(int64_t)it.seq.k0 * p.cache.width + (key >> p.cache.page_shift)];
+      if ((uint64_t)own < (uint64_t)p.cache.pages) factor = p.cache.scales[cache_row(own, key) + (t < L::KEYS ? 0 : head_rows)];
+    }
+  };
+  auto place = [&](int buf) {
+    uint8_t* at = lds + buf * L::SLOT + crow * L::PITCH;
+    static_for<2>([&](auto h) {
+      const int c = 2 * cchunk + h;
+      *reinterpret_cast<v4i*>(at + ((c ^ k_swizzle<L::PITCH>(crow)) << 4)) = attention_widen<F16>(v2i{key_codes[2 * h], key_codes[2 * h + 1]});
+      *reinterpret_cast<v4i*>(at + L::TILE + ((c ^ v_swizzle<L::PITCH>(crow)) << 4)) =
+          attention_widen<false>(v2i{value_codes[2 * h], value_codes[2 * h + 1]});
+    });
+    const int t = (int)threadIdx.x;
+    if (t < 2 * L::KEYS) factors[buf][t / L::KEYS][t % L::KEYS] = factor;
+  };
 
-  if (first < last) issue(0, first);
+  int64_t next = -1;  // the page of the tile after the one on its way
+  if (first < last) {
+    if constexpr (E4M3) fetch(first, look(first));
+    else issue(0, first, look(first));
+    next = look(first + L::KEYS);
+  }
   v4i q[QS];
   static_for<QS>([&](auto s) { q[s] = attention_query(p, it, row, s * 16 + fh * 8); });
   v16f o[DB];
@@ -111,13 +184,38 @@ __global__ void __launch_bounds__(64 * WAVES, DP <= 64 ? 4 : 3) attention_tiles(
   const uint8_t* vrow = lds + L::TILE + vr * L::PITCH + (lane & 1) * 8;
   const int vsw = v_swizzle<L::PITCH>(vr);  // rows 8 apart share it
 
+  if constexpr (E4M3) {
+    if (first < last) place(0);
+    __syncthreads();
+  }
   for (int key0 = first, buf = 0; key0 < last; key0 += L::KEYS, buf ^= 1) {
-    wait_vmcnt<0, false>();
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_barrier();  // this tile has landed for every wave, and the other buffer is read
-    asm volatile("" ::: "memory");
-    if (key0 + L::KEYS < last) issue(buf ^ 1, key0 + L::KEYS);
-    if (key0 >= end) continue;
+    const bool more = key0 + L::KEYS < last;
+    if constexpr (E4M3) {
+      // This tile's other buffer is written at the end, after the barrier of the one before.
+      if (more) {
+        fetch(key0 + L::KEYS, next);
+        next = look(key0 + 2 * L::KEYS);
+      }
+    } else {
+      wait_vmcnt<0, false>();
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_s_barrier();  // this tile has landed for every wave, and the other buffer is read
+      asm volatile("" ::: "memory");
+      if (more) {
+        issue(buf ^ 1, key0 + L::KEYS, next);
+        next = look(key0 + 2 * L::KEYS);
+      }
+    }
+    auto after = [&] {
+      if constexpr (E4M3) {
+        if (more) place(buf ^ 1);
+        __syncthreads();
+      }
+    };
+    if (key0 >= end) {
+      after();
+      continue;
+    }
     v16f s[L::KB];
     static_for<L::KB>([&](auto kbk) { s[kbk] = v16f{}; });
     static_for<QS>([&](auto st) {
@@ -127,6 +225,11 @@ __global__ void __launch_bounds__(64 * WAVES, DP <= 64 ? 4 : 3) attention_tiles(
         s[kbk] = mfma32<F16>(a, q[st], s[kbk]);
       });
     });
+    if constexpr (E4M3)
+      static_for<4 * L::KB>([&](auto g) {
+        const v4f f = *reinterpret_cast<const v4f*>(&factors[buf][0][8 * g + 4 * fh]);
+        static_for<4>([&](auto r) { s[g / 4][(int)(g % 4 * 4 + r)] *= f[(int)r]; });
+      });
     if (key0 + L::KEYS > open) {  // some row of the wave masks some key
       const int lim = limit - key0 - 4 * fh;
       static_for<L::KB>([&](auto kbk) {
@@ -139,20 +242,27 @@ __global__ void __launch_bounds__(64 * WAVES, DP <= 64 ? 4 : 3) attention_tiles(
     v4i pk[2 * L::KB];
     float sum;
     auto weights = [&](auto far_rows) {
-      const float ref = attention_shift<F16>(p) - attention_top(m, p.c);
+      const float ref = attention_shift<W16>(p) - attention_top(m, p.c);
       sum = 0;
       static_for<2 * L::KB>([&](auto st) {
         static_for<4>([&](auto j) {
           constexpr int r = (st % 2) * 8 + 2 * j;
-          pk[st][(int)j] = pack2<F16>(attention_weight<far_rows>(s[st / 2][r], p.c, m, ref, attention_shift<F16>(p)),
-                                      attention_weight<far_rows>(s[st / 2][r + 1], p.c, m, ref, attention_shift<F16>(p)));
-          sum = attention_sum2<F16>(pk[st][(int)j], sum);
+          const float w0 = attention_weight<far_rows>(s[st / 2][r], p.c, m, ref, attention_shift<W16>(p));
+          const float w1 = attention_weight<far_rows>(s[st / 2][r + 1], p.c, m, ref, attention_shift<W16>(p));
+          if constexpr (E4M3) {
+            const v2f f = *reinterpret_cast<const v2f*>(&factors[buf][1][st / 2 * 32 + 8 * (r / 4) + 4 * fh + r % 4]);
+            pk[st][(int)j] = pack2<W16>(w0 * f[0], w1 * f[1]);
+            sum += w0 + w1;
+          } else {
+            pk[st][(int)j] = pack2<W16>(w0, w1);
+            sum = attention_sum2<W16>(pk[st][(int)j], sum);
+          }
         });
       });
     };
     if (far) weights(std::true_type{});
     else weights(std::false_type{});
-    if (__builtin_amdgcn_ballot_w64(!(sum <= attention_bound<F16>(p)))) {
+    if (__builtin_amdgcn_ballot_w64(!(sum <= attention_bound<W16>(p)))) {
       // The first keys that a row sees, or scores far above those before.
       float mx = s[0][0];
       static_for<16 * L::KB - 1>([&](auto r) { mx = fmaxf(mx, s[(r + 1) / 16][(int)((r + 1) % 16)]); });
@@ -169,9 +279,10 @@ __global__ void __launch_bounds__(64 * WAVES, DP <= 64 ? 4 : 3) attention_tiles(
       static_for<DB>([&](auto db) {
         const uint8_t* src = vrow + buf * L::SLOT + st * 16 * L::PITCH + (((4 * db + vc) ^ vsw) << 4);
         const v2i lo = lds_read_tr16(src), hi = lds_read_tr16(src + 8 * L::PITCH);
-        o[db] = mfma32<F16>(v4i{lo[0], lo[1], hi[0], hi[1]}, pk[st], o[db]);
+        o[db] = mfma32<W16>(v4i{lo[0], lo[1], hi[0], hi[1]}, pk[st], o[db]);
       });
     });
+    after();
   }
   l = sum_across32(l);
 
@@ -212,9 +323,9 @@ __global__ void __launch_bounds__(64 * WAVES, DP <= 64 ? 4 : 3) attention_tiles(
 
 // The sum over a tile's splits: out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s.  A workgroup
 // takes every eighth row of a tile, half a wave a row, four d a lane.
-template <bool F16>
+template <bool F16, bool PAGED>
 __global__ void __launch_bounds__(256) attention_join(const AttentionParams p, int rows) {
-  const AttentionItem it = attention_item<true>(p, blockIdx.x);
+  const AttentionItem it = attention_item<true, PAGED>(p, blockIdx.x);
   if (!it.live || it.splits == 1) return;
   const int d = 4 * ((int)threadIdx.x & 31);
   const int last_token = min(it.seq.nq, (it.tile + 1) * p.tile_tokens) - 1;
@@ -248,18 +359,16 @@ void launch_attention_step(const AttentionParams&, bool, AttentionStore, int, in
 
 namespace {
 
-template <bool F16>
-void launch_tiles(const AttentionParams& p, int64_t grid, hipStream_t s) {
-  const dim3 g((unsigned)grid), b(64 * kTileWaves);
-  if (p.dim <= 32) attention_tiles<F16, 32, kTileWaves><<<g, b, 0, s>>>(p);
-  else if (p.dim <= 64) attention_tiles<F16, 64, kTileWaves><<<g, b, 0, s>>>(p);
-  else if (p.dim <= 96) attention_tiles<F16, 96, kTileWaves><<<g, b, 0, s>>>(p);
-  else attention_tiles<F16, 128, kTileWaves><<<g, b, 0, s>>>(p);
+template <bool F16, int STORE>
+void launch_tiles(const AttentionParams& p, const AttentionPlan& plan, hipStream_t s) {
+  const dim3 g((unsigned)plan.grid), b(64 * kTileWaves);
+  if (p.dim <= 32) attention_tiles<F16, 32, kTileWaves, STORE><<<g, b, 0, s>>>(p);
+  else if (p.dim <= 64) attention_tiles<F16, 64, kTileWaves, STORE><<<g, b, 0, s>>>(p);
+  else if (p.dim <= 96) attention_tiles<F16, 96, kTileWaves, STORE><<<g, b, 0, s>>>(p);
+  else attention_tiles<F16, 128, kTileWaves, STORE><<<g, b, 0, s>>>(p);
+  if (!plan.join) return;
+  attention_join<F16, STORE != kStoreRows><<<dim3((unsigned)plan.join, 8), dim3(256), 0, s>>>(p, plan.rows);
 }
-
-}  // namespace
-
-namespace {
 
 int64_t workspace_of(const AttentionParams& p, const AttentionPlan& plan) { return p.slots * plan.rows * (p.dim + 2) * 4; }
 
@@ -313,24 +422,29 @@ hipError_t launch_attention(const AttentionParams& params, bool f16, void* works
     launch_attention_step(p, f16, kStoreRows, (int)plan.grid, 4, (int)plan.join, s);
     return hipGetLastError();
   }
-  if (f16) launch_tiles<true>(p, plan.grid, s);
-  else launch_tiles<false>(p, plan.grid, s);
-  if (plan.join) {
-    const dim3 g((unsigned)plan.join, 8);
-    if (f16) attention_join<true><<<g, dim3(256), 0, s>>>(p, plan.rows);
-    else attention_join<false><<<g, dim3(256), 0, s>>>(p, plan.rows);
-  }
+  if (f16) launch_tiles<true, kStoreRows>(p, plan, s);
+  else launch_tiles<false, kStoreRows>(p, plan, s);
   return hipGetLastError();
 }
 
 hipError_t launch_paged_attention(const AttentionParams& params, bool f16, void* workspace, hipStream_t s) {
   AttentionParams p = params;
   const AttentionPlan plan = paged_attention_plan(p, p.cache.scales != nullptr);
-  // Tiles of 16 follow the maximum once it is 2^8 above: no shift for more, so that weights times the factors of small
-  // E4M3 values stay above bf16's subnormals.
+  // The maximum is followed once it is 2^8 above: no shift for more, so that weights times the factors of small E4M3
+  // values stay above bf16's subnormals.
   attention_memory(p, plan, (int)kAttentionSlack, workspace);
-  launch_attention_step(p, f16, p.cache.scales ? kStoreE4M3 : kStorePages, (int)plan.grid, plan.waves, (int)plan.join,
-                        s);
+  const bool codes = p.cache.scales != nullptr;
+  if (plan.step) {
+    launch_attention_step(p, f16, codes ? kStoreE4M3 : kStorePages, (int)plan.grid, plan.waves, (int)plan.join, s);
+    return hipGetLastError();
+  }
+  if (codes) {
+    if (f16) launch_tiles<true, kStoreE4M3>(p, plan, s);
+    else launch_tiles<false, kStoreE4M3>(p, plan, s);
+  } else {
+    if (f16) launch_tiles<true, kStorePages>(p, plan, s);
+    else launch_tiles<false, kStorePages>(p, plan, s);
+  }
   return hipGetLastError();
 }
 

@@ -51,14 +51,42 @@ inline void attention_step_plan(AttentionParams& p, AttentionPlan& plan, bool sp
   p.slots = split ? 2 * plan.grid : 0;
 }
 
-// Over a paged cache every call runs in tiles of 16.  A sequence's room stands for its length, which varies: the keys are
-// split from 768 where the tiles leave half of the workgroups idle, and else from 1536.  Equal lengths, us
-// whole and split, 32 heads over 8 of dimension 128 in bf16 and E4M3, and of 64 in bf16: one of 500 keys 11.4 12.0, 10.2 11.4,
-// 8.1 10.4; of 1000 16.3 12.3, 14.5 11.8, 10.7 10.9; of 2000 25.9 13.5, 22.7 12.9, 16.2 11.9; 16 of 1000 18.6 21.5,
-// 15.6 18.2, 11.9 15.6; 16 of 2000 33.0 34.7, 24.4 22.0, 17.8 19.7; 32 of 2000 51.9 54.5, 29.9 34.5, 27.0 31.5.
-// E4M3 tiles take half the LDS, and two workgroups where bf16 has one: 61 sequences of 1 to 8191 keys 117 us, 129 with one.
+// The rest of the plan of tiles of 128.
+inline void attention_tiles_plan(AttentionParams& p, AttentionPlan& plan) {
+  const int64_t cus = compute_units();
+  const int64_t tiles = attention_tiles_at_most(p), whole = p.tokens / p.tile_tokens;
+  // About how many tiles there are: whole ones, or one a sequence.
+  int64_t about = p.batch < p.tokens ? p.batch : p.tokens;
+  if (about < whole) about = whole;
+  p.target = (int)(3 * cus);  // what the GPU holds of them
+  p.min_chunk = 8;
+  if (((int64_t)p.keys + 63) / 64 <= p.min_chunk || 4 * about * p.head_blocks >= 3 * cus) p.target = 0;
+  p.slots = p.target ? 2 * p.target + p.head_blocks : 0;
+  plan.join = p.target ? tiles * p.head_blocks : 0;
+  plan.grid = tiles * p.head_blocks + (p.target ? p.slots : 0);
+  plan.grid = (plan.grid + 7) / 8 * 8;  // whole rounds of the XCDs
+}
+
+// Tiles of 16 rows, or of 128.
+inline bool attention_few_rows(const AttentionParams& p) {
+  const int64_t rows = (int64_t)p.tokens * (p.group < kStepRows ? p.group : kStepRows);
+  return rows <= kStepRows * p.batch || (rows <= 2 * kStepRows * p.batch && 2 * p.batch * p.head_blocks < compute_units());
+}
+
+// Over a paged cache, in tiles of 16 or 128 as packed attention is.  For tiles of 16 a sequence's room stands for its
+// length, which varies: the keys are split from 768 where the tiles leave half of the workgroups idle, and else from
+// 1536.  Equal lengths, us whole and split, 32 heads over 8 of dimension 128 in bf16 and E4M3, and of 64 in bf16: one of
+// 500 keys 11.4 12.0, 10.2 11.4, 8.1 10.4; of 1000 16.3 12.3, 14.5 11.8, 10.7 10.9; of 2000 25.9 13.5, 22.7 12.9, 16.2
+// 11.9; 16 of 1000 18.6 21.5, 15.6 18.2, 11.9 15.6; 16 of 2000 33.0 34.7, 24.4 22.0, 17.8 19.7; 32 of 2000 51.9 54.5,
+// 29.9 34.5, 27.0 31.5.  E4M3 tiles take half the LDS, and two workgroups where bf16 has one: 61 sequences of 1 to 8191
+// keys 117 us, 129 with one.
 inline AttentionPlan paged_attention_plan(AttentionParams& p, bool e4m3) {
   AttentionPlan plan{};
+  attention_shape(p, plan, false);
+  if (!attention_few_rows(p)) {
+    attention_tiles_plan(p, plan);
+    return plan;
+  }
   attention_shape(p, plan, true);
   // About how many tiles there are: whole ones, or one a sequence.
   int64_t tiles = p.batch < p.tokens ? p.batch : p.tokens;
@@ -102,27 +130,14 @@ inline AttentionPlan paged_attention_plan(AttentionParams& p, bool e4m3) {
 // 500 17, in one call 153, in tiles of 16; 100 over 1000 keys 93 and a prompt of 2000 56, in one call
 // 137, in tiles of 128.
 inline AttentionPlan attention_plan(AttentionParams& p) {
-  const int64_t cus = compute_units();
   AttentionPlan plan{};
-  auto shape = [&](bool step) { attention_shape(p, plan, step); };
-  shape(false);
-  const int64_t rows = (int64_t)p.tokens * (p.group < kStepRows ? p.group : kStepRows);
-  if (rows <= kStepRows * p.batch || (rows <= 2 * kStepRows * p.batch && 2 * p.batch * p.head_blocks < cus)) shape(true);
+  attention_shape(p, plan, false);
+  if (attention_few_rows(p)) attention_shape(p, plan, true);
   if (plan.step) {
     attention_step_plan(p, plan, p.keys > 768 && p.keys > 512 * p.batch, p.dim <= 64 ? 2 : 1);
     return plan;
   }
-  const int64_t tiles = attention_tiles_at_most(p), whole = p.tokens / p.tile_tokens;
-  // About how many tiles there are: whole ones, or one a sequence.
-  int64_t about = p.batch < p.tokens ? p.batch : p.tokens;
-  if (about < whole) about = whole;
-  p.target = (int)(3 * cus);  // what the GPU holds of them
-  p.min_chunk = 8;
-  if (((int64_t)p.keys + 63) / 64 <= p.min_chunk || 4 * about * p.head_blocks >= 3 * cus) p.target = 0;
-  p.slots = p.target ? 2 * p.target + p.head_blocks : 0;
-  plan.join = p.target ? tiles * p.head_blocks : 0;
-  plan.grid = tiles * p.head_blocks + (p.target ? p.slots : 0);
-  plan.grid = (plan.grid + 7) / 8 * 8;  // whole rounds of the XCDs
+  attention_tiles_plan(p, plan);
   return plan;
 }
 

@@ -15,7 +15,7 @@
 // load fetches one block ahead.  E4M3 codes go to LDS as they are, with their factors, and become 16 bits between
 // LDS and the matrix cores (exactly): a key's factor multiplies its score, a value's its weight before that is
 // rounded, to bf16 whatever q's type (a factor has binary32's range).
-#include "attention.h"
+#include "attention_codes.h"
 
 namespace vfa {
 
@@ -49,18 +49,6 @@ __device__ __forceinline__ int step_v_code_swizzle(int r) {
   return PITCH == 128 ? (r >> 1 & 3) | (r >> 4 & 1) << 2 : (r >> 2 & 1) | (r >> 4 & 1) << 1;
 }
 
-// Eight E4M3 codes as 16-bit operands of a product; exact.
-template <bool F16>
-__device__ __forceinline__ v4i step_widen(v2i c) {
-  v4i w;
-  static_for<4>([&](auto i) {
-    if constexpr (F16)
-      w[(int)i] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c[i / 2], 1.0f, (i & 1) != 0));
-    else
-      w[(int)i] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[i / 2], 1.0f, (i & 1) != 0));
-  });
-  return w;
-}
 // Eight bytes per lane, transposed inside each group of 16 lanes: lanes 2 r and 2 r + 1 give the address of
 // elements 0 .. 7 and 8 .. 15 of row r, and lane i receives element i of the eight rows.
 __device__ __forceinline__ v2i lds_read_tr8(const uint8_t* p) {
@@ -207,7 +195,7 @@ __global__ void __launch_bounds__(64 * W, 1) attention_step(const AttentionParam
         static_for<QS>([&](auto st) {
           const uint8_t* src = krow + buf * L::SLOT + kbk * 16 * L::PITCH;
           v4i a;
-          if constexpr (E4M3) a = step_widen<F16>(*reinterpret_cast<const v2i*>(src + (((2 * st + (fg >> 1)) ^ ksw) << 4)));
+          if constexpr (E4M3) a = attention_widen<F16>(*reinterpret_cast<const v2i*>(src + (((2 * st + (fg >> 1)) ^ ksw) << 4)));
           else a = *reinterpret_cast<const v4i*>(src + (((4 * st + fg) ^ ksw) << 4));
           s[kbk] = mfma16<F16>(a, q[st], s[kbk]);
         });
@@ -250,7 +238,7 @@ __global__ void __launch_bounds__(64 * W, 1) attention_step(const AttentionParam
       else weights(std::false_type{});
       static_for<DB>([&](auto db) {
         if constexpr (E4M3) {
-          const v4i a = step_widen<false>(lds_read_tr8(vrow + buf * L::SLOT + ((db ^ vsw) << 4)));
+          const v4i a = attention_widen<false>(lds_read_tr8(vrow + buf * L::SLOT + ((db ^ vsw) << 4)));
           o[db] = mfma16<W16>(a, pk, o[db]);
         } else {
           const uint8_t* src = vrow + buf * L::SLOT + (((2 * db + vc) ^ vsw) << 4);

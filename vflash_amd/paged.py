@@ -137,13 +137,13 @@ def paged_attention(q, cache: PagedCache, table, lengths, *, q_offsets=None, sca
 
     The cache, ``table``, ``lengths`` and ``q_offsets`` are those of ``paged_append`` (which comes first);
     ``heads`` is a multiple of the cache's key heads, and head ``h`` reads key head
-    ``h // (heads // key_heads)``.  One token a sequence without ``q_offsets``, else a few (drafted tokens, the
-    end of a prompt): token ``i`` of ``n`` sees the sequence's first ``lengths[b] - n + i + 1`` tokens.  Rows that
+    ``h // (heads // key_heads)``.  One token a sequence without ``q_offsets``, else any number (drafted tokens, a
+    prompt or its next piece): token ``i`` of ``n`` sees the sequence's first ``lengths[b] - n + i + 1`` tokens.  Rows that
     see none, and rows outside every sequence, are zeros.  ``scale`` defaults to ``dim ** -0.5``.
 
-    Any number of tokens is right, in tiles of 16 rows (token and head) that each read their keys: whole
-    prompts run faster in ``attention.packed_attention``.  Softmax and sums are binary32; weights are
-    rounded to the operands' type, to bf16 after the values' scales with an E4M3 cache.  As there, infinities and
+    Single tokens and a few run in tiles of 16 rows (token and head), whole prompts and pieces of prompts in
+    tiles of 128, as in ``packed_attention``.  Softmax and sums are binary32; weights are rounded to the operands'
+    type, to bf16 after the values' scales with an E4M3 cache.  As there, infinities and
     NaN in the values of a sequence can reach its masked queries as NaN.  Inference only.
     """
     if isinstance(q, torch.Tensor) and q.is_cuda and isinstance(cache, PagedCache):
