@@ -559,7 +559,7 @@ int vflash_paged_attention(const void* q, int64_t q_ts, int64_t q_hs, int f16, i
  *   workspace vflash_request_adapters_workspace(...) bytes, 16-byte aligned, without contents to keep; one call at a
  *             time
  *   Requires width % 16 == 0, 16 <= width <= 128, adapters < 8192, k % 8 == 0, every widths[b] % 8 == 0 and < 2^21, rows <
- *   2^24, row strides multiples of 8 (equal where out is base), 16-byte aligned matrices.
+ *   2^21, row strides multiples of 8 (equal where out is base), 16-byte aligned matrices.
  */
 int64_t vflash_request_adapters_workspace(int64_t rows, int64_t k, const int64_t* widths, int64_t branches,
                                           int64_t adapters, int64_t width);

@@ -304,7 +304,7 @@ def test_adapter_entry_refuses():
                     stream=None)
     for change in (dict(base=None), dict(x=None), dict(down=None), dict(up=None), dict(scaling=None), dict(ranks=None),
                    dict(index=None), dict(out=None), dict(workspace=None), dict(ldb=72), dict(ldb=84), dict(ldx=24),
-                   dict(ldx=36), dict(ldo=72), dict(out=P, ldo=88), dict(rows=0), dict(rows=1 << 24), dict(k=0), dict(k=36),
+                   dict(ldx=36), dict(ldo=72), dict(out=P, ldo=88), dict(rows=0), dict(rows=1 << 21), dict(k=0), dict(k=36),
                    dict(widths=None), dict(widths=(ctypes.c_int64 * 3)(48, 12, 16)),
                    dict(widths=(ctypes.c_int64 * 3)(48, 0, 16)), dict(branches=0), dict(branches=4), dict(adapters=0),
                    dict(adapters=8192), dict(width=0), dict(width=24), dict(width=144), dict(workspace_bytes=16),

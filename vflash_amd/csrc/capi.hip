@@ -233,7 +233,7 @@ bool set_rotary(vfa::RotaryParams& r, const uint64_t* phases, const int64_t* axi
 
 bool request_sizes(vfa::RequestAdapterParams& p, int64_t rows, int64_t k, const int64_t* widths, int64_t branches,
                    int64_t adapters, int64_t width) {
-  if (rows < 1 || rows >= (int64_t(1) << 24) || k < 8 || k % 8 || k >= ROWS_LIMIT || !widths) return false;
+  if (rows < 1 || rows >= (int64_t(1) << 21) || k < 8 || k % 8 || k >= ROWS_LIMIT || !widths) return false;
   if (branches < 1 || branches > vfa::RA_BRANCHES || adapters < 1 || adapters >= 8192) return false;
   if (width < 16 || width > 128 || width % 16) return false;
   int64_t n = 0;

@@ -262,12 +262,12 @@ __global__ void __launch_bounds__(64 * RU_WAVES) request_up(const RequestAdapter
   constexpr int PITCH = 64 * NC + 8;  // of a row in LDS: high parts, low parts, and eight against bank conflicts
   __shared__ int rows[64];
   __shared__ __attribute__((aligned(16))) uint16_t low_rank[64 * PITCH];
-  const RequestItem it = uniform(request_listed(p, (int)blockIdx.x, rows));
+  const RequestItem it = uniform(request_listed(p, (int)blockIdx.y, rows));
   __syncthreads();
   if (it.count == 0) return;
   const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int fr = lane & 15, fg = lane >> 4;
-  int branch = 0, group = (int)blockIdx.y;
+  int branch = 0, group = (int)blockIdx.x;
   while (branch + 1 < p.branches && group >= p.groups[branch]) ++branch;
   if (branch) group -= p.groups[branch - 1];
   const int first_col = branch ? p.ends[branch - 1] : 0, stop = p.ends[branch];
@@ -376,7 +376,10 @@ int request_ranks(const RequestAdapterParams& p) {
 // The launch of a call, from its sizes alone.
 void request_plan(RequestAdapterParams& p) {
   const int64_t cus = compute_units();
-  p.item_rows = p.rows > 512 ? 64 : 16;
+  // Items of 64 rows read A and B less often, those of 16 are more: us with 64 and with 16, K 5120: 256 rows of 24 adapters of
+  // rank 64 beside three branches 28.8, 27.9, 400 rows 32.7, 40.7; of rank 32 beside one, 600 rows 20.5, 19.8, 1000 rows
+  // 23.6, 26.1; 1000 rows of 4 adapters of rank 16 21.5, 19.1.
+  p.item_rows = p.rows > 300 && p.rows * p.branches * p.width >= 24576 ? 64 : 16;
   const int64_t groups = p.rows < p.adapters + 1 ? p.rows : p.adapters + 1;
   p.items = (int)(p.rows / p.item_rows + groups);
   if (p.items > p.rows) p.items = (int)p.rows;
@@ -415,7 +418,8 @@ hipError_t launch_request_adapters(const RequestAdapterParams& params, bool f16,
     p.groups[b] = groups;
   }
   const dim3 down((unsigned)p.items, (unsigned)p.splits, (unsigned)((p.branches * p.width + ranks - 1) / ranks));
-  const dim3 up((unsigned)p.items, (unsigned)groups);
+  // An item's columns next to each other: 4093 rows 83.4 us, with the items next to each other 85.5.
+  const dim3 up((unsigned)groups, (unsigned)p.items);
   auto run_down = [&](auto type, auto blocks) {
     constexpr bool F16 = type;
     constexpr int RB = blocks;
