@@ -75,7 +75,7 @@ def indices(dev, rows, count, order, seed=0):
 
 @pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
 @pytest.mark.parametrize("ranks", [[16], [1, 7, 16], [32, 8, 0, 20], [64, 33, 64], [128, 4, 100, 65]], ids=str)
-@pytest.mark.parametrize("rows", [1, 2, 16, 17, 63, 64, 65, 200, 513, 700])
+@pytest.mark.parametrize("rows", [1, 2, 16, 17, 63, 64, 65, 200, 513, 700, 1700])
 def test_rows_and_ranks(dev, rows, ranks, dtype):
     k, widths = 264, (72,)
     pack = stack(dev, ranks, k, widths, dtype)

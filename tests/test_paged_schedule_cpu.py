@@ -125,7 +125,7 @@ def test_places(tmp_path, head):
 # tokens, room, sequences, heads, group, dim
 SIZES = {
     "one a sequence": (90, 4096, 90, 8, 4, 128), "XCDs": (70, 2048, 70, 32, 2, 128), "not split": (40, 512, 40, 6, 3, 64),
-    "many": (150, 131072, 150, 4, 4, 64), "several": (90, 4096, 20, 8, 4, 64), "wide group": (3, 4096, 3, 40, 40, 64),
+    "many": (150, 131072, 150, 4, 4, 64), "very many": (4200, 4096, 4200, 2, 2, 64), "several": (90, 4096, 20, 8, 4, 64), "wide group": (3, 4096, 3, 40, 40, 64),
     "tiles, wide group": (9, 4096, 3, 40, 40, 64),
     "tiles, no sequence": (5, 4096, 0, 4, 2, 64), "tiles": (900, 4096, 2, 8, 8, 128), "tiles, several": (700, 8192, 5, 8, 1, 64),
     "tiles, many": (3000, 2048, 100, 4, 2, 64), "tiles, not split": (6000, 512, 9, 7, 7, 64),
@@ -136,6 +136,10 @@ SIZES = {
 def test_paged_schedule(tmp_path, head, size):
     tokens, room, batch, heads, group, dim = size
     text = head.replace("attention_line(p,", "attention_line<true>(p,").replace("attention_segment(p,", "attention_segment<true>(p,")
+    text = text.replace("      AttentionSegment seg = attention_segment<true>(p, line, (int)b, pos, stop);", """
+      seg = pos == begin ? attention_segment<true>(p, line, (int)b, pos, stop)
+                         : attention_following<true>(p, line, (int)b, seg, pos, stop);""")
+    text = text.replace("    for (uint32_t pos = begin; pos < stop;) {", "    AttentionSegment seg{};\n    for (uint32_t pos = begin; pos < stop;) {")
     text = text.replace("attention_item<false>(p,", "attention_item<false, true>(p,").replace("attention_item<true>(p,", "attention_item<true, true>(p,")
     text += r"""
 int main() {

@@ -366,6 +366,9 @@ struct AttentionLine {
   int unit_shift;
   int xcds;             // 8: the line is one XCD's
   AttentionSeq mine;    // of this lane, where there are at most 64 sequences
+  // Over a paged cache, one token a sequence: this lane's run of `run` sequences and the lanes' before it, in units.
+  int64_t run;
+  uint32_t own, upto;
 };
 struct AttentionSegment {
   AttentionItem it;  // seq, tile, head_block
@@ -376,7 +379,17 @@ __device__ __forceinline__ uint32_t attention_units_of(const AttentionLine& l, c
   return max(1u, ((uint32_t)s.nk + (1u << l.unit_shift) - 1) >> l.unit_shift);
 }
 
-// Over a paged cache, one token a sequence and whole sequences: unit i of a head block is sequence i.
+// Over a paged cache, one token a sequence: a sequence is a tile, and the workgroup that ends one goes on with the next.
+__device__ __forceinline__ int attention_keys(const AttentionParams& p, int64_t length) {
+  return length < 0 ? 0 : length < p.keys ? (int)length : p.keys;
+}
+// A sequence that the wave shares, by a scalar load.
+__device__ __forceinline__ AttentionSeq attention_single(const AttentionParams& p, int64_t sequence) {
+  typedef const __attribute__((address_space(4))) int64_t lengths_t;
+  const int s = __builtin_amdgcn_readfirstlane((int)sequence);
+  return AttentionSeq{s, s, 1, attention_keys(p, ((lengths_t*)(uintptr_t)p.cache.lengths)[s])};
+}
+// Of whole sequences, unit i of a head block is sequence i.
 __device__ __forceinline__ bool attention_direct(const AttentionParams& p) { return !p.q_offsets && p.unit_shift == 31; }
 
 template <bool PAGED = false>
@@ -385,9 +398,20 @@ __device__ __forceinline__ AttentionLine attention_line(const AttentionParams& p
   AttentionLine l{};
   l.unit_shift = p.unit_shift;
   int reached = 0;
-  const bool direct = PAGED && attention_direct(p);
-  if (direct) l.units = (uint32_t)p.batch;
-  for (int64_t base = 0; base < p.batch + 2 && !direct; base += 64) {
+  const bool singles = PAGED && !p.q_offsets;
+  if (PAGED && attention_direct(p)) {
+    l.units = (uint32_t)p.batch;
+  } else if (singles) {
+    // A lane's loads do not wait for each other, and one scan serves any number of sequences.
+    l.run = (p.batch + 63) / 64;
+    const int64_t s0 = lane * l.run, s1 = s0 + l.run < p.batch ? s0 + l.run : p.batch;
+#pragma unroll 4
+    for (int64_t s = s0; s < s1; ++s) l.own += attention_units_of(l, AttentionSeq{0, 0, 1, attention_keys(p, p.cache.lengths[s])});
+    int sum;
+    l.upto = (uint32_t)wave_scan((int)l.own, lane, sum);
+    l.units = (uint32_t)sum;
+  }
+  for (int64_t base = 0; base < p.batch + 2 && !singles; base += 64) {
     l.mine = attention_sequence<PAGED>(p, base, reached);
     int sum;
     wave_scan((int)(attention_tiles_of(p, l.mine) * attention_units_of(l, l.mine)), lane, sum);
@@ -410,11 +434,33 @@ __device__ __forceinline__ AttentionSegment attention_segment(const AttentionPar
   AttentionSegment g{};
   const uint32_t local = attention_quotient(pos, line.units), x = pos - local * line.units;
   g.it.head_block = line.xcds == 8 ? (b & 7) + 8 * (int)local : (int)local;
-  if (PAGED && attention_direct(p)) {
-    const int64_t keys = p.cache.lengths[x];
-    g.it.seq = AttentionSeq{(int)x, (int)x, 1, keys < 0 ? 0 : keys < p.keys ? (int)keys : p.keys};
-    g.of = g.count = 1;
-    g.it.live = true;
+  if (PAGED && !p.q_offsets) {
+    auto take = [&](int64_t s, uint32_t before) {
+      g.it.seq = attention_single(p, s);
+      g.of = attention_units_of(line, g.it.seq);
+      g.first = x - before;
+      g.count = min(g.of - g.first, stop - pos);
+      g.it.live = true;
+    };
+    if (attention_direct(p)) {
+      take(x, x);
+      return g;
+    }
+    const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(line.upto > x));
+    const int64_t s0 = l * line.run, s1 = s0 + line.run < p.batch ? s0 + line.run : p.batch;
+    uint32_t before = (uint32_t)__builtin_amdgcn_readlane((int)(line.upto - line.own), l);
+    for (int64_t base = s0; base < s1; base += 64) {
+      const int64_t s = base + lane;
+      const int own = s < s1 ? (int)attention_units_of(line, AttentionSeq{0, 0, 1, attention_keys(p, p.cache.lengths[s])}) : 0;
+      int sum;
+      const uint32_t incl = (uint32_t)wave_scan(own, lane, sum);
+      if (x < before + (uint32_t)sum) {
+        const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(before + incl > x));
+        take(base + at, before + (uint32_t)__builtin_amdgcn_readlane((int)incl - own, at));
+        return g;
+      }
+      before += (uint32_t)sum;
+    }
     return g;
   }
   uint32_t before = 0;
@@ -439,6 +485,38 @@ __device__ __forceinline__ AttentionSegment attention_segment(const AttentionPar
     before += (uint32_t)sum;
   }
   return g;
+}
+
+// The segment at `pos`, behind one that ends its tile there.
+template <bool PAGED>
+__device__ __forceinline__ AttentionSegment attention_following(const AttentionParams& p, const AttentionLine& line, int b,
+                                                                const AttentionSegment& ended, uint32_t pos, uint32_t stop) {
+  if (!PAGED || p.q_offsets) return attention_segment<PAGED>(p, line, b, pos, stop);
+  AttentionSegment g = ended;
+  int s = ended.it.seq.k0 + 1;
+  if (s == p.batch) {
+    s = 0;
+    g.it.head_block += line.xcds;
+  }
+  g.it.seq = attention_single(p, s);
+  g.of = attention_units_of(line, g.it.seq);
+  g.first = 0;
+  g.count = min(g.of, stop - pos);
+  return g;
+}
+
+// In scalar registers, where the compiler does not see that the search is uniform.
+__device__ __forceinline__ AttentionSegment attention_scalar(const AttentionSegment& g) {
+  auto u = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+  AttentionSegment s{};
+  s.it.seq = AttentionSeq{u(g.it.seq.q0), u(g.it.seq.k0), u(g.it.seq.nq), u(g.it.seq.nk)};
+  s.it.tile = u(g.it.tile);
+  s.it.head_block = u(g.it.head_block);
+  s.it.live = u(g.it.live) != 0;
+  s.first = (uint32_t)u((int)g.first);
+  s.count = (uint32_t)u((int)g.count);
+  s.of = (uint32_t)u((int)g.of);
+  return s;
 }
 
 }  // namespace vfa

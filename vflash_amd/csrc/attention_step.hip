@@ -63,8 +63,9 @@ __device__ __forceinline__ void lds_dma4(__amdgpu_buffer_rsrc_t r, uint32_t lds_
                : "m0");
 }
 
+// E4M3 at dimension 64: four workgroups a CU.
 template <bool F16, int DP, int STORE, int W>
-__global__ void __launch_bounds__(64 * W, 1) attention_step(const AttentionParams p) {
+__global__ void __launch_bounds__(64 * W, STORE == kStoreE4M3 && DP <= 64 ? 4 : 1) attention_step(const AttentionParams p) {
   using L = AttentionSteps<DP, STORE, W>;
   constexpr bool PAGED = STORE != kStoreRows, E4M3 = L::E4M3;
   constexpr bool W16 = F16 && !E4M3;  // the type of the weights
@@ -80,8 +81,16 @@ __global__ void __launch_bounds__(64 * W, 1) attention_step(const AttentionParam
 
   const AttentionLine line = attention_line<PAGED>(p, gridDim.x);
   const uint32_t begin = (blockIdx.x >> (line.xcds == 8 ? 3 : 0)) * line.quota, stop = min(begin + line.quota, line.end);
+  [[maybe_unused]] AttentionSegment ended{};
   for (uint32_t pos = begin; pos < stop;) {
-    const AttentionSegment seg = attention_segment<PAGED>(p, line, blockIdx.x, pos, stop);
+    const AttentionSegment seg = [&] {
+      if constexpr (PAGED)
+        return attention_scalar(pos == begin ? attention_segment<true>(p, line, blockIdx.x, pos, stop)
+                                             : attention_following<true>(p, line, blockIdx.x, ended, pos, stop));
+      else
+        return attention_segment(p, line, blockIdx.x, pos, stop);
+    }();
+    if constexpr (PAGED) ended = seg;
     const AttentionItem& it = seg.it;
     if (!it.live) return;
     const AttentionRow row = attention_row(p, it, fr);
