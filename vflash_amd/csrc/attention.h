@@ -421,7 +421,7 @@ __device__ __forceinline__ AttentionLine attention_line(const AttentionParams& p
   const int shift = l.xcds == 8 ? 3 : 0;
   l.end = l.units * (uint32_t)(p.head_blocks >> shift);
   const uint32_t parts = (uint32_t)grid >> shift;
-  l.quota = max(1u, attention_quotient(l.end + parts - 1, parts));
+  l.quota = max(PAGED ? p.least_units : 1u, attention_quotient(l.end + parts - 1, parts));
   return l;
 }
 

@@ -41,6 +41,7 @@ struct AttentionParams {
   // Splitting of the keys, off where target is 0.
   int target, min_chunk;  // items, blocks of 64 keys
   int64_t slots;          // what the workspace holds
+  uint32_t least_units;  // of a workgroup of a paged call
   int unit_shift;  // attention_step: log2 of a unit's keys (31: a whole sequence)
   float* part;  // [slot][row][d], then [slot][row] maxima and sums
   float* part_ml;

@@ -99,6 +99,9 @@ inline AttentionPlan paged_attention_plan(AttentionParams& p, bool e4m3) {
   // four waves 42; of 700 70 and 75; 64 of 250 in E4M3, which fit, 13.2 and 12.7.
   plan.waves = !split && tiles > held ? 2 : 4;
   attention_step_plan(p, plan, split, per_cu * 4 / plan.waves);
+  // Of several tokens a sequence a workgroup takes two units at least, half as many segments for their join: four tokens after
+  // 8000 keys in E4M3 18.6 us, by single units 22.0, after 2000 14.3 either way; one token of 2000 keys 14.4 and 13.7.
+  p.least_units = split && p.tokens > p.batch ? 2 : 1;
   if (plan.join) {
     // A join of 256 threads takes 16 / rows segments of a tile at a time, one of 1024 four times as many, but its
     // grid takes longer to start: 128 sequences of 1000 keys in E4M3 58 and 62 us, 15 of four tokens 25.8 and 23.1.
