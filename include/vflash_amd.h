@@ -528,7 +528,8 @@ int vflash_paged_append(const void* q, int64_t q_ts, int64_t q_hs, const void* k
  * Attention of new tokens over a paged cache that holds them already: vflash_packed_attention, causal, with the keys and
  * values of vflash_paged_append.  No reference counterpart.
  *   q_offsets, values, scales, table, lengths, batch as there; out as vflash_packed_attention
- *   With scales, a key's factor multiplies its score and a value's its weight before that is rounded to bf16.
+ *   With scales, a key's factor multiplies its score and a value's its weight before that is rounded to bf16; values
+ *   whose factors are below 2^-117 times width * page may lose bits.
  * Lengths are clamped to the table.  Keys on a page outside [0, pages) count as keys and values of zeros.  Nothing
  * else outside a sequence's pages is read.  Masked keys, rows that see none, and scores as vflash_packed_attention.
  *   workspace  vflash_paged_attention_workspace(...) bytes (e4m3: with scales; 0: may be NULL), 16-byte aligned,
@@ -554,7 +555,7 @@ int vflash_paged_attention(const void* q, int64_t q_ts, int64_t q_hs, int f16, i
  *   scaling   fp32 [adapters, branches];  ranks int32 [adapters]
  *   index     int64 [rows]: the row's adapter; outside [0, adapters): none
  *   out[m, n] = base[m, n] + scaling[i, b] sum_r (sum_k x[m, k] down[i, b * width + r, k]) up[i, n, r], i = index[m],
- *   b the branch of column n.  Sums are binary32; t = scaling (x down^T) enters the second product as two 16-bit parts,
+ *   b the branch of column n.  Sums are binary32; t = x down^T enters the second product as two 16-bit parts,
  *   and the result is rounded once.  Rows without an adapter are copied.
  *   workspace vflash_request_adapters_workspace(...) bytes, 16-byte aligned, without contents to keep; one call at a
  *             time

@@ -516,3 +516,24 @@ def test_empty_calls(dev):
     q = make(dev, 1, 4, 64)
     assert not paged_append(empty, q[:, :2], q[:, :2], zero[None], zero + 1, q=q, rotary=rotary).any()
     assert not paged_attention(q, empty, zero[None], zero + 1).any()
+
+
+def test_autograd_notices_that_a_cache_has_changed(dev):
+    cache, table = pool(dev, [9, 9], 16, 2, 64, BF16)
+    n, k = torch.tensor([9, 9], device=dev), make(dev, 2, 2, 64)
+    for append in (lambda: paged_append(cache, k, k, table, n),
+                   lambda: kernels.paged_append(cache, None, k, k, table, n, None, None, None)):
+        w = torch.ones((), device=dev, dtype=BF16, requires_grad=True)
+        y = (cache.values * w).sum()
+        append()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    with torch.inference_mode():
+        paged_append(PagedCache.zeros(3, 16, 2, 64, device=dev), k, k, table, n)
+
+
+def test_rotary_of_another_kind_is_refused(dev):
+    cache, table = pool(dev, [9], 16, 2, 64, BF16)
+    k = make(dev, 1, 2, 64)
+    with pytest.raises(ValueError, match="take a Rotary"):
+        paged_append(cache, k, k, table, torch.tensor([9], device=dev), rotary=1)

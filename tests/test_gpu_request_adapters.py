@@ -273,3 +273,20 @@ def test_a_slot_taken_by_another_adapter(dev):
     x, base, index = make(dev, 20, 64, seed=1), make(dev, 20, 48, seed=2), indices(dev, 20, 2, "mixed")
     check(add_request_adapters(base, x, pack, index), base, x, pack, index)
     assert isinstance(pack, RequestAdapters)
+
+
+def test_autograd_notices_a_base_changed_in_place(dev):
+    pack = stack(dev, [16, 24], 128, (64, 32), BF16)
+    x, index = make(dev, 9, 128, seed=1), indices(dev, 9, 2, "mixed")
+    for add in (add_request_adapters, lambda b, *a, inplace: kernels.request_adapters(b, *a, inplace)):
+        base = make(dev, 9, 96, seed=2)
+        w = torch.ones((), device=dev, dtype=BF16, requires_grad=True)
+        y = (base * w).sum()
+        add(base, x, pack, index, inplace=False)
+        before = base._version
+        add(base, x, pack, index, inplace=True)
+        assert base._version > before
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    with torch.inference_mode():
+        add_request_adapters(make(dev, 9, 96), x, pack, index, inplace=True)

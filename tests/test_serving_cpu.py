@@ -133,6 +133,15 @@ def test_cache_refusals():
     refused("plain memory", torch.zeros(3 * 4096 + 1, dtype=BF16)[1:].view(3, 2, 2, 16, 64))
 
 
+def test_attributes_stay():
+    # Their sizes bound what the kernels read: they are not replaced behind the checks.
+    c, r = cache(dtype=E4M3), turning(axes=[0, 1] * 16)
+    for thing, names in ((c, ("values", "scales")), (r, ("phases", "pairs", "axis", "axes", "interleaved", "magnitude"))):
+        for name in names:
+            with pytest.raises(AttributeError, match="made of"):
+                setattr(thing, name, getattr(thing, name))
+
+
 TABLE, LENGTHS = torch.zeros((4, 2), dtype=torch.int64), torch.ones(4, dtype=torch.int64)
 
 

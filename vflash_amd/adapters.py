@@ -114,7 +114,7 @@ def add_request_adapters(base, x, adapters: RequestAdapters, index, *, inplace: 
     may come in any order; each adapter in use is read about once.  ``inplace`` writes to ``base``.
 
     Sums are binary32 and the result is rounded once (the one-adapter epilogues round each step, as the
-    reference's hook does).  Inference only.
+    reference's hook does).  Infinities and NaN of a row of ``x`` reach all branches of its adapter.  Inference only.
     """
     if isinstance(base, torch.Tensor) and base.is_cuda and isinstance(adapters, RequestAdapters):
         # The whole call in native code; None sends any other layout, and every refusal, on from here.

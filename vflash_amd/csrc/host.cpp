@@ -253,6 +253,11 @@ PyObject* packed_attention(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// Tells autograd, which may have saved it, that the tensor has other values now.
+void written(const at::Tensor* t) {
+  if (t && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
 // A [rows, heads, dim] operand as the kernels of the heads take it, with nothing to record.
 bool heads_ok(const at::Tensor* t, const at::Tensor& like) {
   return t->dim() == 3 && t->size(1) >= 1 && t->size(2) == like.size(2) && t->scalar_type() == like.scalar_type() &&
@@ -378,6 +383,8 @@ PyObject* paged_append(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
         c10::hip::getCurrentHIPStream(d.index()).stream());
   }
   if (status != VFLASH_OK) Py_RETURN_NONE;
+  written(c.values);
+  written(c.scales);
   if (!q) Py_RETURN_TRUE;
   return THPVariable_Wrap(std::move(q_out));
   END_HANDLE_TH_ERRORS
@@ -456,7 +463,10 @@ PyObject* request_adapters(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
                                      workspace.data_ptr(), bytes, c10::hip::getCurrentHIPStream(d.index()).stream());
   }
   if (status != VFLASH_OK) Py_RETURN_NONE;
-  if (a[8] == Py_True) return Py_NewRef(a[0]);
+  if (a[8] == Py_True) {
+    written(base);
+    return Py_NewRef(a[0]);
+  }
   return THPVariable_Wrap(std::move(out));
   END_HANDLE_TH_ERRORS
 }

@@ -76,8 +76,8 @@ __global__ void __launch_bounds__(RT_THREADS, 8) rotate_heads(const RotateParams
   const int64_t position = place.position, page = place.page;
   if (r.phases) {
     for (int i = (int)threadIdx.x; i < r.pairs; i += RT_THREADS) {
-      const int axis = r.axis ? (int)r.axis[i] : 0;
-      const int64_t at = !r.positions ? position : (unsigned)axis < (unsigned)r.axes ? r.positions[token * r.axes + axis] : 0;
+      const int64_t axis = r.axis ? r.axis[i] : 0;
+      const int64_t at = !r.positions ? position : (uint64_t)axis < (uint64_t)r.axes ? r.positions[token * r.axes + axis] : 0;
       const uint64_t turn = (uint64_t)at * r.phases[i];
       const v2f cs = cos_sin((uint32_t)((turn + 0x80000000ull) >> 32));
       cosines[i] = cs[0] * r.magnitude;

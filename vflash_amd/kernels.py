@@ -736,6 +736,13 @@ def _rotary_arguments(rotary, positions):
             rotary.axes)
 
 
+def _written(*tensors):
+    """Tells autograd, which may have saved them, that these have other values now."""
+    for t in tensors:
+        if t is not None and not t.is_inference():
+            torch.autograd.graph.increment_version(t)
+
+
 def rotate(q, k, positions, rotary):
     """Rotary positions of q and k (operands as ``rotary.rotate`` checks them)."""
     device = require_device(q, k, positions, rotary.phases, rotary.axis)
@@ -769,6 +776,7 @@ def paged_append(cache, q, k, v, table, lengths, q_offsets, rotary, positions):
              q.shape[1] if q is not None else 0, key_heads, dim, ptr(q_offsets), *_rotary_arguments(rotary, positions),
              ptr(values), ptr(cache.scales), values.shape[0], values.shape[3], ptr(table), table.shape[1], ptr(lengths),
              table.shape[0], ptr(q_out), stream_of(device))
+        _written(values, cache.scales)
     elif q_out is not None:
         q_out.zero_()  # a cache without pages has no place
     return q_out
@@ -834,4 +842,6 @@ def request_adapters(base, x, adapters, index, inplace):
          int(x.dtype == torch.float16), rows, k, widths, branches, ptr(adapters.down), ptr(adapters.up),
          ptr(adapters.scaling), ptr(adapters.ranks), count, width, ptr(index), ptr(rows_out), rows_out.stride(0),
          ptr(workspace), size, stream_of(device))
+    if inplace:
+        _written(base)
     return out

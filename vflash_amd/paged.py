@@ -49,8 +49,11 @@ class PagedCache:
             raise ValueError("scales must be a contiguous fp32 [pages, 2, key_heads, page] tensor beside the pages")
         if any(t is not None and (t.requires_grad or t.is_neg() or t.data_ptr() % 16) for t in (values, scales)):
             raise ValueError("a paged cache is plain memory, 16-byte aligned, without gradients")
-        self.values = values
-        self.scales = scales
+        object.__setattr__(self, "values", values)
+        object.__setattr__(self, "scales", scales)
+
+    def __setattr__(self, name, value):
+        raise AttributeError("a paged cache keeps the tensors that it was made of")
 
     @classmethod
     def zeros(cls, pages, page, key_heads, dim, dtype=torch.bfloat16, device="cuda"):
@@ -105,7 +108,8 @@ def paged_append(cache: PagedCache, k, v, table, lengths, *, q=None, q_offsets=N
     that does not exist) is not stored, and its rows of ``q`` come back as zeros: a batch
     padded with sequences of length 0 leaves the cache alone.  Inference only.
     """
-    if isinstance(k, torch.Tensor) and k.is_cuda and isinstance(cache, PagedCache):
+    if (isinstance(k, torch.Tensor) and k.is_cuda and isinstance(cache, PagedCache)
+            and (rotary is None or isinstance(rotary, Rotary))):
         # The whole call in native code; None sends any other layout, and every refusal, on from here.
         host = _lib.host()
         if host is not None:

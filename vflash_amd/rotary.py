@@ -86,18 +86,21 @@ class Rotary:
         # within binary32, as the kernel multiplies
         if not abs(magnitude) <= 3.39e38:
             raise ValueError("the rotary magnitude must be finite")
-        self.phases = torch.tensor([_phase(f) for f in frequencies], dtype=torch.int64, device=device)
-        self.pairs = len(frequencies)
-        self.interleaved = layout == "interleaved"
-        self.magnitude = float(magnitude)
-        self.axis, self.axes = None, 1
+        axis, count = None, 1
         if axes is not None:
             axes = [int(a) for a in axes]
-            if len(axes) != self.pairs or min(axes) < 0 or max(axes) > 63:
+            if len(axes) != len(frequencies) or min(axes) < 0 or max(axes) > 63:
                 raise ValueError("rotary axes are one of 0 to 63 for each pair")
-            self.axes = max(axes) + 1
-            if self.axes > 1:
-                self.axis = torch.tensor(axes, dtype=torch.int64, device=device)
+            count = max(axes) + 1
+            if count > 1:
+                axis = torch.tensor(axes, dtype=torch.int64, device=device)
+        phases = torch.tensor([_phase(f) for f in frequencies], dtype=torch.int64, device=device)
+        for name, value in (("phases", phases), ("pairs", len(frequencies)), ("interleaved", layout == "interleaved"),
+                            ("magnitude", float(magnitude)), ("axis", axis), ("axes", count)):
+            object.__setattr__(self, name, value)
+
+    def __setattr__(self, name, value):
+        raise AttributeError("rotary positions keep what they were made of")
 
 
 def rotate(q, k, positions, rotary: Rotary):
