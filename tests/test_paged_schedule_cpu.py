@@ -140,6 +140,21 @@ def test_paged_schedule(tmp_path, head, size):
       seg = pos == begin ? attention_segment<true>(p, line, (int)b, pos, stop)
                          : attention_following<true>(p, line, (int)b, seg, pos, stop);""")
     text = text.replace("    for (uint32_t pos = begin; pos < stop;) {", "    AttentionSegment seg{};\n    for (uint32_t pos = begin; pos < stop;) {")
+    # What a workgroup leaves for the join is what the join of packed attention finds.
+    text = text.replace("static void steps() {", "static AttentionBegun left[1 << 16];\nstatic void steps() {").replace("""      pos += seg.count;
+    }
+""", """      pos += seg.count;
+    }
+    const AttentionBegun own = attention_begun(p, line, (int)b, seg, stop);
+    if (threadIdx.x == 0) left[b] = own;
+""")
+    text = text.replace("    if (begin >= stop) continue;", "    AttentionBegun own = left[b];\n    if (begin >= stop && own.segments) exit(13);\n    if (begin >= stop) continue;")
+    text = text.replace("tile_end <= stop) continue;", "tile_end <= stop) { if (own.segments) exit(14); continue; }")
+    text = text.replace("    for (int s = 0; s < segments && threadIdx.x == 0", """    const int row = seg.it.tile * p.tile_tokens;
+    if (own.segments != segments || own.row != seg.it.seq.q0 + row || own.head_block != seg.it.head_block ||
+        own.tokens != min(p.tile_tokens, seg.it.seq.nq - row)) exit(15);
+    for (int s = 0; s < segments && threadIdx.x == 0""")
+    assert all(text.count(part) == 1 for part in ("exit(13)", "exit(14)", "exit(15)", "left[b] = own"))
     text = text.replace("attention_item<false>(p,", "attention_item<false, true>(p,").replace("attention_item<true>(p,", "attention_item<true, true>(p,")
     text += r"""
 int main() {

@@ -505,6 +505,21 @@ __device__ __forceinline__ AttentionSegment attention_following(const AttentionP
   return g;
 }
 
+// The tile that a workgroup of attention_step began and others end: its segments (0: none), its first row of
+// q, its tokens and its head block.  Over a paged cache it is left in memory for the join, which finds it again from
+// the lengths otherwise: 15 sequences of four tokens 21.2 us, 23.8 without; one of 8000 keys, four tokens 24.2 and 25.4.
+struct AttentionBegun {
+  int segments, row, tokens, head_block;
+};
+// `seg`: the last that the workgroup took, up to `stop`.
+__device__ __forceinline__ AttentionBegun attention_begun(const AttentionParams& p, const AttentionLine& line, int b,
+                                                          const AttentionSegment& seg, uint32_t stop) {
+  if (!seg.it.live || seg.first || seg.count == seg.of) return AttentionBegun{};
+  const int segments = (int)((stop - seg.count + seg.of - 1) / line.quota) - (b >> (line.xcds == 8 ? 3 : 0)) + 1;
+  const int row = seg.it.tile * p.tile_tokens;
+  return AttentionBegun{segments, seg.it.seq.q0 + row, min(p.tile_tokens, seg.it.seq.nq - row), seg.it.head_block};
+}
+
 // In scalar registers, where the compiler does not see that the search is uniform.
 __device__ __forceinline__ AttentionSegment attention_scalar(const AttentionSegment& g) {
   auto u = [](int v) { return __builtin_amdgcn_readfirstlane(v); };

@@ -399,7 +399,7 @@ int64_t attention_workspace(const AttentionParams& params) {
 int64_t paged_attention_workspace(const AttentionParams& params, bool e4m3) {
   AttentionParams p = params;
   const AttentionPlan plan = paged_attention_plan(p, e4m3);
-  return workspace_of(p, plan);
+  return workspace_of(p, plan) + (plan.step && plan.join ? 16 * plan.grid : 0);
 }
 
 // false: the grid would pass HIP's limit, or a line of attention_step 2^32 units (its workgroups'
@@ -434,6 +434,7 @@ hipError_t launch_paged_attention(const AttentionParams& params, bool f16, void*
   // values stay above bf16's subnormals.
   attention_memory(p, plan, (int)kAttentionSlack, workspace);
   const bool codes = p.cache.scales != nullptr;
+  if (plan.step && plan.join) p.begun = reinterpret_cast<int32_t*>(p.part_ml + p.slots * plan.rows * 2);
   if (plan.step) {
     launch_attention_step(p, f16, codes ? kStoreE4M3 : kStorePages, (int)plan.grid, plan.waves, (int)plan.join, s);
     return hipGetLastError();

@@ -45,6 +45,7 @@ struct AttentionParams {
   int unit_shift;  // attention_step: log2 of a unit's keys (31: a whole sequence)
   float* part;  // [slot][row][d], then [slot][row] maxima and sums
   float* part_ml;
+  int32_t* begun;  // [workgroup][4], of a paged call: AttentionBegun
 };
 
 }  // namespace vfa

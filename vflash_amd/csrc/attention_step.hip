@@ -81,7 +81,7 @@ __global__ void __launch_bounds__(64 * W, STORE == kStoreE4M3 && DP <= 64 ? 4 : 
 
   const AttentionLine line = attention_line<PAGED>(p, gridDim.x);
   const uint32_t begin = (blockIdx.x >> (line.xcds == 8 ? 3 : 0)) * line.quota, stop = min(begin + line.quota, line.end);
-  [[maybe_unused]] AttentionSegment ended{};
+  [[maybe_unused]] AttentionSegment ended{};  // the last
   for (uint32_t pos = begin; pos < stop;) {
     const AttentionSegment seg = [&] {
       if constexpr (PAGED)
@@ -92,7 +92,7 @@ __global__ void __launch_bounds__(64 * W, STORE == kStoreE4M3 && DP <= 64 ? 4 : 
     }();
     if constexpr (PAGED) ended = seg;
     const AttentionItem& it = seg.it;
-    if (!it.live) return;
+    if (!it.live) break;
     const AttentionRow row = attention_row(p, it, fr);
     const int key_head = attention_key_head(p, it.head_block);
     const int last_token = min(it.seq.nq, (it.tile + 1) * p.tile_tokens) - 1;
@@ -301,6 +301,12 @@ __global__ void __launch_bounds__(64 * W, STORE == kStoreE4M3 && DP <= 64 ? 4 : 
     pos += seg.count;
     if (pos < stop) __syncthreads();  // the sums are read: the rings may be filled again
   }
+  if constexpr (PAGED) {
+    if (p.begun && threadIdx.x == 0) {
+      const AttentionBegun own = attention_begun(p, line, blockIdx.x, ended, stop);
+      *reinterpret_cast<v4i*>(p.begun + 4 * blockIdx.x) = v4i{own.segments, own.row, own.tokens, own.head_block};
+    }
+  }
 }
 
 // The sum over a tile's segments: out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s.  Workgroup b
@@ -308,17 +314,30 @@ __global__ void __launch_bounds__(64 * W, STORE == kStoreE4M3 && DP <= 64 ? 4 : 
 // 64 more, one row, every groups-th segment under a maximum of its own; the groups meet in LDS.
 template <bool F16, bool PAGED, int THREADS>
 __global__ void __launch_bounds__(THREADS) attention_step_join(const AttentionParams p) {
-  const AttentionLine line = attention_line<PAGED>(p, gridDim.x);
-  const int part = blockIdx.x >> (line.xcds == 8 ? 3 : 0);
-  const uint32_t begin = part * line.quota, stop = min(begin + line.quota, line.end);
-  if (begin >= stop) return;
-  const AttentionSegment seg = attention_segment<PAGED>(p, line, blockIdx.x, stop - 1, line.end);
-  const uint32_t tile_begin = stop - 1 - seg.first, tile_end = tile_begin + seg.of;
-  if (!seg.it.live || tile_begin < begin || tile_end <= stop) return;
-  const int segments = (int)((tile_end - 1) / line.quota) - part + 1;
+  AttentionItem it{};
+  int segments;
+  if constexpr (PAGED) {
+    const v4i begun = *reinterpret_cast<const v4i*>(p.begun + 4 * blockIdx.x);
+    auto u = [&](int i) { return __builtin_amdgcn_readfirstlane(begun[i]); };
+    segments = u(0);
+    if (segments == 0) return;
+    it.seq = AttentionSeq{u(1), 0, u(2), 0};
+    it.head_block = u(3);
+  } else {
+    const AttentionLine line = attention_line(p, gridDim.x);
+    const int part = blockIdx.x >> (line.xcds == 8 ? 3 : 0);
+    const uint32_t begin = part * line.quota, stop = min(begin + line.quota, line.end);
+    if (begin >= stop) return;
+    const AttentionSegment seg = attention_segment(p, line, blockIdx.x, stop - 1, line.end);
+    const uint32_t tile_begin = stop - 1 - seg.first, tile_end = tile_begin + seg.of;
+    if (!seg.it.live || tile_begin < begin || tile_end <= stop) return;
+    segments = (int)((tile_end - 1) / line.quota) - part + 1;
+    it = seg.it;
+  }
   // Segment s lies in workgroup blockIdx.x + xcds s, slot 1 for the first, 0 for the others.
-  auto slot = [&](int s) { return 2 * ((int64_t)blockIdx.x + line.xcds * s) + (s == 0); };
-  const int tokens = min(p.tile_tokens, seg.it.seq.nq - seg.it.tile * p.tile_tokens);
+  const int xcds = p.head_blocks % 8 == 0 ? 8 : 1;
+  auto slot = [&](int s) { return 2 * ((int64_t)blockIdx.x + xcds * s) + (s == 0); };
+  const int tokens = min(p.tile_tokens, it.seq.nq - it.tile * p.tile_tokens);
   const int rows = min(16, tokens * p.heads_per_tile);
   const int pow = rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 4 ? 4 : rows <= 8 ? 8 : 16;
   const int groups = min(16, THREADS / 16 / pow);
@@ -346,7 +365,7 @@ __global__ void __launch_bounds__(THREADS) attention_step_join(const AttentionPa
     mine[129] = top;
   }
   __syncthreads();
-  const AttentionRow row = attention_row(p, seg.it, r);
+  const AttentionRow row = attention_row(p, it, r);
   if (sg || !row.live) return;
   float all = top;
   for (int q = 1; q < groups; ++q) all = fmaxf(all, sums[q * pow + r][129]);
@@ -360,7 +379,7 @@ __global__ void __launch_bounds__(THREADS) attention_step_join(const AttentionPa
     l += other[128] * f;
   }
   const float inv = 1.0f / l;
-  uint16_t* dst = p.out + (int64_t)(seg.it.seq.q0 + row.token) * p.o_ts + (int64_t)row.head * p.o_hs;
+  uint16_t* dst = p.out + (int64_t)(it.seq.q0 + row.token) * p.o_ts + (int64_t)row.head * p.o_hs;
   static_for<2>([&](auto h) {
     const int d = 4 * e + 64 * h;
     const v4f y = l == 0 ? v4f{} : x[h] * inv;
