@@ -290,3 +290,27 @@ def test_autograd_notices_a_base_changed_in_place(dev):
             y.backward()
     with torch.inference_mode():
         add_request_adapters(make(dev, 9, 96), x, pack, index, inplace=True)
+
+
+@pytest.mark.parametrize("ranks", [[1, 7, 16], [64, 33, 0]], ids=str)
+@pytest.mark.parametrize("rows", [1, 17, 64, 65, 200, 513])
+def test_long_inputs(dev, rows, ranks):
+    # Two launches and three, where short inputs take one and two.
+    pack = stack(dev, ranks, 2056, (200, 72), BF16)
+    x, base, index = make(dev, rows, 2056, seed=1), make(dev, rows, 272, seed=2), indices(dev, rows, len(ranks), "mixed")
+    check(add_request_adapters(base, x, pack, index), base, x, pack, index)
+
+
+@pytest.mark.parametrize("rows", [1, 9, 100, 400])
+def test_the_input_is_the_base(dev, rows):
+    # In place on its own input: nothing of x is read after it was written.
+    pack = stack(dev, [16, 24], 1024, (1024,), BF16)
+    x, index = make(dev, rows, 1024, seed=1), indices(dev, rows, 2, "mixed")
+    want = add_request_adapters(x.clone(), x, pack, index)
+    check(want, x, x, pack, index)
+    own = x.clone()
+    add_request_adapters(own, own, pack, index, inplace=True)
+    check(own, x, x, pack, index)
+    wide = torch.cat((x, torch.zeros_like(x)), 1)  # the halves overlap in memory, row by row, but not in a value
+    add_request_adapters(wide[:, 1024:], wide[:, :1024], pack, index, inplace=True)
+    check(wide[:, 1024:], torch.zeros_like(x), x, pack, index)

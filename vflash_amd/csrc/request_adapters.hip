@@ -10,6 +10,7 @@
 //   request_up    adds the splits up in their order, keeps t of its item in LDS as two bf16, a high and a low part (16
 //                 bits of it or more, in binary32's range), and multiplies by B.  Binary16 factors of B are two bf16
 //                 as well, exactly.  scaling, base and one rounding follow.
+// Few rows of short inputs take both in one launch, request_few.
 // Nothing is added by atomics: a row's result does not depend on its company.
 // Bound by launches for a few rows, by the adapters' bytes for a decoding batch, and by base and out for prompts.
 #include "request_adapters.h"
@@ -24,6 +25,7 @@ int compute_units();
 
 namespace {
 
+typedef int v2i __attribute__((ext_vector_type(2)));
 constexpr int RD_WAVES = 8;  // of request_down: parts of K
 constexpr int RU_WAVES = 4;  // of request_up: column tiles
 
@@ -254,24 +256,112 @@ __global__ void __launch_bounds__(64 * RD_WAVES) request_down(const RequestAdapt
   });
 }
 
-// Tiles of 64 columns of one branch and item, ranks in NC runs of 32.  MFMA block j of a tile holds the columns
-// 32 (j / 2) + 8 g + 4 (j % 2) + e in its rows 4 g + e, so that a lane ends with two runs of eight columns of one row, and
-// the four lanes of a row store 64 bytes at once.
+namespace {
+
+// A branch's columns: those of workgroup `group` of the call's groups.
+struct RequestColumns {
+  int branch, group, first, stop;
+};
+__device__ __forceinline__ RequestColumns request_columns(const RequestAdapterParams& p, int group) {
+  int branch = 0;
+  while (branch + 1 < p.branches && group >= p.groups[branch]) ++branch;
+  if (branch) group -= p.groups[branch - 1];
+  return RequestColumns{branch, group, branch ? p.ends[branch - 1] : 0, p.ends[branch]};
+}
+
+// A wave's tile of 64 columns of one branch and item (RB blocks of 16 rows), ranks in NC runs of 32.  MFMA block j
+// holds the columns 32 (j / 2) + 8 g + 4 (j % 2) + e in its rows 4 g + e, so that a lane ends with two runs of eight columns
+// of one row, and the four lanes of a row store 64 bytes at once.
+template <bool F16, int RB, int NC>
+struct RequestTile {
+  static constexpr int PITCH = 64 * NC + 8;  // of a row in LDS: high parts, low parts, and eight against bank conflicts
+  v4i b[NC][4], base[RB][2];
+  int64_t row[RB];
+
+  __device__ __forceinline__ void load(const RequestAdapterParams& p, const RequestItem& it, const int* rows, int n0, int stop) {
+    const int lane = (int)threadIdx.x & 63, fr = lane & 15, fg = lane >> 4;
+    const int n = n0 + 8 * fg;  // this lane's columns: n .. n + 7 and 32 further, up to stop
+    static_for<NC>([&](auto c) {
+      const int r = c * 32 + 8 * fg;
+      static_for<4>([&](auto j) {
+        const int col = n0 + 32 * (j / 2) + 8 * (fr >> 2) + 4 * (j % 2) + (fr & 3);
+        b[c][j] = r < it.rank && col < stop
+                      ? *reinterpret_cast<const v4i*>(p.up + ((int64_t)it.adapter * p.n + col) * p.width + r) : v4i{};
+      });
+    });
+    static_for<RB>([&](auto i) {
+      if (16 * i >= it.count) return;
+      row[i] = rows[min(16 * (int)i + fr, it.count - 1)];
+      static_for<2>([&](auto h) {
+        base[i][h] = n + 32 * h < stop ? *reinterpret_cast<const v4i*>(p.base + row[i] * p.ldb + n + 32 * h) : v4i{};
+      });
+    });
+  }
+
+  __device__ __forceinline__ void store(const RequestAdapterParams& p, const RequestItem& it, const uint16_t* low_rank,
+                                        float scaling, int n0, int stop) {
+    const int lane = (int)threadIdx.x & 63, fr = lane & 15, fg = lane >> 4;
+    const int n = n0 + 8 * fg;
+    v4i rest[NC][4];
+    if constexpr (F16)
+      static_for<NC>([&](auto c) {
+        static_for<4>([&](auto j) {
+          static_for<4>([&](auto e) {
+            const uint32_t w = (uint32_t)b[c][j][(int)e];
+            int high, low;
+            parts(widen<true>(w, 0), widen<true>(w, 1), high, low);
+            b[c][j][(int)e] = high;
+            rest[c][j][(int)e] = low;
+          });
+        });
+      });
+    static_for<RB>([&](auto i) {
+      if (16 * i >= it.count) return;
+      v4f acc[4];
+      static_for<4>([&](auto j) { acc[j] = v4f{}; });
+      const uint16_t* src = low_rank + min(16 * (int)i + fr, it.count - 1) * PITCH + 8 * fg;
+      static_for<NC>([&](auto c) {
+        if (c * 32 >= it.rank) return;
+        const v4i high = *reinterpret_cast<const v4i*>(src + c * 32), low = *reinterpret_cast<const v4i*>(src + 32 * NC + c * 32);
+        static_for<4>([&](auto j) {
+          acc[j] = mfma16<false>(b[c][j], high, acc[j]);
+          acc[j] = mfma16<false>(b[c][j], low, acc[j]);
+        });
+        if constexpr (F16) {
+          const v4i near = finite(high);  // an infinity is in the first product
+          static_for<4>([&](auto j) { acc[j] = mfma16<false>(rest[c][j], near, acc[j]); });
+        }
+      });
+      if (16 * i + fr >= it.count) return;
+      static_for<2>([&](auto h) {
+        if (n + 32 * h >= stop) return;
+        v4i o;
+        static_for<4>([&](auto e) {
+          constexpr int at = 8 * h + 2 * e;
+          const uint32_t w = (uint32_t)base[i][h][(int)e];
+          o[(int)e] = pack<F16>(__builtin_fmaf(acc[at / 4][at % 4], scaling, widen<F16>(w, 0)),
+                                __builtin_fmaf(acc[at / 4][at % 4 + 1], scaling, widen<F16>(w, 1)));
+        });
+        *reinterpret_cast<v4i*>(p.out + row[i] * p.ldo + n + 32 * h) = it.rank > 0 ? o : base[i][h];
+      });
+    });
+  }
+};
+
+}  // namespace
+
+// out from t, four tiles of columns and an item a workgroup.
 template <bool F16, int NC>
 __global__ void __launch_bounds__(64 * RU_WAVES) request_up(const RequestAdapterParams p) {
-  constexpr int PITCH = 64 * NC + 8;  // of a row in LDS: high parts, low parts, and eight against bank conflicts
+  using Tile = RequestTile<F16, 4, NC>;
   __shared__ int rows[64];
-  __shared__ __attribute__((aligned(16))) uint16_t low_rank[64 * PITCH];
+  __shared__ __attribute__((aligned(16))) uint16_t low_rank[64 * Tile::PITCH];
   const RequestItem it = uniform(request_listed(p, (int)blockIdx.y, rows));
   __syncthreads();
   if (it.count == 0) return;
-  const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int fr = lane & 15, fg = lane >> 4;
-  int branch = 0, group = (int)blockIdx.x;
-  while (branch + 1 < p.branches && group >= p.groups[branch]) ++branch;
-  if (branch) group -= p.groups[branch - 1];
-  const int first_col = branch ? p.ends[branch - 1] : 0, stop = p.ends[branch];
-  const float scaling = it.adapter < 0 ? 0.0f : p.scaling[it.adapter * p.branches + branch];
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const RequestColumns columns = request_columns(p, (int)blockIdx.x);
+  const float scaling = it.adapter < 0 ? 0.0f : p.scaling[it.adapter * p.branches + columns.branch];
 
   // t, eight ranks a thread; zeros past the rank.
   if (it.rank > 0) {
@@ -280,7 +370,7 @@ __global__ void __launch_bounds__(64 * RU_WAVES) request_up(const RequestAdapter
       const int row = e / (4 * NC), r = e % (4 * NC) * 8;
       v4f x[2] = {v4f{}, v4f{}};
       if (r < it.rank) {
-        const float* src = p.t + (int64_t)rows[row] * all + branch * p.width + r;
+        const float* src = p.t + (int64_t)rows[row] * all + columns.branch * p.width + r;
 #pragma unroll 4
         for (int s = 0; s < p.splits; ++s, src += p.rows * all) {
           x[0] += *reinterpret_cast<const v4f*>(src);
@@ -294,75 +384,78 @@ __global__ void __launch_bounds__(64 * RU_WAVES) request_up(const RequestAdapter
         high[(int)i] = h;
         low[(int)i] = l;
       });
-      *reinterpret_cast<v4i*>(low_rank + row * PITCH + r) = high;
-      *reinterpret_cast<v4i*>(low_rank + row * PITCH + 32 * NC + r) = low;
+      *reinterpret_cast<v4i*>(low_rank + row * Tile::PITCH + r) = high;
+      *reinterpret_cast<v4i*>(low_rank + row * Tile::PITCH + 32 * NC + r) = low;
     }
   }
   __syncthreads();
 
-  const int n0 = first_col + (group * RU_WAVES + wave) * 64;
-  if (n0 >= stop) return;
-  const int n = n0 + 8 * fg;  // this lane's columns: n .. n + 7 and 32 further, up to stop
-  v4i b[NC][4], rest[NC][4];
-  static_for<NC>([&](auto c) {
-    const int r = c * 32 + 8 * fg;
-    static_for<4>([&](auto j) {
-      const int col = n0 + 32 * (j / 2) + 8 * (fr >> 2) + 4 * (j % 2) + (fr & 3);
-      b[c][j] = r < it.rank && col < stop
-                    ? *reinterpret_cast<const v4i*>(p.up + ((int64_t)it.adapter * p.n + col) * p.width + r) : v4i{};
+  const int n0 = columns.first + (columns.group * RU_WAVES + wave) * 64;
+  if (n0 >= columns.stop) return;
+  Tile tile;
+  tile.load(p, it, rows, n0, columns.stop);
+  tile.store(p, it, low_rank, scaling, n0, columns.stop);
+}
+
+// Both products in one launch, for up to 64 rows and small A: eight tiles of columns and an item of 16 rows a workgroup, each
+// of which forms t of its branch for itself, RK blocks of 16 ranks.  x must not overlap out.
+template <bool F16, int RK>
+__global__ void __launch_bounds__(64 * RD_WAVES) request_few(const RequestAdapterParams p) {
+  constexpr int NC = (RK + 1) / 2;
+  using Tile = RequestTile<F16, 1, NC>;
+  __shared__ int rows[16];
+  __shared__ v4f part[RD_WAVES][RK][64];
+  __shared__ __attribute__((aligned(16))) uint16_t low_rank[16 * Tile::PITCH];
+  const RequestItem it = uniform(p.rows > RA_WAVE_ROWS ? request_listed(p, (int)blockIdx.y, rows) : request_find(p, (int)blockIdx.y, rows));
+  __syncthreads();
+  if (it.count == 0) return;
+  const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int fr = lane & 15, fg = lane >> 4;
+  const RequestColumns columns = request_columns(p, (int)blockIdx.x);
+  const int n0 = columns.first + (columns.group * RD_WAVES + wave) * 64;
+  const float scaling = it.adapter < 0 ? 0.0f : p.scaling[it.adapter * p.branches + columns.branch];
+  Tile tile;
+  tile.load(p, it, rows, n0, columns.stop);  // on its way beside A and x
+  if (it.rank > 0) {
+    const uint16_t* xr = p.x + (int64_t)rows[min(fr, it.count - 1)] * p.ldx;
+    const uint16_t* ar[RK];
+    static_for<RK>([&](auto j) {
+      ar[j] = p.down + (((int64_t)it.adapter * p.branches + columns.branch) * p.width + min(j * 16 + fr, p.width - 1)) * p.k;
     });
-  });
-  int64_t row[4];
-  v4i base[4][2];
-  static_for<4>([&](auto i) {
-    if (16 * i >= it.count) return;
-    row[i] = rows[min(16 * (int)i + fr, it.count - 1)];
-    static_for<2>([&](auto h) {
-      base[i][h] = n + 32 * h < stop ? *reinterpret_cast<const v4i*>(p.base + row[i] * p.ldb + n + 32 * h) : v4i{};
-    });
-  });
-  if constexpr (F16)
-    static_for<NC>([&](auto c) {
-      static_for<4>([&](auto j) {
-        static_for<4>([&](auto e) {
-          const uint32_t w = (uint32_t)b[c][j][(int)e];
-          int high, low;
-          parts(widen<true>(w, 0), widen<true>(w, 1), high, low);
-          b[c][j][(int)e] = high;
-          rest[c][j][(int)e] = low;
-        });
+    const int steps = (int)((p.k + 31) / 32), s0 = steps * wave / RD_WAVES, s1 = steps * (wave + 1) / RD_WAVES;
+    constexpr int AHEAD = RK == 1 ? 16 : 8;
+    v4f acc[RK];
+    static_for<RK>([&](auto j) { acc[j] = v4f{}; });
+    for (int s = s0; s < s1; s += AHEAD) {
+      v4i xv[AHEAD], av[AHEAD][RK];
+      static_for<AHEAD>([&](auto a) {
+        const int64_t at = (int64_t)(s + a) * 32 + fg * 8;
+        const bool ok = s + a < s1 && at < p.k;
+        xv[a] = ok ? *reinterpret_cast<const v4i*>(xr + at) : v4i{};
+        static_for<RK>([&](auto j) { av[a][j] = ok && j * 16 < it.rank ? *reinterpret_cast<const v4i*>(ar[j] + at) : v4i{}; });
       });
-    });
-  static_for<4>([&](auto i) {
-    if (16 * i >= it.count) return;
-    v4f acc[4];
-    static_for<4>([&](auto j) { acc[j] = v4f{}; });
-    const uint16_t* src = low_rank + min(16 * (int)i + fr, it.count - 1) * PITCH + 8 * fg;
-    static_for<NC>([&](auto c) {
-      if (c * 32 >= it.rank) return;
-      const v4i high = *reinterpret_cast<const v4i*>(src + c * 32), low = *reinterpret_cast<const v4i*>(src + 32 * NC + c * 32);
-      static_for<4>([&](auto j) {
-        acc[j] = mfma16<false>(b[c][j], high, acc[j]);
-        acc[j] = mfma16<false>(b[c][j], low, acc[j]);
+      static_for<AHEAD>([&](auto a) { static_for<RK>([&](auto j) { acc[j] = mfma16<F16>(av[a][j], xv[a], acc[j]); }); });
+    }
+    static_for<RK>([&](auto j) { part[wave][j][lane] = acc[j]; });
+    __syncthreads();
+    // Wave j: t of row fr, ranks 16 j + 4 fg + 0 .. 3, zeros past the rank.
+    if (wave < 2 * NC) {
+      const int r = 16 * wave + 4 * fg;
+      v4f sum = v4f{};
+      if (wave < RK) static_for<RD_WAVES>([&](auto w) { sum += part[w][wave][lane]; });
+      v2i high, low;
+      static_for<2>([&](auto i) {
+        int h, l;
+        parts(r + 2 * i < it.rank ? sum[2 * i] : 0.0f, r + 2 * i + 1 < it.rank ? sum[2 * i + 1] : 0.0f, h, l);
+        high[(int)i] = h;
+        low[(int)i] = l;
       });
-      if constexpr (F16) {
-        const v4i near = finite(high);  // an infinity is in the first product
-        static_for<4>([&](auto j) { acc[j] = mfma16<false>(rest[c][j], near, acc[j]); });
-      }
-    });
-    if (16 * i + fr >= it.count) return;
-    static_for<2>([&](auto h) {
-      if (n + 32 * h >= stop) return;
-      v4i o;
-      static_for<4>([&](auto e) {
-        constexpr int at = 8 * h + 2 * e;
-        const uint32_t w = (uint32_t)base[i][h][(int)e];
-        o[(int)e] = pack<F16>(__builtin_fmaf(acc[at / 4][at % 4], scaling, widen<F16>(w, 0)),
-                              __builtin_fmaf(acc[at / 4][at % 4 + 1], scaling, widen<F16>(w, 1)));
-      });
-      *reinterpret_cast<v4i*>(p.out + row[i] * p.ldo + n + 32 * h) = it.rank > 0 ? o : base[i][h];
-    });
-  });
+      *reinterpret_cast<v2i*>(low_rank + fr * Tile::PITCH + r) = high;
+      *reinterpret_cast<v2i*>(low_rank + fr * Tile::PITCH + 32 * NC + r) = low;
+    }
+  }
+  __syncthreads();
+  if (n0 < columns.stop) tile.store(p, it, low_rank, scaling, n0, columns.stop);
 }
 
 namespace {
@@ -392,6 +485,29 @@ void request_plan(RequestAdapterParams& p) {
   p.splits = (int)((steps + p.steps - 1) / p.steps);
 }
 
+// Groups of `columns` columns of one branch.
+int request_grouped(RequestAdapterParams& p, int columns) {
+  int groups = 0;
+  for (int b = 0; b < p.branches; ++b) {
+    groups += (p.ends[b] - (b ? p.ends[b - 1] : 0) + columns - 1) / columns;
+    p.groups[b] = groups;
+  }
+  return groups;
+}
+
+// Whether request_few takes the call: a launch less, but every workgroup reads A of its item and branch, of which a CU gets
+// 33 bytes a ns.  us with and without, one projection: 1 row, K 1536, rank 16 6.6, 9.3, rank 32 8.6, 10.0, rank 64 11.7,
+// 11.1; K 1024, rank 64 10.1, 10.9; K 5120, rank 16 10.7, 9.6.  40 rows of 20 adapters, K 1536, rank 32 12.0, 13.5.  100 rows of
+// 4, K 1536, rank 16 11.1, 12.9, rank 32 13.4, 13.4; K 2048, rank 16 12.3, 11.4.  600 rows, 440 workgroups 17.3, 14.1.
+bool request_alone(RequestAdapterParams& p) {
+  const int64_t most = p.rows > RA_WAVE_ROWS ? 32768 : 65536;
+  if (p.item_rows > 16 || p.width > 64 || p.k > 1536 || p.k * p.width > most) return false;
+  if (4 * (int64_t)p.items * request_grouped(p, 64 * RD_WAVES) > 5 * compute_units()) return false;
+  // Its workgroups read x while others write.
+  const uint16_t *x = p.x, *x_end = x + (p.rows - 1) * p.ldx + p.k, *out = p.out, *out_end = out + (p.rows - 1) * p.ldo + p.n;
+  return x_end <= out || out_end <= x;
+}
+
 // Values of t.
 int64_t request_low_ranks(const RequestAdapterParams& p) { return (int64_t)p.splits * p.rows * p.branches * p.width; }
 
@@ -411,12 +527,19 @@ hipError_t launch_request_adapters(const RequestAdapterParams& params, bool f16,
   p.order = p.list + 4 * (int64_t)p.items;
   p.before = p.order + (int64_t)p.items * p.item_rows;
   if (p.rows > RA_WAVE_ROWS) request_groups<<<1, 1024, 4 * (p.adapters + 1), s>>>(p);
-  const int ranks = request_ranks(p);
-  int groups = 0;
-  for (int b = 0; b < p.branches; ++b) {
-    groups += (p.ends[b] - (b ? p.ends[b - 1] : 0) + 64 * RU_WAVES - 1) / (64 * RU_WAVES);
-    p.groups[b] = groups;
+  if (request_alone(p)) {
+    const dim3 grid((unsigned)request_grouped(p, 64 * RD_WAVES), (unsigned)p.items);
+    auto few = [&](auto type) {
+      constexpr bool F16 = type;
+      if (p.width <= 16) request_few<F16, 1><<<grid, 64 * RD_WAVES, 0, s>>>(p);
+      else if (p.width <= 32) request_few<F16, 2><<<grid, 64 * RD_WAVES, 0, s>>>(p);
+      else request_few<F16, 4><<<grid, 64 * RD_WAVES, 0, s>>>(p);
+    };
+    if (f16) few(std::true_type{});
+    else few(std::false_type{});
+    return hipGetLastError();
   }
+  const int ranks = request_ranks(p), groups = request_grouped(p, 64 * RU_WAVES);
   const dim3 down((unsigned)p.items, (unsigned)p.splits, (unsigned)((p.branches * p.width + ranks - 1) / ranks));
   // An item's columns next to each other: 4093 rows 83.4 us, with the items next to each other 85.5.
   const dim3 up((unsigned)groups, (unsigned)p.items);
