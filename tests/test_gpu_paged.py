@@ -68,13 +68,9 @@ def attended(cache, q, table, lengths, q_offsets, got, scale=None):
     if cache.scales is None:
         check(got, q, k.to(q.dtype), v.to(q.dtype), qo, ko, causal=True, scale=scale)
         return
-    # E4M3: weights round to bf16 whatever q's type, and normalise unrounded; a factor's product is one
-    # binary32 rounding more in a score and in a weight.
-    want, bound = packed_attention(q.to(torch.bfloat16) if q.dtype == BF16 else q, k, v, qo, ko, causal=True, scale=scale)
-    if q.dtype == F16:
-        # The reference's bound has binary16's half step of each weight: bf16's is eight of them.
-        _, spread = packed_attention(q, k, v.abs(), qo, ko, causal=True, scale=scale)
-        bound = 8 * spread
+    # E4M3: weights round to bf16, for f16 to two of it (2^-17, inside binary16's half step), and normalise unrounded; a
+    # factor's product is one binary32 rounding more in a score and in a weight.
+    want, bound = packed_attention(q, k, v, qo, ko, causal=True, scale=scale)
     got = got.cpu().double()
     assert bool(torch.isfinite(got).all())
     worst = ((got - want).abs() - bound).max().item()

@@ -21,7 +21,8 @@
 //
 // A paged cache differs in where a wave's part of a tile comes from: rows of one 16 keys, which lie in one page.
 // E4M3 codes go through registers, a tile ahead, and reach LDS as 16-bit numbers (exactly), converted once for
-// all waves; a key's factor multiplies its score, a value's its weight before that is rounded, to bf16.
+// all waves; a key's factor multiplies its score, a value's its weight before that is rounded, to bf16
+// (for f16 queries to two of it).
 #include "attention_codes.h"
 #include "attention_plan.h"
 
@@ -240,6 +241,7 @@ __global__ void __launch_bounds__(64 * WAVES, (DP <= 64 ? 4 : 3) - (STORE == kSt
       });
     }
     v4i pk[2 * L::KB];
+    [[maybe_unused]] v4i rest[E4M3 && F16 ? 2 * L::KB : 1];
     float sum;
     auto weights = [&](auto far_rows) {
       const float ref = attention_shift<W16>(p) - attention_top(m, p.c);
@@ -252,6 +254,7 @@ __global__ void __launch_bounds__(64 * WAVES, (DP <= 64 ? 4 : 3) - (STORE == kSt
           if constexpr (E4M3) {
             const v2f f = *reinterpret_cast<const v2f*>(&factors[buf][1][st / 2 * 32 + 8 * (r / 4) + 4 * fh + r % 4]);
             pk[st][(int)j] = pack2<W16>(w0 * f[0], w1 * f[1]);
+            if constexpr (F16) rest[st][(int)j] = attention_rest(w0 * f[0], w1 * f[1], pk[st][(int)j]);
             sum += w0 + w1;
           } else {
             pk[st][(int)j] = pack2<W16>(w0, w1);
@@ -280,6 +283,7 @@ __global__ void __launch_bounds__(64 * WAVES, (DP <= 64 ? 4 : 3) - (STORE == kSt
         const uint8_t* src = vrow + buf * L::SLOT + st * 16 * L::PITCH + (((4 * db + vc) ^ vsw) << 4);
         const v2i lo = lds_read_tr16(src), hi = lds_read_tr16(src + 8 * L::PITCH);
         o[db] = mfma32<W16>(v4i{lo[0], lo[1], hi[0], hi[1]}, pk[st], o[db]);
+        if constexpr (E4M3 && F16) o[db] = mfma32<W16>(v4i{lo[0], lo[1], hi[0], hi[1]}, rest[st], o[db]);
       });
     });
     after();

@@ -17,4 +17,10 @@ __device__ __forceinline__ v4i attention_widen(v2i c) {
   return w;
 }
 
+// What two bf16 leave of the weights that they were rounded from, as bf16: f16 queries take both, so that their
+// results keep f16's precision (16 bits of a weight; binary32's range, which factors need).
+__device__ __forceinline__ int attention_rest(float a, float b, int rounded) {
+  return pack2<false>(a - bf16_lo((uint32_t)rounded), b - bf16_hi((uint32_t)rounded));
+}
+
 }  // namespace vfa

@@ -14,7 +14,7 @@
 // A paged cache differs in where a block's keys come from: each 16 lie in one page, whose number a scalar
 // load fetches one block ahead.  E4M3 codes go to LDS as they are, with their factors, and become 16 bits between
 // LDS and the matrix cores (exactly): a key's factor multiplies its score, a value's its weight before that is
-// rounded, to bf16 whatever q's type (a factor has binary32's range).
+// rounded, to bf16 whatever q's type (a factor has binary32's range); for f16 to two of it.
 #include "attention_codes.h"
 
 namespace vfa {
@@ -228,6 +228,7 @@ __global__ void __launch_bounds__(64 * W, STORE == kStoreE4M3 && DP <= 64 ? 4 : 
       }
       const float ref = attention_shift<W16>(p) - attention_top(m, p.c);
       v4i pk;
+      [[maybe_unused]] v4i rest;
       auto weights = [&](auto far_rows) {
         static_for<4>([&](auto j) {
           constexpr int r = (j % 2) * 2;
@@ -236,6 +237,7 @@ __global__ void __launch_bounds__(64 * W, STORE == kStoreE4M3 && DP <= 64 ? 4 : 
           if constexpr (E4M3) {
             const v2f f = *reinterpret_cast<const v2f*>(factors + buf * L::SLOT + (j / 2) * 256 + 64 + r * 4);
             pk[(int)j] = pack2<W16>(w0 * f[0], w1 * f[1]);
+            if constexpr (F16) rest[(int)j] = attention_rest(w0 * f[0], w1 * f[1], pk[(int)j]);
             l += w0 + w1;
           } else {
             pk[(int)j] = pack2<W16>(w0, w1);
@@ -249,6 +251,7 @@ __global__ void __launch_bounds__(64 * W, STORE == kStoreE4M3 && DP <= 64 ? 4 : 
         if constexpr (E4M3) {
           const v4i a = attention_widen<false>(lds_read_tr8(vrow + buf * L::SLOT + ((db ^ vsw) << 4)));
           o[db] = mfma16<W16>(a, pk, o[db]);
+          if constexpr (F16) o[db] = mfma16<W16>(a, rest, o[db]);
         } else {
           const uint8_t* src = vrow + buf * L::SLOT + (((2 * db + vc) ^ vsw) << 4);
           const v2i lo = lds_read_tr16(src), hi = lds_read_tr16(src + 16 * L::PITCH);
