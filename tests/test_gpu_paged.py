@@ -204,6 +204,21 @@ def test_head_dimensions(dev, dim):
             attended(cache, q, table, [45, 900], qo, paged_attention(q, cache, table, n, q_offsets=qo))
 
 
+@pytest.mark.parametrize("dtype,store", [(BF16, BF16), (F16, F16), (BF16, E4M3), (F16, E4M3)])
+@pytest.mark.parametrize("dim,page,new", [(128, 16, 1), (64, 32, 1), (96, 64, 2), (128, 256, 1)])
+def test_many_short_sequences(dev, dim, page, new, dtype, store):
+    # More tiles than twice what the GPU holds, of up to 256 keys: workgroups of one wave.
+    batch, heads = (230, 9) if dim <= 64 else (130, 9)
+    rng = random.Random(dim)
+    lengths = [rng.choice((0, 1, page - 1, page, rng.randint(1, page))) for _ in range(batch)]
+    cache, table = pool(dev, lengths, page, heads, dim, store)
+    news = [1] * batch if new == 1 else [min(new, n) for n in lengths]
+    qo = None if new == 1 else offsets(news, dev)
+    q = make(dev, sum(news), heads, dim, dtype=dtype, std=2.0)
+    got = paged_attention(q, cache, table, torch.tensor(lengths, device=dev), q_offsets=qo)
+    attended(cache, q, table, lengths, qo, got)
+
+
 @pytest.mark.parametrize("page", [16, 32, 64, 256, 1024, 4096])
 @pytest.mark.parametrize("store", [BF16, E4M3])
 def test_pages(dev, page, store):

@@ -407,7 +407,8 @@ void launch_attention_step(const AttentionParams& p, bool f16, AttentionStore st
     else launch_step<false, stored, w>(p, grid, join, s);
   };
   auto paged = [&](auto stored) {
-    if (waves == 2) of(stored, std::integral_constant<int, 2>{});
+    if (waves == 1) of(stored, std::integral_constant<int, 1>{});
+    else if (waves == 2) of(stored, std::integral_constant<int, 2>{});
     else of(stored, std::integral_constant<int, 4>{});
   };
   if (store == kStoreE4M3) paged(std::integral_constant<int, kStoreE4M3>{});
