@@ -528,8 +528,8 @@ int vflash_paged_append(const void* q, int64_t q_ts, int64_t q_hs, const void* k
  * Attention of new tokens over a paged cache that holds them already: vflash_packed_attention, causal, with the keys and
  * values of vflash_paged_append.  No reference counterpart.
  *   q_offsets, values, scales, table, lengths, batch as there; out as vflash_packed_attention
- *   With scales, a key's factor multiplies its score and a value's its weight before that is rounded to bf16; values
- *   whose factors are below 2^-117 times width * page may lose bits.
+ *   With scales, a key's factor multiplies its score and a value's its weight before that is rounded to bf16 (for f16 to
+ *   two bf16, which carry 16 bits); values whose factors are below 2^-100 times width * page may lose bits.
  * Lengths are clamped to the table.  Keys on a page outside [0, pages) count as keys and values of zeros.  Nothing
  * else outside a sequence's pages is read.  Masked keys, rows that see none, and scores as vflash_packed_attention.
  *   workspace  vflash_paged_attention_workspace(...) bytes (e4m3: with scales; 0: may be NULL), 16-byte aligned,

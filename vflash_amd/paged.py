@@ -147,7 +147,7 @@ def paged_attention(q, cache: PagedCache, table, lengths, *, q_offsets=None, sca
 
     Single tokens and a few run in tiles of 16 rows (token and head), whole prompts and pieces of prompts in
     tiles of 128, as in ``packed_attention``.  Softmax and sums are binary32; weights are rounded to the operands'
-    type, to bf16 after the values' scales with an E4M3 cache.  As there, infinities and
+    type; with an E4M3 cache to bf16 after the values' scales, for f16 queries to two bf16.  As there, infinities and
     NaN in the values of a sequence can reach its masked queries as NaN.  Inference only.
     """
     if isinstance(q, torch.Tensor) and q.is_cuda and isinstance(cache, PagedCache):
