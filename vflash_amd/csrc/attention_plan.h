@@ -98,10 +98,10 @@ inline AttentionPlan paged_attention_plan(AttentionParams& p, bool e4m3) {
   // More whole sequences than the GPU holds go in workgroups of two waves, twice as many: 128 of 250 keys in bf16 32 us, in
   // four waves 42; of 700 70 and 75; 64 of 250 in E4M3, which fit, 13.2 and 12.7.
   plan.waves = !split && tiles > held ? 2 : 4;
-  // More than twice as many, of little room, in workgroups of one wave, four times as many: 86 of up to 32 keys, 56 heads of
-  // their own, in bf16 30 us, of two waves 50; of 250 94 and 108; of 500 174 and 170.  120 of 32, 8 key heads, 9.3, 13.1.
+  // More than twice as many, of little room, in workgroups of one wave: 86 of up to 32 keys, 56 heads of their own, in bf16
+  // 21 us, of two waves 50; of 250 93 and 108; of 500, of one with two slots, 174 and 170.  120 of 32, 8 key heads, 8.7, 13.1.
   if (!split && tiles > 2 * held && p.keys <= 256) plan.waves = 1;
-  attention_step_plan(p, plan, split, per_cu * 4 / plan.waves);
+  attention_step_plan(p, plan, split, plan.waves == 1 ? (p.dim <= 64 ? 16 : 8) : per_cu * 4 / plan.waves);
   // Of several tokens a sequence a workgroup takes two units at least, half as many segments for their join: four tokens after
   // 8000 keys in E4M3 18.6 us, by single units 22.0, after 2000 14.3 either way; one token of 2000 keys 14.4 and 13.7.
   p.least_units = split && p.tokens > p.batch ? 2 : 1;
