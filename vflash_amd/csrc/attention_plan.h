@@ -82,16 +82,26 @@ inline bool attention_few_rows(const AttentionParams& p) {
 // keys 117 us, 129 with one.
 inline AttentionPlan paged_attention_plan(AttentionParams& p, bool e4m3) {
   AttentionPlan plan{};
+  attention_shape(p, plan, true);
+  // About how many tiles of 16 there are: whole ones, or one a sequence.
+  int64_t tiles = p.batch < p.tokens ? p.batch : p.tokens;
+  if (tiles < p.tokens / p.tile_tokens) tiles = p.tokens / p.tile_tokens;
+  tiles *= p.head_blocks;
+  // Beside the few rows of packed attention, drafts and short pieces whose tiles of 16 are so few that reading K and V
+  // again for each costs less than the long chain of a tile of 128.  us in tiles of 16 and of 128: bf16, 8 query heads a key
+  // head, 1 sequence of 500 keys, 5 tokens 11.5 16.0, 4 of 2000 15.5 24.9, of 8000 22.6 28.3, 16 of 2000, 12 tokens (96 tiles)
+  // 28.3 26.9; 100 keys 8.3 7.5; E4M3, 32 heads over 8, 16 of 2000 keys, 16 tokens 42.7 45.7, 8 of 1000, 64 tokens 31.2 43.1, 128
+  // tokens (2048 tiles) 60.8 54.5, 8 of 4000, 24 tokens 48.9 46.5; up to 64 rows of 128 at any length, 16 of 8000, 9 tokens 97 145.
   attention_shape(p, plan, false);
-  if (!attention_few_rows(p)) {
+  const bool few = attention_few_rows(p);
+  const bool drafts = (int64_t)p.tokens * p.group <= 64 * p.batch;
+  const bool pieces = e4m3 ? tiles <= 4 * compute_units() && (drafts || tiles * p.keys <= 1 << 20)
+                           : 2 * tiles <= compute_units() && tiles * p.keys <= 163840 && p.keys > 128;
+  if (!few && !pieces) {
     attention_tiles_plan(p, plan);
     return plan;
   }
   attention_shape(p, plan, true);
-  // About how many tiles there are: whole ones, or one a sequence.
-  int64_t tiles = p.batch < p.tokens ? p.batch : p.tokens;
-  if (tiles < p.tokens / p.tile_tokens) tiles = p.tokens / p.tile_tokens;
-  tiles *= p.head_blocks;
   const int per_cu = (p.dim <= 64 ? 2 : 1) * (e4m3 ? 2 : 1);
   const int64_t held = (int64_t)compute_units() * per_cu;
   const bool split = p.keys > (2 * tiles < held ? 768 : 1536);
