@@ -128,7 +128,7 @@ SIZES = {
     "many": (150, 131072, 150, 4, 4, 64), "very many": (4200, 4096, 4200, 2, 2, 64), "several": (90, 4096, 20, 8, 4, 64), "wide group": (3, 4096, 3, 40, 40, 64),
     "drafts, wide group": (9, 4096, 3, 40, 40, 64), "no sequence": (5, 4096, 0, 4, 2, 64), "a piece": (60, 512, 1, 32, 4, 128),
     "tiles, wide group": (300, 4096, 3, 40, 40, 64), "tiles, no sequence": (5000, 4096, 0, 4, 2, 64), "tiles": (900, 4096, 2, 8, 8, 128), "tiles, several": (700, 8192, 5, 8, 1, 64),
-    "tiles, many": (3000, 2048, 100, 4, 2, 64), "tiles, not split": (6000, 512, 9, 7, 7, 64),
+    "tiles, many": (4000, 2048, 100, 4, 2, 64), "tiles, not split": (6000, 512, 9, 7, 7, 64),
 }
 
 
