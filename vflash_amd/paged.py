@@ -145,7 +145,7 @@ def paged_attention(q, cache: PagedCache, table, lengths, *, q_offsets=None, sca
     prompt or its next piece): token ``i`` of ``n`` sees the sequence's first ``lengths[b] - n + i + 1`` tokens.  Rows that
     see none, and rows outside every sequence, are zeros.  ``scale`` defaults to ``dim ** -0.5``.
 
-    Single tokens and a few run in tiles of 16 rows (token and head), whole prompts and pieces of prompts in
+    Single tokens, drafts and short pieces run in tiles of 16 rows (token and head), prompts and longer pieces in
     tiles of 128, as in ``packed_attention``.  Softmax and sums are binary32; weights are rounded to the operands'
     type; with an E4M3 cache to bf16 after the values' scales, for f16 queries to two bf16.  As there, infinities and
     NaN in the values of a sequence can reach its masked queries as NaN.  Inference only.
