@@ -1,0 +1,52 @@
+"""What a serving step keeps can be copied, deep-copied and pickled, as the modules that hold it are."""
+
+import copy
+import io
+import pickle
+
+import pytest
+import torch
+
+from vflash_amd.rotary import Rotary, _rotary_of, rotary_frequencies
+
+
+def through_pickle(thing):
+    return pickle.loads(pickle.dumps(thing))
+
+
+def through_save(thing):
+    file = io.BytesIO()
+    torch.save(thing, file)
+    file.seek(0)
+    return torch.load(file, weights_only=False)
+
+
+COPIES = [copy.copy, copy.deepcopy, through_pickle, through_save]
+
+
+class Holder(torch.nn.Module):
+    def __init__(self, thing):
+        super().__init__()
+        self.thing = thing
+
+
+@pytest.mark.parametrize("made", COPIES, ids=lambda f: f.__name__)
+@pytest.mark.parametrize("kwargs", [{}, dict(layout="interleaved", magnitude=1.25), dict(axes=[0, 1, 2, 0] * 8)], ids=str)
+def test_rotary(made, kwargs):
+    one = Rotary(rotary_frequencies(64), device="cpu", **kwargs)
+    for two in (made(one), made(Holder(one)).thing):
+        assert type(two) is Rotary and (made is copy.copy) == (two.phases is one.phases)
+        for name in Rotary.__slots__:
+            a, b = getattr(one, name), getattr(two, name)
+            assert type(a) is type(b) and (torch.equal(a, b) if isinstance(a, torch.Tensor) else a == b), name
+        with pytest.raises(AttributeError, match="made of"):
+            two.pairs = 1 << 20
+
+
+def test_rotary_of_other_parts_is_refused():
+    phases = torch.arange(4)
+    for parts in ((phases[:0], None, 1, False, 1.0), (phases.int(), None, 1, False, 1.0), (phases[::2], None, 1, False, 1.0),
+                  (phases, phases[:3], 2, False, 1.0), (phases, None, 2, False, 1.0), (phases, phases, 65, False, 1.0),
+                  (phases, None, 1, False, float("inf")), (phases[None], None, 1, False, 1.0)):
+        with pytest.raises(ValueError, match="rotary"):
+            _rotary_of(Rotary, *parts)

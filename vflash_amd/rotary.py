@@ -95,12 +95,31 @@ class Rotary:
             if count > 1:
                 axis = torch.tensor(axes, dtype=torch.int64, device=device)
         phases = torch.tensor([_phase(f) for f in frequencies], dtype=torch.int64, device=device)
-        for name, value in (("phases", phases), ("pairs", len(frequencies)), ("interleaved", layout == "interleaved"),
-                            ("magnitude", float(magnitude)), ("axis", axis), ("axes", count)):
+        self._keep(phases, axis, count, layout == "interleaved", float(magnitude))
+
+    def _keep(self, phases, axis, axes, interleaved, magnitude):
+        for name, value in (("phases", phases), ("pairs", phases.numel()), ("interleaved", interleaved),
+                            ("magnitude", magnitude), ("axis", axis), ("axes", axes)):
             object.__setattr__(self, name, value)
 
     def __setattr__(self, name, value):
         raise AttributeError("rotary positions keep what they were made of")
+
+    def __reduce__(self):
+        return _rotary_of, (type(self), self.phases, self.axis, self.axes, self.interleaved, self.magnitude)
+
+
+def _rotary_of(cls, phases, axis, axes, interleaved, magnitude):
+    """What ``copy`` and ``pickle`` make of the parts that another was kept in."""
+    for t in (phases, axis):
+        if t is not None and (t.dtype != torch.int64 or t.shape != (max(phases.numel(), 1),) or not t.is_contiguous()
+                              or t.device != phases.device):
+            raise ValueError("rotary phases and axes are int64 vectors of one length")
+    if not 1 <= axes <= 64 or (axes == 1) != (axis is None) or not abs(magnitude) <= 3.39e38:
+        raise ValueError("rotary positions of unknown parts")
+    rotary = cls.__new__(cls)
+    rotary._keep(phases, axis, int(axes), bool(interleaved), float(magnitude))
+    return rotary
 
 
 def rotate(q, k, positions, rotary: Rotary):
