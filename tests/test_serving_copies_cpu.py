@@ -7,6 +7,7 @@ import pickle
 import pytest
 import torch
 
+from vflash_amd.paged import PagedCache
 from vflash_amd.rotary import Rotary, _rotary_of, rotary_frequencies
 
 
@@ -50,3 +51,20 @@ def test_rotary_of_other_parts_is_refused():
                   (phases, None, 1, False, float("inf")), (phases[None], None, 1, False, 1.0)):
         with pytest.raises(ValueError, match="rotary"):
             _rotary_of(Rotary, *parts)
+
+
+@pytest.mark.parametrize("made", COPIES, ids=lambda f: f.__name__)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float8_e4m3fn], ids=str)
+def test_paged_cache(made, dtype):
+    one = PagedCache.zeros(3, 16, 2, 64, dtype, device="cpu")
+    one.values.view(torch.uint8).copy_(torch.randint(0, 100, (*one.values.view(torch.uint8).shape,)))
+    if one.scales is not None:
+        one.scales.uniform_()
+    for two in (made(one), made(Holder(one)).thing):
+        assert type(two) is PagedCache and two.values.dtype == dtype
+        assert torch.equal(two.values.view(torch.uint8), one.values.view(torch.uint8))
+        assert two.scales is None if one.scales is None else torch.equal(two.scales, one.scales)
+        # A shallow copy is another view of the same pages, the others are pages of their own.
+        assert (made is copy.copy) == (two.values.data_ptr() == one.values.data_ptr())
+        with pytest.raises(AttributeError, match="made of"):
+            two.values = one.values

@@ -55,6 +55,11 @@ class PagedCache:
     def __setattr__(self, name, value):
         raise AttributeError("a paged cache keeps the tensors that it was made of")
 
+    def __reduce__(self):
+        # As bytes where they are codes: pickle has no name for torch's storage of these.
+        values = self.values if self.scales is None else self.values.view(torch.uint8)
+        return _cache_of, (type(self), values, self.scales)
+
     @classmethod
     def zeros(cls, pages, page, key_heads, dim, dtype=torch.bfloat16, device="cuda"):
         """An empty cache."""
@@ -63,6 +68,11 @@ class PagedCache:
         if dtype == torch.float8_e4m3fn:
             scales = torch.ones((pages, 2, key_heads, page), dtype=torch.float32, device=device)
         return cls(values, scales)
+
+
+def _cache_of(cls, values, scales):
+    """What ``copy`` and ``pickle`` make of another's tensors, which are checked as those were."""
+    return cls(values if scales is None else values.view(torch.float8_e4m3fn), scales)
 
 
 def _plain(t):
