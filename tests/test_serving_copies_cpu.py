@@ -7,6 +7,8 @@ import pickle
 import pytest
 import torch
 
+from vflash_amd.adapters import RequestAdapters, stack_request_adapters
+from vflash_amd.fused import LowRankResidual
 from vflash_amd.paged import PagedCache
 from vflash_amd.rotary import Rotary, _rotary_of, rotary_frequencies
 
@@ -68,3 +70,16 @@ def test_paged_cache(made, dtype):
         assert (made is copy.copy) == (two.values.data_ptr() == one.values.data_ptr())
         with pytest.raises(AttributeError, match="made of"):
             two.values = one.values
+
+
+@pytest.mark.parametrize("made", COPIES, ids=lambda f: f.__name__)
+def test_request_adapters(made):
+    g = torch.Generator().manual_seed(3)
+    pack = [tuple(LowRankResidual(torch.randn((r, 32), generator=g), torch.randn((n, r), generator=g), 0.5) for n in (48, 16))
+            for r in (3, 20)]
+    one = stack_request_adapters(pack, 32, (48, 16), device="cpu")
+    for two in (made(one), made(Holder(one)).thing):
+        assert type(two) is RequestAdapters and two.widths == (48, 16) and list(two.c_widths) == [48, 16]
+        for name in ("down", "up", "scaling", "ranks"):
+            assert torch.equal(getattr(two, name), getattr(one, name))
+            assert (made is copy.copy) == (getattr(two, name).data_ptr() == getattr(one, name).data_ptr())

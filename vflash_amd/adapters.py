@@ -64,6 +64,9 @@ class RequestAdapters:
         object.__setattr__(self, "widths", widths)
         object.__setattr__(self, "c_widths", (ctypes.c_int64 * len(widths))(*widths))
 
+    def __reduce__(self):  # copy and pickle: c_widths is made again, and the tensors are checked as these were
+        return type(self), (self.down, self.up, self.scaling, self.ranks, self.widths)
+
 
 def stack_request_adapters(adapters, k: int, widths, *, dtype=torch.bfloat16, device="cuda") -> RequestAdapters:
     """``RequestAdapters`` of a list of adapters, each a ``LowRankResidual`` or, for merged branches, a tuple with
