@@ -43,17 +43,26 @@ __device__ __forceinline__ uint32_t quant1(float x, float scale) {
 // makes the row kernels instruction-bound.  The divisor is fixed per row, so
 // rows with 2^-72 <= s <= FLT_MAX use Markstein's correction on the correctly
 // rounded reciprocal y = RN(1/s), formed once per row:
-//   q0 = RN(x y),  r = x - q0 s (exact, one fma),  q = RN(q0 + r y).
+//   q0 = RN(x y),  r = RN(x - q0 s) (one fma),  q = RN(q0 + r y).
 // The residual is formed negated, r' = RN(q0 s - x) = -r, and the correction
 // as RN(q0 + r' (-y)): the same value (RN is symmetric) with the sign of a
-// zero quotient right (x = -0 gives -0), at no extra instruction.  For every
-// bf16 x with |x| <= amax,
-// the E4M3 code of clamp(q) equals that of clamp(x / s): an exhaustive check
-// over all pairs of bf16 values finds the first disagreement at amax near
-// 2^-104.7, in rows whose residual underflows, far below the bound here
-// (s >= 2^-72 means amax > 2^-64).  Rows outside the bound, including
-// non-finite scales, divide exactly.  The on-device probe
-// tests/probes/row_division.hip repeats the comparison on the GPU.
+// zero quotient right (x = -0 gives -0), at no extra instruction.  The E4M3
+// code of clamp(q) equals that of clamp(x / s) for every binary32 x with
+// |x| <= amax (the paged append's rotated keys are unrounded):
+// with s in [1, 2), q0 + r y is off x / s by (x / s - q0)(1 - s y) and r's
+// rounding (r takes a 25th bit where q0 is more than a unit off), below 2^-45.
+// So q and RN(x / s) differ only where x / s lies that near a midpoint of
+// binary32, and their codes only where that is next to a midpoint B of E4M3, of
+// five bits: x = (B +- ulp / 2) s up to 2^-44.  x - B s is a whole number of
+// 2^-27 (quotients from 1 on; 2^-28 below), which brings s within 9 units of a
+// multiple of 1/8.  These few x and s, compared one by one, all have the exact quotient
+// (tests/test_row_division_cpu.py); 2e9 random pairs show none that has not.
+// Nothing underflows: |x / s| < 2^-11 has the code of zero either way, and else
+// r is a whole number of 2^-129.  For bf16 x an exhaustive check over all pairs of
+// values finds the first disagreement at amax near 2^-104.7, far below the
+// bound here (s >= 2^-72 means amax > 2^-64); the on-device probe
+// tests/probes/row_division.hip repeats it on the GPU.  Rows outside the bound,
+// including non-finite scales, divide exactly.
 struct RowDivisor {
   float s, y;
   bool fast;  // uniform over the wave: the scale and the row maximum must be

@@ -26,7 +26,7 @@ namespace {
 constexpr int RT_THREADS = 64;
 constexpr int RT_PAIRS = 128;  // at most
 
-// row_divisor for heads that share a wave: fast where all of them are.
+// row_divisor for heads that share a wave: fast where all of them are (either way gives the same codes).
 __device__ __forceinline__ RowDivisor heads_divisor(float s, float amax) {
   RowDivisor d{s, 1.0f / s, false};
   d.fast = __builtin_amdgcn_ballot_w64(!(amax <= 3.40282347e38f && s >= 0x1p-72f && s <= 3.40282347e38f)) == 0;
