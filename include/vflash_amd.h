@@ -487,7 +487,8 @@ int vflash_packed_attention(const void* q, int64_t q_ts, int64_t q_hs, const voi
  *   k      the same with key_heads, or NULL (then k_out is not used)
  *   phases uint64 [pairs]: pair i turns by phases[i] 2^-64 of a turn a position (modulo one turn)
  *   axis   int64 [pairs]: which of the token's positions pair i follows, or NULL (the first); outside [0, axes): none
- *   positions int64 [tokens, axes], any value
+ *   positions int64 [tokens, axes], any value; position * phases modulo 2^64 is not rounded before its upper 32 bits are
+ *             taken, so an angle is off by what the caller's phases are, times the position, and by 2^-33 of a turn
  *   pair i is the elements 2 i and 2 i + 1 (interleaved) or i and i + pairs; elements past 2 pairs are copied
  *   (a, b) -> magnitude (a cos - b sin, a sin + b cos), in binary32 with one rounding
  *   q_out, k_out  contiguous, apart from the inputs

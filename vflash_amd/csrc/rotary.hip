@@ -5,9 +5,10 @@
 // in binary32 with one rounding.  Pair i is (2 i, 2 i + 1) of the head (interleaved) or (i, i + pairs) (half);
 // what lies past 2 pairs is copied.
 //
-// The angle is never a rounded product: f is held as turns in 2^-64, so that position * f modulo one turn is
-// a 64-bit integer product, right for every 64-bit position, and its upper 32 bits are the phase (2^-33 of a turn
-// off at most, 7e-10 rad).  No table of cosines is read.
+// The angle is never a rounded product: f is held as turns, rounded to 2^-64, so that position * f modulo one turn is
+// a 64-bit integer product without a rounding of its own, and its upper 32 bits are the phase.  Against the
+// frequency itself it is 2^-33 + |position| 2^-65 of a turn off at most: 7e-10 rad, twice that at positions of 2^32,
+// 1.9e-7 rad at 2^40.  No table of cosines is read.
 //
 // Bound by the copy: each value is read and written once.  A workgroup is one wave and takes one token, whose sines and
 // cosines it forms once in LDS, a lane a pair, for all heads.  What counts is how many tokens are on their way: 32

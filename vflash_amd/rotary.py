@@ -5,8 +5,8 @@ and attention.
 they follow), ``rotate`` applies it to queries and keys in one launch, and
 ``paged.paged_append`` does so on the way into a paged cache.  The reference rotates split
 halves by a table of cosines (src/vflash/native/h3_fused_ops.py:428-507); here the
-angles are formed in the kernel from integers, exactly for every position, and no
-table is read.
+angles are formed in the kernel from integers, and no table is read.  An angle is off by
+``2 ** -33 + abs(position) * 2 ** -65`` of a turn at most: 1.5e-9 rad up to position ``2 ** 32``.
 """
 
 from __future__ import annotations
@@ -57,7 +57,8 @@ def rotary_frequencies(dim: int, base: float = 10000.0, *, scaling: str | None =
 
 
 def _phase(frequency: float) -> int:
-    """Turns a position in 2^-64, modulo one turn, as a signed 64-bit word: to nearest, in integers."""
+    """Turns a position in 2^-64, modulo one turn, as a signed 64-bit word: to nearest, in integers, so that
+    ``position`` of them are ``abs(position) * 2 ** -65`` of a turn off at most."""
     n, d = frequency.as_integer_ratio()  # d is a power of two
     shift = 135 + d.bit_length()  # 200 - 64 + log2(d)
     turns = (n * _PER_TURN + (1 << (shift - 1)) >> shift) + 2**63
@@ -129,7 +130,7 @@ def rotate(q, k, positions, rotary: Rotary):
     type; ``dim`` is a multiple of 8 up to 256 that holds the pairs.  Any strides are taken
     (slices of a merged projection); a layout whose rows are not 16-byte runs is copied
     first.  ``positions`` is int64 ``[tokens]``, or ``[tokens, axes]`` where the pairs follow
-    several, of any values (a negative position turns back).
+    several, of any values (a negative position turns back); angles lose bits past ``2 ** 32``, as above.
 
     ``(a, b)`` becomes ``magnitude (a cos - b sin, a sin + b cos)`` in binary32, rounded once.  Inference only.
     """
