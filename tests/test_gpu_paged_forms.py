@@ -10,6 +10,7 @@ import torch
 
 from tests.attention_reference import packed_attention
 from tests.test_gpu_paged import attended, make, offsets, pool, rows_of
+from vflash_amd import attention
 from vflash_amd.paged import PagedCache, paged_attention
 
 pytestmark = pytest.mark.gpu
@@ -183,3 +184,18 @@ def test_a_captured_call_replays_other_lengths_and_pages(dev, form, dtype, store
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, paged_attention(q, cache, table, n, q_offsets=qo)), turn
+
+
+@pytest.mark.parametrize("lengths,heads,kv", [([700, 2000, 33, 5000], 32, 8), ([500, 30, 7], 8, 2), ([300] * 70, 16, 8)])
+def test_packed_attention_over_the_same_keys(dev, lengths, heads, kv):
+    # The two forms see different room, so that they may split, scale weights and sum differently: each is within the
+    # definition's bound, and their difference within twice that.
+    cache, table = pool(dev, lengths, 64, kv, 128, BF16)
+    q, qo, ko = make(dev, len(lengths), heads, 128, std=2.0), torch.arange(len(lengths) + 1), offsets(lengths, "cpu")
+    got = paged_attention(q, cache, table, torch.tensor(lengths, device=dev))
+    k, v = (x.to(BF16) for x in rows_of(cache, table, lengths))
+    contiguous = attention.packed_attention(q, k.to(dev), v.to(dev), qo.to(dev), ko.to(dev), causal=True)
+    want, bound = packed_attention(q, k, v, qo, ko, causal=True)
+    for out in (got, contiguous):
+        assert bool(((out.cpu().double() - want).abs() <= bound).all())
+    assert bool(((got.double() - contiguous.double()).abs().cpu() <= 2 * bound).all())
