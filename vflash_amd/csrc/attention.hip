@@ -76,6 +76,14 @@ __global__ void __launch_bounds__(64 * WAVES, (DP <= 64 ? 4 : 3) - (STORE == kSt
   const int open = min(attention_limit(p, it.seq, wave_first_token), last);
   const int end = min(attention_limit(p, it.seq, wave_last_token), last);
 
+  const uint8_t *kb = nullptr, *vb = nullptr;  // rows: of this sequence and key head
+  uint32_t kts = (uint32_t)p.dim * 2, vts = kts;  // bytes of a row
+  if constexpr (!PAGED) {
+    kb = reinterpret_cast<const uint8_t*>(p.k + (int64_t)it.seq.k0 * p.k_ts + (int64_t)part_head * p.k_hs);
+    vb = reinterpret_cast<const uint8_t*>(p.v + (int64_t)it.seq.k0 * p.v_ts + (int64_t)part_head * p.v_hs);
+    kts = (uint32_t)p.k_ts * 2;
+    vts = (uint32_t)p.v_ts * 2;
+  }
   // DMA: block i of this wave holds rows (wave * BLOCKS + i) * ROWS + lane / CHUNKS; lane l fills
   // slot l % CHUNKS.  Rows past the keys and chunks past the head read as zeros.
   constexpr int WAVE_ROWS = BLOCKS * L::ROWS;
@@ -99,23 +107,16 @@ __global__ void __launch_bounds__(64 * WAVES, (DP <= 64 ? 4 : 3) - (STORE == kSt
   auto issue = [&](int buf, int key0, int64_t page) {
     const int left = last - key0;
     const uint32_t dst = base_lds + buf * L::SLOT + wave * BLOCKS * 1024;
-    uint32_t kts, vts, from;  // bytes of a row; the first row of the resources
+    const uint32_t from = PAGED ? (uint32_t)group : 0;  // the first row of the resources
     __amdgpu_buffer_rsrc_t rk, rv;
     if constexpr (PAGED) {
       const bool none = (uint64_t)page >= (uint64_t)p.cache.pages;  // reads zeros
       const uint8_t* at = p.cache.values + (none ? 0 : cache_row(page, key0 + group) * p.dim * 2);
       rk = make_rsrc(at, none ? 0 : 0x7fffffffu);
       rv = make_rsrc(at + head_rows * p.dim * 2, none ? 0 : 0x7fffffffu);
-      kts = vts = (uint32_t)p.dim * 2;
-      from = (uint32_t)group;
     } else {
-      kts = (uint32_t)p.k_ts * 2;
-      vts = (uint32_t)p.v_ts * 2;
-      from = 0;
-      rk = make_rsrc(reinterpret_cast<const uint8_t*>(p.k + (int64_t)it.seq.k0 * p.k_ts + (int64_t)part_head * p.k_hs) +
-                         (int64_t)key0 * kts, 0x7fffffffu);
-      rv = make_rsrc(reinterpret_cast<const uint8_t*>(p.v + (int64_t)it.seq.k0 * p.v_ts + (int64_t)part_head * p.v_hs) +
-                         (int64_t)key0 * vts, 0x7fffffffu);
+      rk = make_rsrc(kb + (int64_t)key0 * kts, 0x7fffffffu);
+      rv = make_rsrc(vb + (int64_t)key0 * vts, 0x7fffffffu);
     }
     static_for<BLOCKS>([&](auto i) {
       const int r = drow + i * L::ROWS;

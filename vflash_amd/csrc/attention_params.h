@@ -25,7 +25,6 @@ struct AttentionParams {
   uint16_t* out;
   int64_t q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, o_ts, o_hs;
   const int64_t *q_offsets, *k_offsets, *k_lengths;  // k_lengths: or null
-  PagedCacheParams cache;  // pages: these instead of k, v, k_offsets and k_lengths; q_offsets may be null
   int tokens, keys;  // rows; pages: the most that a sequence has
   int64_t batch;
   int heads, group, dim;  // group: query heads of a key head
@@ -41,11 +40,13 @@ struct AttentionParams {
   // Splitting of the keys, off where target is 0.
   int target, min_chunk;  // items, blocks of 64 keys
   int64_t slots;          // what the workspace holds
-  uint32_t least_units;  // of a workgroup of a paged call
   int unit_shift;  // attention_step: log2 of a unit's keys (31: a whole sequence)
   float* part;  // [slot][row][d], then [slot][row] maxima and sums
   float* part_ml;
-  int32_t* begun;  // [workgroup][4], of a paged call: AttentionBegun
+  // Of a call over pages, last: the loads of the others' arguments stay as wide as they are.
+  PagedCacheParams cache;  // these instead of k, v, k_offsets and k_lengths; q_offsets may be null
+  uint32_t least_units;    // of a workgroup
+  int32_t* begun;          // [workgroup][4]: AttentionBegun
 };
 
 }  // namespace vfa

@@ -106,6 +106,14 @@ __global__ void __launch_bounds__(64 * W, STORE == kStoreE4M3 && DP <= 64 ? 4 : 
     const int open = min(attention_limit(p, it.seq, min(it.tile * p.tile_tokens, it.seq.nq)), last);
 
     const int drow = lane / L::CHUNKS, dslot = lane % L::CHUNKS;
+    const uint8_t *kb = nullptr, *vb = nullptr;  // rows: of this sequence and key head
+    uint32_t kts = 0, vts = 0;
+    if constexpr (!PAGED) {
+      kb = reinterpret_cast<const uint8_t*>(p.k + (int64_t)it.seq.k0 * p.k_ts + (int64_t)key_head * p.k_hs);
+      vb = reinterpret_cast<const uint8_t*>(p.v + (int64_t)it.seq.k0 * p.v_ts + (int64_t)key_head * p.v_hs);
+      kts = (uint32_t)p.k_ts * 2;
+      vts = (uint32_t)p.v_ts * 2;
+    }
     struct Halves {
       int64_t page[2];
     };
@@ -125,9 +133,6 @@ __global__ void __launch_bounds__(64 * W, STORE == kStoreE4M3 && DP <= 64 ? 4 : 
       const int left = last - key0;  // none: every lane reads zeros
       const uint32_t dst = ring_lds + buf * L::SLOT;
       if constexpr (!PAGED) {
-        const uint8_t* kb = reinterpret_cast<const uint8_t*>(p.k + (int64_t)it.seq.k0 * p.k_ts + (int64_t)key_head * p.k_hs);
-        const uint8_t* vb = reinterpret_cast<const uint8_t*>(p.v + (int64_t)it.seq.k0 * p.v_ts + (int64_t)key_head * p.v_hs);
-        const uint32_t kts = (uint32_t)p.k_ts * 2, vts = (uint32_t)p.v_ts * 2;
         const __amdgpu_buffer_rsrc_t rk = make_rsrc(kb + (int64_t)key0 * kts, 0x7fffffffu);
         const __amdgpu_buffer_rsrc_t rv = make_rsrc(vb + (int64_t)key0 * vts, 0x7fffffffu);
         static_for<L::TILE / 1024>([&](auto i) {
@@ -279,30 +284,32 @@ __global__ void __launch_bounds__(64 * W, STORE == kStoreE4M3 && DP <= 64 ? 4 : 
     __syncthreads();
     // Thread t: row t / 16 (and those 4 WAVES further), the d of t % 16 in runs of four.
     const int e = (int)threadIdx.x & 15;
-    static_for<4 / L::WAVES>([&](auto turn) {
+#pragma unroll
+    for (int turn = 0; turn < 4 / L::WAVES; ++turn) {
       const int r = ((int)threadIdx.x >> 4) + turn * (4 * L::WAVES);
       const AttentionRow mine = attention_row(p, it, r);
-      if (!mine.live) return;
-      float top = stat[0][r][0], sum = 0, f[L::WAVES];
-      static_for<L::WAVES - 1>([&](auto w) { top = fmaxf(top, stat[w + 1][r][0]); });
-      static_for<L::WAVES>([&](auto w) {
-        f[w] = __builtin_amdgcn_exp2f(stat[w][r][0] - top);
-        sum += f[w] * stat[w][r][1];
-      });
-      const bool whole = seg.count == seg.of;
-      const int64_t at = (2 * (int64_t)blockIdx.x + (seg.first == 0)) * 16 + r;
-      if (!whole && e == 0) *reinterpret_cast<v2f*>(p.part_ml + at * 2) = v2f{top, sum};
-      const float inv = whole ? 1.0f / sum : 1.0f;
-      uint16_t* dst = p.out + (int64_t)(it.seq.q0 + mine.token) * p.o_ts + (int64_t)mine.head * p.o_hs;
-      for (int d = 4 * e; d < p.dim; d += 64) {
-        v4f x = v4f{};
-        static_for<L::WAVES>(
-            [&](auto w) { x += *reinterpret_cast<const v4f*>(lds + (w * 16 + r) * L::ACC + d * 4) * f[w]; });
-        x = sum == 0 ? v4f{} : x * inv;
-        if (whole) *reinterpret_cast<v2i*>(dst + d) = v2i{pack2<F16>(x[0], x[1]), pack2<F16>(x[2], x[3])};
-        else *reinterpret_cast<v4f*>(p.part + at * p.dim + d) = x;
+      if (mine.live) {
+        float top = stat[0][r][0], sum = 0, f[L::WAVES];
+        static_for<L::WAVES - 1>([&](auto w) { top = fmaxf(top, stat[w + 1][r][0]); });
+        static_for<L::WAVES>([&](auto w) {
+          f[w] = __builtin_amdgcn_exp2f(stat[w][r][0] - top);
+          sum += f[w] * stat[w][r][1];
+        });
+        const bool whole = seg.count == seg.of;
+        const int64_t at = (2 * (int64_t)blockIdx.x + (seg.first == 0)) * 16 + r;
+        if (!whole && e == 0) *reinterpret_cast<v2f*>(p.part_ml + at * 2) = v2f{top, sum};
+        const float inv = whole ? 1.0f / sum : 1.0f;
+        uint16_t* dst = p.out + (int64_t)(it.seq.q0 + mine.token) * p.o_ts + (int64_t)mine.head * p.o_hs;
+        for (int d = 4 * e; d < p.dim; d += 64) {
+          v4f x = v4f{};
+          static_for<L::WAVES>(
+              [&](auto w) { x += *reinterpret_cast<const v4f*>(lds + (w * 16 + r) * L::ACC + d * 4) * f[w]; });
+          x = sum == 0 ? v4f{} : x * inv;
+          if (whole) *reinterpret_cast<v2i*>(dst + d) = v2i{pack2<F16>(x[0], x[1]), pack2<F16>(x[2], x[3])};
+          else *reinterpret_cast<v4f*>(p.part + at * p.dim + d) = x;
+        }
       }
-    });
+    }
     pos += seg.count;
     if (pos < stop) __syncthreads();  // the sums are read: the rings may be filled again
   }
