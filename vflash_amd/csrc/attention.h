@@ -45,9 +45,10 @@ template <bool FAR>
 __device__ __forceinline__ float attention_weight(float s, float c, float m, float ref, float shift) {
   return __builtin_amdgcn_exp2f(FAR ? (s - m) * c + shift : __builtin_fmaf(s, c, ref));
 }
-// l plus the two weights of a packed pair, as they were rounded: the sum that normalises them, in
-// every kernel, so that what their roundings have in common cancels (a value that all keys share
-// comes back as it is).
+// l plus the two weights of a packed pair, as they were rounded: the sum that normalises them
+// over values in the operands' type, so that what their roundings have in common cancels (a value that
+// all keys share comes back as it is).  Over E4M3 pages a weight is rounded with its value's factor, and the
+// sum is that of the unrounded weights: errors against 64 bits are 1.4 times those of weights in 32 bits.
 template <bool F16>
 __device__ __forceinline__ float attention_sum2(int pair, float l) {
   if constexpr (F16)

@@ -5,11 +5,13 @@
 // where K position (lane row g, j) stands for key 4 g + j of the first 16 keys (j < 4) or
 // 4 g + j - 4 of the second, which is where the scores lie.
 //
-// Each wave takes every fourth block of 32 keys of the item and keeps a ring of two in LDS, which
-// its own DMA fills: 128 KB a CU in flight or in use, no barrier before the end, where the four
-// waves' sums are added up.  131071 keys of 8 heads of 128: 107 us, 5.0 TB/s, what a copy of 1 GiB
-// reaches; 16 sequences of up to 8191: 65 us, 4.2 TB/s; 77 keys: 7.5 us a call, a chain of loads, search
-// and sums in one wave after another.
+// Each of a workgroup's W waves takes every W-th block of 32 keys of the item and keeps a ring of NS blocks in
+// LDS, which its own DMA fills: no barrier before the end, where the waves' sums are added up.  W is 4 over
+// rows and wherever keys are split, 2 or 1 for many whole sequences over pages (the plan says which); NS is 2, but 1 for
+// single waves of what is not E4M3 at dimension 128: these have one block each on its way, and overlap loads and
+// products across the workgroups of a CU alone.  Four waves of two blocks of 16 bits hold 128 KB a CU in flight or in
+// use: 131071 keys of 8 heads of 128 107 us, 5.0 TB/s, what a copy of 1 GiB reaches; 16 sequences of up
+// to 8191: 63 us, 4.4 TB/s; 77 keys: 7.7 us a call, a chain of loads, search and sums in one wave after another.
 //
 // A paged cache differs in where a block's keys come from: each 16 lie in one page, whose number a scalar
 // load fetches one block ahead.  E4M3 codes go to LDS as they are, with their factors, and become 16 bits between

@@ -159,6 +159,11 @@ def paged_attention(q, cache: PagedCache, table, lengths, *, q_offsets=None, sca
     tiles of 128, as in ``packed_attention``.  Softmax and sums are binary32; weights are rounded to the operands'
     type; with an E4M3 cache to bf16 after the values' scales, for f16 queries to two bf16.  As there, infinities and
     NaN in the values of a sequence can reach its masked queries as NaN.  Inference only.
+
+    The lengths stay on the device, so the launch is chosen by the table's room (its width times the page) in their
+    place.  Pass a table as wide as the longest sequence needs where that is known (``table[:, :n].contiguous()``): 77 keys
+    take 7.2 us in a room of 77 and 10.6 in one of 2048 or more, 128 single tokens over 200 keys 22 and 35, five drafts
+    after 500 11.5 and, in a room of 131072, 20.8.  A captured step keeps the room that it was captured with.
     """
     if isinstance(q, torch.Tensor) and q.is_cuda and isinstance(cache, PagedCache):
         host = _lib.host()
