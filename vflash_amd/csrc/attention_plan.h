@@ -75,7 +75,7 @@ inline bool attention_few_rows(const AttentionParams& p) {
 
 // Over a paged cache, in tiles of 16 or 128 as packed attention is.  For tiles of 16 a sequence's room stands for its
 // length, which varies: the keys are split from 768 where the tiles leave half of the workgroups idle, and else from
-// 1536.  Equal lengths, us whole and split, 32 heads over 8 of dimension 128 in bf16 and E4M3, and of 64 in bf16: one of
+// 1536.  Equal lengths that fill their room, us whole and split, 32 heads over 8 of dimension 128 in bf16 and E4M3, and of 64 in bf16: one of
 // 500 keys 11.4 12.0, 10.2 11.4, 8.1 10.4; of 1000 16.3 12.3, 14.5 11.8, 10.7 10.9; of 2000 25.9 13.5, 22.7 12.9, 16.2
 // 11.9; 16 of 1000 18.6 21.5, 15.6 18.2, 11.9 15.6; 16 of 2000 33.0 34.7, 24.4 22.0, 17.8 19.7; 32 of 2000 51.9 54.5,
 // 29.9 34.5, 27.0 31.5.  E4M3 tiles take half the LDS, and two workgroups where bf16 has one: 61 sequences of 1 to 8191
